@@ -25,7 +25,9 @@ from . import _native
 from ._native import PyxisError, QTYPE_BF16, QTYPE_F32, QTYPE_INT4, QTYPE_INT8, DTYPE_BF16, DTYPE_F32, check
 
 __all__ = ["Weights", "CudaMatmul", "get_cuda", "matmul", "matmul_batch", "matmul_dev", "argmax",
-           "argmax_dev", "PyxisError", "synth_normal_f32", "synth_normal_bf16", "synth_tokens"]
+           "argmax_dev", "sample_dev", "rope_frequencies", "qk_norm_rope_dev", "tree_attention_dev",
+           "kv_copy_pages_dev", "kv_compact_dev", "PagePool", "PyxisError", "synth_normal_f32", "synth_normal_bf16",
+           "synth_tokens"]
 
 INT4_BLOCK_SIZE = 32  # src/model.rs:20
 
@@ -378,3 +380,8 @@ def synth_tokens(seed: int, n: int, vocab: int) -> np.ndarray:
     out = np.empty(n, dtype=np.int32)
     _native.lib().pyxis_synth_tokens(seed, n, vocab, out.ctypes.data_as(C.c_void_p))
     return out
+
+
+# -- a decoding step over a paged cache (include/pyxis_serve.h) -------------------------------------
+from .serve import (PagePool, kv_compact_dev, kv_copy_pages_dev, qk_norm_rope_dev, rope_frequencies,  # noqa: E402
+                    sample_dev, tree_attention_dev)

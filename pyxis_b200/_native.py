@@ -1,5 +1,5 @@
 """ctypes binding of libpyxis_cuda.so (include/pyxis_cuda.h, pyxis_decode.h, pyxis_comm.h,
-include/pyxis_synth.h).
+pyxis_serve.h, include/pyxis_synth.h).
 
 The library is built in-tree by ``pyxis_b200.build``.  There is no fallback: if the shared
 library is missing or cannot be loaded, importing the CUDA path raises.
@@ -72,6 +72,14 @@ SIGNATURES = {
     "pyxis_cuda_head_greedy_dev": (C.c_int, [_vp, _vp, _sz, _sz, _sz, _sz, _vp, _sz, _sz, _vp, _vp]),
     "pyxis_cuda_head_reserve": (C.c_int, [_vp, _sz, _sz]),
     "pyxis_cuda_model_set_vocab_parallel": (C.c_int, [_vp, _vp, _vp, _sz, _sz]),
+    "pyxis_rope_frequencies": (C.c_int, [C.c_int, C.c_double, C.c_int, C.c_double, C.c_double, C.c_double, C.c_double,
+                                         _vp, _vp]),
+    "pyxis_cuda_qk_norm_rope_dev": (C.c_int, [_vp, _vp, _vp, _vp]),
+    "pyxis_cuda_tree_attention_dev": (C.c_int, [_vp, _vp, _vp, _vp, _sz, _vp]),
+    "pyxis_cuda_tree_attention_workspace_size": (_sz, [_vp, _vp, _vp]),
+    "pyxis_cuda_kv_copy_pages_dev": (C.c_int, [_vp, _vp, _vp, _vp, _sz, _vp]),
+    "pyxis_cuda_kv_compact_dev": (C.c_int, [_vp, _vp, _vp, _sz, _sz, _vp, _vp, _sz, _vp, _vp]),
+    "pyxis_cuda_sample_dev": (C.c_int, [_vp, _vp, C.c_int, _sz, _sz, _sz, _vp, _vp, _vp, _vp, _vp]),
     "pyxis_synth_normal_f32": (None, [C.c_uint64, _sz, C.c_float, _vp]),
     "pyxis_synth_normal_bf16": (None, [C.c_uint64, _sz, C.c_float, _vp]),
     "pyxis_synth_tokens": (None, [C.c_uint64, _sz, C.c_uint32, _vp]),

@@ -139,10 +139,12 @@ constexpr size_t kWsTickets = 16384;  // 128-row tiles: matrices of up to 2M row
 
 int grow_workspace(pyxis_cuda_ctx *ctx, size_t want) {
     if (ctx->ws_cap >= want) return PYXIS_OK;
-    cudaFree(ctx->ws);
-    ctx->ws = nullptr;
-    ctx->ws_cap = 0;
-    PYXIS_CUDA_TRY(cudaMalloc(&ctx->ws, want), "cudaMalloc(workspace)");
+    want = std::max(want, ctx->ws_cap + ctx->ws_cap / 2);  // few steps to any size
+    void *bigger = nullptr;
+    PYXIS_CUDA_TRY(cudaMalloc(&bigger, want), "cudaMalloc(workspace)");
+    // a captured graph may still name the smaller one: it lives as long as the context
+    if (ctx->ws) ctx->ws_retired.push_back(ctx->ws);
+    ctx->ws = bigger;
     ctx->ws_cap = want;
     return PYXIS_OK;
 }
@@ -163,6 +165,10 @@ int ensure_ctx_workspace(pyxis_cuda_ctx *ctx, size_t want, cudaStream_t st) {
 }  // namespace
 
 int pyxis::record_error(int code, const char *msg) { return fail(code, "%s", msg); }
+
+int pyxis::context_workspace(pyxis_cuda_ctx *ctx, size_t bytes, cudaStream_t st) {
+    return ensure_ctx_workspace(ctx, bytes, st);
+}
 
 namespace {
 // Weight-streaming tensor-core matmul for decode-shaped batches of 9-64 tokens (int4 / int8 with
@@ -338,6 +344,7 @@ int pyxis_cuda_destroy(pyxis_cuda_ctx *ctx) {
     cudaFree(ctx->dx);
     cudaFree(ctx->dy);
     cudaFree(ctx->ws);
+    for (void *p : ctx->ws_retired) cudaFree(p);
     cudaFree(ctx->amax_mem);
     cudaFree(ctx->d_err);
     cudaFree(ctx->tcg_scratch);

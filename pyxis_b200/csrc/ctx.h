@@ -6,6 +6,7 @@
 #include <stdint.h>
 
 #include <mutex>
+#include <vector>
 
 #include "argmax.h"
 
@@ -23,6 +24,7 @@ struct pyxis_cuda_ctx {
     // workspace kept for pyxis_cuda_matmul_dev calls that pass none
     void *ws = nullptr;
     size_t ws_cap = 0;
+    std::vector<void *> ws_retired;  // workspaces it outgrew, freed with the context
     // argmax scratch (allocated and zeroed at init)
     pyxis::ArgmaxScratch amax{};
     void *amax_mem = nullptr;
@@ -59,4 +61,7 @@ int run_matmul(pyxis_cuda_ctx *ctx, const pyxis_cuda_weights *w, const float *X,
 bool head_gemv_keys(pyxis_cuda_ctx *ctx, const pyxis_cuda_weights *w, const float *X, size_t M, size_t ldx, size_t N,
                     size_t K, float *Y, size_t ldy, int64_t index_base, uint64_t *keys, cudaStream_t st,
                     cudaError_t *err);
+// Makes ctx->ws hold at least `bytes` for work on `st`, growing it outside stream capture (a
+// pyxis_status; EINVAL while `st` is captured and it would have to grow).
+int context_workspace(pyxis_cuda_ctx *ctx, size_t bytes, cudaStream_t st);
 }  // namespace pyxis

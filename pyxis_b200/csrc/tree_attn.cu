@@ -1,0 +1,467 @@
+// tree_attn.cu -- attention of a tree of drafted tokens over a paged KV cache
+// (src/attention.rs:107-135 with pages, grouped heads and a per-node mask; definition in
+// include/pyxis_serve.h), f32 or bf16, on the CUDA cores in f32.
+//
+//   s_rj = scale q_r . k_j;  m = max_j s_rj;  o_r = sum_j 2^(s_rj - m) v_j / sum_j 2^(s_rj - m)
+//
+// (scores in log2 units).  The rows of one (sequence, kv head) are its nodes times the G query
+// heads that share the kv head, so a key is read once for all of them.  A CTA takes a tile of RT
+// rows and a range of the keys (the host's split); its warps work through the range's 32-key blocks
+// on their own, each with its own shared-memory buffers, running maximum, sum and output, so no
+// barrier stands between the loads of one warp and the arithmetic of another.  The warps' results
+// are joined in shared memory, the splits' by a second kernel.
+//
+// Within a block a lane first is a key: its key row lies in shared memory (rows padded by 16 bytes,
+// so 16-byte reads of 32 rows do not collide), the query rows are broadcast reads.  For P V a lane
+// is HD / 32 columns of the output and the probabilities are broadcast.  Rows arrive by one bulk
+// copy each (an mbarrier per buffer): the next block's keys are under way during P V, its values
+// during Q K.
+#include <cuda_bf16.h>
+
+#include <algorithm>
+#include <atomic>
+
+#include "common.cuh"
+#include "serve.h"
+#include "tc_ptx.cuh"
+
+namespace pyxis {
+namespace {
+
+constexpr int kBlock = 32;  // keys of a warp's block: one per lane
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr uint64_t kTimeoutNs = 2000000000ull;
+enum { kErrLoad = 0x701, kErrDrain = 0x702 };
+
+struct TreeParams {
+    const char *q, *k, *v;
+    char *out;
+    long long q_row, q_head, out_row, out_head;              // bytes
+    long long page_stride, slot_stride, head_stride;         // bytes
+    const int32_t *q_start, *context_len, *block_table;
+    const unsigned long long *tree_mask;
+    long long table_stride, capacity;                        // capacity: positions that a table row names
+    int n_rows, n_q, n_kv, group, page_size, num_pages, max_tree, splits, row_tiles;
+    float scale2;                                            // scale * log2 e
+    float *part_o, *part_ml;                                 // [row][head][split][HD], [..][2] (splits > 1)
+    int *err;
+};
+
+// A sequence's rows and keys, from device memory and clamped to what the buffers hold.
+struct SeqShape {
+    int row0, nodes;
+    long long ctx, total;
+};
+PYXIS_DEVINL SeqShape seq_shape(const TreeParams &p, int seq) {
+    SeqShape s;
+    s.row0 = min(max(p.q_start[seq], 0), p.n_rows);
+    const int end = min(max(p.q_start[seq + 1], s.row0), p.n_rows);
+    s.nodes = min(end - s.row0, p.max_tree);
+    s.ctx = min((long long)max(p.context_len[seq], 0), p.capacity);
+    s.total = min(s.ctx + s.nodes, p.capacity);
+    return s;
+}
+
+PYXIS_DEVINL float redux_max(float v) {
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+}
+
+// Four consecutive elements of a row in shared memory as f32.
+PYXIS_DEVINL float4 ld4(const float *p) { return *reinterpret_cast<const float4 *>(p); }
+PYXIS_DEVINL float4 ld4(const __nv_bfloat16 *p) {
+    const uint2 u = *reinterpret_cast<const uint2 *>(p);
+    return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xFFFF0000u), __uint_as_float(u.y << 16),
+                       __uint_as_float(u.y & 0xFFFF0000u));
+}
+PYXIS_DEVINL float2 ld2(const float *p) { return *reinterpret_cast<const float2 *>(p); }
+PYXIS_DEVINL float2 ld2(const __nv_bfloat16 *p) {
+    const uint32_t u = *reinterpret_cast<const uint32_t *>(p);
+    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u));
+}
+PYXIS_DEVINL float to_f32(float x) { return x; }
+PYXIS_DEVINL float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+PYXIS_DEVINL void store(float *p, float x) { *p = x; }
+PYXIS_DEVINL void store(__nv_bfloat16 *p, float x) { *p = __float2bfloat16_rn(x); }
+
+template <typename T, int HD, int RT>
+struct TreeCfg {
+    static constexpr int kPitch = HD * (int)sizeof(T) + 16;          // bytes of a K or V row in shared memory
+    static constexpr int kHalf = kBlock * kPitch;                    // a warp's K buffer (V follows)
+    static constexpr int kPPitch = kBlock + 4;                       // floats of a row of probabilities
+    static constexpr int kWarpBytes = 2 * kHalf + RT * kPPitch * 4;
+    static constexpr int kQBytes = RT * HD * 4 + RT * 8 + 16;        // q, masks, abort flag
+    static constexpr int kPerWarp = kWarpBytes + RT * 8 + 16;        // and its m and l, mbarriers
+    static constexpr int kFit = (232448 - kQBytes) / kPerWarp;
+    static constexpr int kWarps = kFit < 8 ? kFit : 8;
+    static constexpr int kBytes = kQBytes + kWarps * kPerWarp;
+    static_assert(RT * HD * 4 <= 2 * kHalf, "a warp's output fits its buffers");
+    static_assert(kBytes <= 232448, "227 KB of shared memory per CTA");
+};
+
+template <typename T, int HD, int RT>
+__global__ void __launch_bounds__(TreeCfg<T, HD, RT>::kWarps * 32) tree_attention_kernel(const TreeParams p) {
+    using C = TreeCfg<T, HD, RT>;
+    constexpr int kWarps = C::kWarps, kCols = HD / 32;
+    extern __shared__ __align__(128) unsigned char smem[];
+    float *sq = reinterpret_cast<float *>(smem + kWarps * C::kWarpBytes);  // [RT][HD], times scale2
+    unsigned long long *smask = reinterpret_cast<unsigned long long *>(sq + RT * HD);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smask + RT);  // [kWarps][2]: K, V
+    float *sml = reinterpret_cast<float *>(bars + 2 * kWarps);  // [kWarps][RT][2]: maximum and sum
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(sml + kWarps * RT * 2);
+
+    pdl_wait();
+    pdl_trigger();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int split = blockIdx.x, kvh = blockIdx.y / p.row_tiles, r0 = (blockIdx.y % p.row_tiles) * RT, seq = blockIdx.z;
+    const SeqShape sh = seq_shape(p, seq);
+    const int rows = sh.nodes * p.group - r0;  // of this tile and later ones
+    if (rows <= 0) return;
+    const long long blocks = (sh.total + kBlock - 1) / kBlock;
+    const long long b0 = blocks * split / p.splits, b1 = blocks * (split + 1) / p.splits;
+
+    unsigned char *mine = smem + warp * C::kWarpBytes;
+    T *sk = reinterpret_cast<T *>(mine), *sv = reinterpret_cast<T *>(mine + C::kHalf);
+    float *sp = reinterpret_cast<float *>(mine + 2 * C::kHalf);
+    uint64_t *kbar = bars + 2 * warp, *vbar = kbar + 1;
+    if (lane == 0) {
+        tc::mbar_init(kbar, 1);
+        tc::mbar_init(vbar, 1);
+        tc::fence_mbar_init();
+    }
+    if (threadIdx.x == 0) *abort_flag = 0;
+    for (int i = threadIdx.x; i < RT * HD; i += kWarps * 32) {
+        const int r = i / HD, d = i % HD;
+        float x = 0.f;
+        if (r < rows) {
+            const int t = (r0 + r) / p.group, g = (r0 + r) % p.group;
+            x = p.scale2 * to_f32(*reinterpret_cast<const T *>(p.q + (sh.row0 + t) * p.q_row +
+                                                               (kvh * p.group + g) * p.q_head + d * sizeof(T)));
+        }
+        sq[i] = x;
+    }
+    if (threadIdx.x < RT) {
+        unsigned long long m = 0;
+        if ((int)threadIdx.x < rows) {
+            const int t = (r0 + threadIdx.x) / p.group;
+            m = p.tree_mask ? p.tree_mask[sh.row0 + t] : (2ull << t) - 1;
+        }
+        smask[threadIdx.x] = m;
+    }
+    __syncthreads();
+
+    // row of key `lane` of block b in the cache (bytes), for the bulk copies
+    auto row_offset = [&](long long b) -> long long {
+        const long long pos = b * kBlock + lane, page_i = pos / p.page_size;
+        if (pos >= sh.total) return -1;
+        const int page = min(max(p.block_table[seq * p.table_stride + page_i], 0), p.num_pages - 1);
+        return page * p.page_stride + (pos - page_i * p.page_size) * p.slot_stride + kvh * p.head_stride;
+    };
+    auto load = [&](const char *base, T *dst, uint64_t *bar, long long off) {
+        constexpr uint32_t bytes = HD * sizeof(T);
+        const unsigned valid = __ballot_sync(0xffffffffu, off >= 0);
+        if (lane == 0) tc::mbar_arrive_expect_tx(bar, __popc(valid) * bytes);
+        __syncwarp();
+        if (off >= 0) tc::bulk_load(reinterpret_cast<char *>(dst) + lane * C::kPitch, base + off, bytes, bar);
+    };
+
+    float2 acc[RT][kCols / 2];
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int c = 0; c < kCols / 2; ++c) acc[r][c] = make_float2(0.f, 0.f);
+    float m_run = -INFINITY, l_run = 0.f;  // of row `lane` (lane < RT)
+
+    bool ok = true;
+    uint32_t phase = 0;
+    long long b = b0 + warp;
+    long long off = b < b1 ? row_offset(b) : -1;
+    if (b < b1) {
+        load(p.k, sk, kbar, off);
+        load(p.v, sv, vbar, off);
+    }
+    for (; b < b1 && ok; b += kWarps, phase ^= 1) {
+        const long long next_off = b + kWarps < b1 ? row_offset(b + kWarps) : -1;
+        const long long pos = b * kBlock + lane;
+        ok = __all_sync(0xffffffffu, tc::mbar_wait_bounded(kbar, phase, abort_flag, p.err, kErrLoad, kTimeoutNs));
+        if (!ok) break;
+        // ---- scores: this lane's key against every row
+        float s[RT];
+        {
+            float2 s2[RT];
+#pragma unroll
+            for (int r = 0; r < RT; ++r) s2[r] = make_float2(0.f, 0.f);
+            const T *krow = reinterpret_cast<const T *>(reinterpret_cast<const char *>(sk) + lane * C::kPitch);
+#pragma unroll 4
+            for (int d = 0; d < HD; d += 4) {
+                const float4 kv = ld4(krow + d);
+#pragma unroll
+                for (int r = 0; r < RT; ++r) {
+                    const float4 qv = ld4(sq + r * HD + d);
+                    s2[r] = ffma2(f2(qv.x, qv.y), f2(kv.x, kv.y), s2[r]);
+                    s2[r] = ffma2(f2(qv.z, qv.w), f2(kv.z, kv.w), s2[r]);
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < RT; ++r) s[r] = s2[r].x + s2[r].y;
+        }
+        __syncwarp();
+        if (b + kWarps < b1) load(p.k, sk, kbar, next_off);
+        const bool tail = (b + 1) * kBlock > sh.ctx;  // holds drafts or ends inside
+        if (tail) {
+            const long long draft = pos - sh.ctx;
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                const bool seen = draft < 0 ? true : pos < sh.total && ((smask[r] >> draft) & 1);
+                if (!seen) s[r] = -INFINITY;
+            }
+        }
+        // ---- running maximum, probabilities
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            const float m_old = __shfl_sync(0xffffffffu, m_run, r);
+            const float m_new = fmaxf(m_old, redux_max(s[r]));
+            const float base = m_new == -INFINITY ? 0.f : m_new;  // nothing seen yet: p = 2^-inf = 0
+            if (m_new > m_old) {
+                const float alpha = exp2f(m_old - base);
+#pragma unroll
+                for (int c = 0; c < kCols / 2; ++c) acc[r][c].x *= alpha, acc[r][c].y *= alpha;
+                if (lane == r) l_run *= alpha, m_run = m_new;
+            }
+            sp[r * C::kPPitch + lane] = exp2f(s[r] - base);
+        }
+        __syncwarp();
+        if (lane < RT) {
+            const float *row = sp + lane * C::kPPitch;
+            float sum = 0.f;
+#pragma unroll
+            for (int j = 0; j < kBlock; j += 4) {
+                const float4 x = ld4(row + j);
+                sum += (x.x + x.y) + (x.z + x.w);
+            }
+            l_run += sum;
+        }
+        ok = __all_sync(0xffffffffu, tc::mbar_wait_bounded(vbar, phase, abort_flag, p.err, kErrLoad, kTimeoutNs));
+        if (!ok) break;
+        // ---- O += P V: this lane's columns
+        const int nk = tail ? (int)min((long long)kBlock, sh.total - b * kBlock) : kBlock;
+        if (!tail) {
+#pragma unroll 2
+            for (int j = 0; j < kBlock; j += 4) {
+                float2 v[4][kCols / 2];
+#pragma unroll
+                for (int jj = 0; jj < 4; ++jj) {
+                    const T *vrow = reinterpret_cast<const T *>(reinterpret_cast<const char *>(sv) + (j + jj) * C::kPitch) +
+                                    lane * kCols;
+                    if constexpr (kCols == 4) {
+                        const float4 x = ld4(vrow);
+                        v[jj][0] = f2(x.x, x.y), v[jj][1] = f2(x.z, x.w);
+                    } else {
+                        v[jj][0] = ld2(vrow);
+                    }
+                }
+#pragma unroll
+                for (int r = 0; r < RT; ++r) {
+                    const float4 pr = ld4(sp + r * C::kPPitch + j);
+#pragma unroll
+                    for (int c = 0; c < kCols / 2; ++c) {
+                        acc[r][c] = ffma2(f2(pr.x, pr.x), v[0][c], acc[r][c]);
+                        acc[r][c] = ffma2(f2(pr.y, pr.y), v[1][c], acc[r][c]);
+                        acc[r][c] = ffma2(f2(pr.z, pr.z), v[2][c], acc[r][c]);
+                        acc[r][c] = ffma2(f2(pr.w, pr.w), v[3][c], acc[r][c]);
+                    }
+                }
+            }
+        } else {
+            // a value that a row does not attend to (p = 0) may be anything: it is left out, not
+            // multiplied by zero; so are the rows past the last key, which were never loaded
+            for (int j = 0; j < nk; ++j) {
+                const T *vrow = reinterpret_cast<const T *>(reinterpret_cast<const char *>(sv) + j * C::kPitch) + lane * kCols;
+                float2 v[kCols / 2];
+#pragma unroll
+                for (int c = 0; c < kCols / 2; ++c) v[c] = ld2(vrow + 2 * c);
+#pragma unroll
+                for (int r = 0; r < RT; ++r) {
+                    const float pr = sp[r * C::kPPitch + j];
+                    if (pr != 0.f) {
+#pragma unroll
+                        for (int c = 0; c < kCols / 2; ++c) acc[r][c] = ffma2(f2(pr, pr), v[c], acc[r][c]);
+                    }
+                }
+            }
+        }
+        __syncwarp();
+        if (b + kWarps < b1) load(p.v, sv, vbar, next_off);
+    }
+    if (!ok) {  // a copy did not land in time: give those in flight a last chance before the buffers go
+        volatile int never = 0;
+        tc::mbar_wait_bounded(kbar, phase, &never, p.err, kErrDrain, 100000000ull);
+        tc::mbar_wait_bounded(vbar, phase, &never, p.err, kErrDrain, 100000000ull);
+    }
+
+    // ---- join the warps: their outputs go where their K and V were
+    __syncwarp();
+    float *so = reinterpret_cast<float *>(mine);
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int c = 0; c < kCols / 2; ++c)
+            *reinterpret_cast<float2 *>(so + r * HD + lane * kCols + 2 * c) = acc[r][c];
+    if (lane < RT) sml[(warp * RT + lane) * 2] = m_run, sml[(warp * RT + lane) * 2 + 1] = l_run;
+    __syncthreads();
+    const int n_out = min(rows, RT) * HD;
+    for (int i = threadIdx.x; i < n_out; i += kWarps * 32) {
+        const int r = i / HD, d = i % HD;
+        float m = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) m = fmaxf(m, sml[(w * RT + r) * 2]);
+        const float base = m == -INFINITY ? 0.f : m;
+        float o = 0.f, l = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const float f = exp2f(sml[(w * RT + r) * 2] - base);
+            o = fmaf(f, reinterpret_cast<const float *>(smem + w * C::kWarpBytes)[r * HD + d], o);
+            l = fmaf(f, sml[(w * RT + r) * 2 + 1], l);
+        }
+        const int t = (r0 + r) / p.group, head = kvh * p.group + (r0 + r) % p.group;
+        const long long row = sh.row0 + t;
+        if (p.splits == 1) {
+            store(reinterpret_cast<T *>(p.out + row * p.out_row + head * p.out_head) + d, l == 0.f ? 0.f : o / l);
+        } else {
+            const long long at = (row * p.n_q + head) * p.splits + split;
+            p.part_o[at * HD + d] = o;
+            if (d == 0) p.part_ml[at * 2] = m, p.part_ml[at * 2 + 1] = l;
+        }
+    }
+}
+
+// Joins the splits: a warp per (node, query head).
+template <typename T, int HD>
+__global__ void __launch_bounds__(256) tree_join_kernel(const TreeParams p) {
+    constexpr int kCols = HD / 32;
+    pdl_wait();
+    pdl_trigger();
+    const int item = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31, seq = blockIdx.y;
+    const SeqShape sh = seq_shape(p, seq);
+    const int t = item / p.n_q, head = item % p.n_q;
+    if (t >= sh.nodes) return;
+    const long long row = sh.row0 + t, at = (row * p.n_q + head) * p.splits;
+    float m = -INFINITY;
+    for (int s = lane; s < p.splits; s += 32) m = fmaxf(m, p.part_ml[(at + s) * 2]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float base = m == -INFINITY ? 0.f : m;
+    float o[kCols] = {}, l = 0.f;
+#pragma unroll 4
+    for (int s = 0; s < p.splits; ++s) {
+        const float f = exp2f(p.part_ml[(at + s) * 2] - base);
+        l = fmaf(f, p.part_ml[(at + s) * 2 + 1], l);
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) o[c] = fmaf(f, p.part_o[(at + s) * HD + lane * kCols + c], o[c]);
+    }
+    T *dst = reinterpret_cast<T *>(p.out + row * p.out_row + head * p.out_head) + lane * kCols;
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) store(dst + c, l == 0.f ? 0.f : o[c] / l);
+}
+
+template <typename T, int HD, int RT>
+cudaError_t run_tile(const TreeParams &p, size_t n_seq, cudaStream_t st) {
+    using C = TreeCfg<T, HD, RT>;
+    auto kern = tree_attention_kernel<T, HD, RT>;
+    static std::atomic<uint64_t> done{0};
+    cudaError_t e = once_per_device(
+        done, [&] { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kBytes); });
+    if (e != cudaSuccess) return e;
+    for (size_t s = 0; s < n_seq; s += 65535) {  // grid.z
+        TreeParams q = p;
+        q.q_start += s, q.context_len += s, q.block_table += s * p.table_stride;
+        const unsigned m = (unsigned)std::min<size_t>(n_seq - s, 65535);
+        e = launch_kernel(kern, dim3(p.splits, p.n_kv * p.row_tiles, m), dim3(C::kWarps * 32), C::kBytes, st, q);
+        if (e == cudaSuccess && p.splits > 1)
+            e = launch_kernel(tree_join_kernel<T, HD>, dim3((p.max_tree * p.n_q + 7) / 8, m), dim3(256), 0, st, q);
+        if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
+}
+
+template <typename T, int HD>
+cudaError_t run_tree(const TreeParams &p, int row_tile, size_t n_seq, cudaStream_t st) {
+    switch (row_tile) {
+    case 2: return run_tile<T, HD, 2>(p, n_seq, st);
+    case 4: return run_tile<T, HD, 4>(p, n_seq, st);
+    case 8: return run_tile<T, HD, 8>(p, n_seq, st);
+    case 16: return run_tile<T, HD, 16>(p, n_seq, st);
+    default: return run_tile<T, HD, 32>(p, n_seq, st);
+    }
+}
+
+}  // namespace
+
+TreePlan plan_tree_attention(const pyxis_tree_attention_args &a, const pyxis_kv_pages &kv, int num_sms) {
+    TreePlan t;
+    const long long rows = (long long)a.max_tree * (a.n_q_heads / kv.n_kv_heads);
+    t.row_tile = 2;
+    while (t.row_tile < 32 && t.row_tile < rows) t.row_tile *= 2;
+    t.row_tiles = (int)((rows + t.row_tile - 1) / t.row_tile);
+    // the split that wastes least of the last wave, a split costing about 64 keys of start-up
+    const long long units = (long long)a.n_seq * kv.n_kv_heads * t.row_tiles;
+    const long long keys = std::max<long long>(1, std::min<long long>(a.max_context + a.max_tree,
+                                                                     (long long)a.table_width * kv.page_size));
+    const long long most = std::min<long long>(256, (keys + 255) / 256);
+    double best = 0;
+    t.splits = 1;
+    for (long long s = 1; s <= most; ++s) {
+        const double waves = (double)((units * s + num_sms - 1) / num_sms);
+        const double cost = waves * ((double)keys / s + 64.0) + (s > 1 ? 128.0 : 0.0);
+        if (s == 1 || cost < best * 0.98) best = cost, t.splits = (int)s;
+    }
+    return t;
+}
+
+size_t tree_attention_workspace(const TreePlan &t, const pyxis_tree_attention_args &a, const pyxis_kv_pages &kv) {
+    return t.splits == 1 ? 0 : a.n_rows * a.n_q_heads * t.splits * (size_t)(kv.head_dim + 2) * 4;
+}
+
+cudaError_t launch_tree_attention(const pyxis_tree_attention_args &a, const pyxis_kv_pages &kv, const TreePlan &t,
+                                  void *workspace, int *err, cudaStream_t st) {
+    const long long es = kv.dtype == PYXIS_DTYPE_F32 ? 4 : 2;
+    TreeParams p;
+    p.q = (const char *)a.q;
+    p.k = (const char *)kv.k;
+    p.v = (const char *)kv.v;
+    p.out = (char *)a.out;
+    p.q_row = a.q_row * es;
+    p.q_head = a.q_head * es;
+    p.out_row = a.out_row * es;
+    p.out_head = a.out_head * es;
+    p.page_stride = kv.page_stride * es;
+    p.slot_stride = kv.slot_stride * es;
+    p.head_stride = kv.head_stride * es;
+    p.q_start = a.q_start;
+    p.context_len = a.context_len;
+    p.block_table = a.block_table;
+    p.tree_mask = (const unsigned long long *)a.tree_mask;
+    p.table_stride = (long long)a.table_stride;
+    p.capacity = (long long)a.table_width * kv.page_size;
+    p.n_rows = (int)a.n_rows;
+    p.n_q = a.n_q_heads;
+    p.n_kv = kv.n_kv_heads;
+    p.group = a.n_q_heads / kv.n_kv_heads;
+    p.page_size = kv.page_size;
+    p.num_pages = kv.num_pages;
+    p.max_tree = a.max_tree;
+    p.splits = t.splits;
+    p.row_tiles = t.row_tiles;
+    p.scale2 = a.scale * kLog2e;
+    p.part_ml = (float *)workspace;
+    p.part_o = p.part_ml ? p.part_ml + a.n_rows * a.n_q_heads * t.splits * 2 : nullptr;
+    p.err = err;
+    if (kv.dtype == PYXIS_DTYPE_F32)
+        return kv.head_dim == 128 ? run_tree<float, 128>(p, t.row_tile, a.n_seq, st)
+                                  : run_tree<float, 64>(p, t.row_tile, a.n_seq, st);
+    return kv.head_dim == 128 ? run_tree<__nv_bfloat16, 128>(p, t.row_tile, a.n_seq, st)
+                              : run_tree<__nv_bfloat16, 64>(p, t.row_tile, a.n_seq, st);
+}
+
+}  // namespace pyxis

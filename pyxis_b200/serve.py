@@ -1,0 +1,339 @@
+"""Operators of a decoding step that verifies drafted tokens over a paged KV cache
+(include/pyxis_serve.h), over torch CUDA tensors:
+
+  qk_norm_rope_dev     QK-RMSNorm, rotary positions and the append to the cache's pages in one pass
+                       over the q|k|v rows (src/attention.rs:81-100, :144-162)
+  tree_attention_dev   attention of a tree of drafted tokens per sequence over the pages
+                       (src/attention.rs:107-135); a tree of one node is a plain decode step
+  sample_dev           temperature, top-k, top-p and min-p from given uniform numbers
+                       (src/sampler.rs:23-110)
+  kv_copy_pages_dev    pages copied in all layers (forks)
+  kv_compact_dev       the accepted branch of each tree moved to the front of its drafts
+  PagePool             which pages are free and how many tables share each (host side)
+
+Pages are two tensors of one shape and layout, ``[..., num_pages, page_size, n_kv_heads, head_dim]``
+with any strides whose last is 1, float32 or bfloat16; the page operators take a leading axis of
+layers.  Calls are asynchronous on ``stream`` (default: torch's current stream of the tensors'
+device) and raise PyxisError on bad arguments.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import numpy as np
+
+from . import _native, _require_cuda
+from ._native import DTYPE_BF16, DTYPE_F32, PYXIS_EINVAL, PyxisError, check
+
+_vp, _sz, _i64 = C.c_void_p, C.c_size_t, C.c_int64
+
+
+class _Pages(C.Structure):
+    _fields_ = [("k", _vp), ("v", _vp), ("dtype", C.c_int), ("n_layers", C.c_int), ("num_pages", C.c_int),
+                ("page_size", C.c_int), ("n_kv_heads", C.c_int), ("head_dim", C.c_int), ("layer_stride", _i64),
+                ("page_stride", _i64), ("slot_stride", _i64), ("head_stride", _i64)]
+
+
+class _RopeArgs(C.Structure):
+    _fields_ = [("qkv", _vp), ("q", _vp), ("n_tokens", _sz), ("ld_qkv", _sz), ("ld_q", _sz), ("positions", _vp),
+                ("slots", _vp), ("inv_freq", _vp), ("q_norm", _vp), ("k_norm", _vp), ("n_q_heads", C.c_int),
+                ("rotary_dim", C.c_int), ("interleaved", C.c_int), ("eps", C.c_float), ("rope_scale", C.c_float)]
+
+
+class _TreeArgs(C.Structure):
+    _fields_ = [("q", _vp), ("out", _vp), ("q_row", _i64), ("q_head", _i64), ("out_row", _i64), ("out_head", _i64),
+                ("n_rows", _sz), ("n_seq", _sz), ("q_start", _vp), ("context_len", _vp), ("block_table", _vp),
+                ("tree_mask", _vp), ("table_stride", _sz), ("table_width", _sz), ("n_q_heads", C.c_int),
+                ("max_tree", C.c_int), ("max_context", _i64), ("scale", C.c_float)]
+
+
+class _SampleParams(C.Structure):
+    _fields_ = [("temperature", _vp), ("top_k", _vp), ("top_p", _vp), ("min_p", _vp), ("temperature_all", C.c_double),
+                ("top_k_all", C.c_int32), ("top_p_all", C.c_double), ("min_p_all", C.c_double)]
+
+
+def _fail(msg: str):
+    raise PyxisError(PYXIS_EINVAL, msg)
+
+
+_DTYPES: dict = {}
+
+
+def _dtype(t) -> int:
+    if not _DTYPES:
+        import torch
+        _DTYPES.update({torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16})
+    d = _DTYPES.get(t.dtype)
+    if d is None:
+        _fail(f"dtype {t.dtype}: float32 or bfloat16 is needed")
+    return d
+
+
+def _where(t):
+    """(context, its device) of a CUDA tensor."""
+    if not t.is_cuda:
+        _fail(f"a CUDA tensor is needed, not one on {t.device}")
+    return _require_cuda(t.device.index or 0)
+
+
+def _stream(stream, device) -> int:
+    import torch
+    h = (stream or torch.cuda.current_stream(device)).cuda_stream
+    return h if h else 0x1  # torch's default stream, as the explicit handle of the legacy one
+
+
+def _array(t, what: str, dtype: str, n: int, ctx) -> int:
+    """Address of a contiguous device array of at least n elements."""
+    if not t.is_cuda or (t.device.index or 0) != ctx.device:
+        _fail(f"{what} must be on cuda:{ctx.device}")
+    if str(t.dtype) != dtype:
+        _fail(f"{what} must be {dtype}, not {t.dtype}")
+    if t.numel() < n or not t.is_contiguous():
+        _fail(f"{what} must hold {n} contiguous elements")
+    return t.data_ptr()
+
+
+def _pages(k, v, ctx, layers: bool) -> _Pages:
+    dims = 5 if layers else 4
+    if k.dim() != dims or k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype:
+        _fail(f"k_pages and v_pages must be {dims}-dimensional tensors of one shape, layout and type")
+    if not k.is_cuda or k.device != v.device or (k.device.index or 0) != ctx.device:
+        _fail(f"cache pages must be on cuda:{ctx.device}")
+    s, n = k.stride(), k.shape
+    if s[-1] != 1:
+        _fail("the elements of a head must be contiguous")
+    return _Pages(k.data_ptr(), v.data_ptr(), _dtype(k), n[0] if layers else 1, n[-4], n[-3], n[-2], n[-1],
+                  s[0] if layers else 0, s[-4], s[-3], s[-2])
+
+
+ROPE_KINDS = {"plain": 0, "linear": 1, "ntk": 2, "yarn": 3}
+
+
+def rope_frequencies(rotary_dim: int, theta: float, kind: str = "plain", factor: float = 1.0,
+                     original_context: float = 0.0, beta_fast: float = 32.0, beta_slow: float = 1.0):
+    """(frequencies [rotary_dim / 2] float64, scale of cos and sin) on the host
+    (pyxis_rope_frequencies): kind "plain", "linear", "ntk" or "yarn"."""
+    if kind not in ROPE_KINDS:
+        _fail(f"unknown frequency scaling {kind!r}")
+    if rotary_dim <= 0:
+        _fail(f"rotary_dim {rotary_dim} is not even and positive")
+    freq = np.empty(rotary_dim // 2, np.float64)
+    scale = C.c_double()
+    check(_native.lib().pyxis_rope_frequencies(ROPE_KINDS[kind], theta, rotary_dim, factor, original_context, beta_fast,
+                                               beta_slow, freq.ctypes.data_as(_vp), C.addressof(scale)))
+    return freq, scale.value
+
+
+def qk_norm_rope_dev(qkv, positions, inv_freq, n_q_heads: int, n_kv_heads: int, head_dim: int, *, k_pages, v_pages, slots,
+                     q_norm=None, k_norm=None, eps: float = 1e-6, interleaved: bool = False, rope_scale: float = 1.0,
+                     q=None, stream=None):
+    """Normalises and rotates the heads of ``qkv`` [tokens, (n_q + 2 n_kv) * head_dim], puts keys and
+    values into ``k_pages`` / ``v_pages`` [pages, page_size, n_kv, head_dim] at ``slots`` (int32; page
+    * page_size + place, -1: none) and returns the queries [tokens, n_q, head_dim]
+    (pyxis_cuda_qk_norm_rope_dev).  ``positions`` int32 [tokens]; ``inv_freq`` float64 [rotary_dim / 2]
+    on the device, or None for no rotation; ``q_norm`` / ``k_norm`` float32 [head_dim] or None;
+    ``q``: a [tokens, n_q, head_dim] tensor with contiguous heads to write, ``qkv``'s own rows
+    included."""
+    import torch
+
+    ctx = _where(qkv)
+    if qkv.dim() != 2 or qkv.shape[1] != (n_q_heads + 2 * n_kv_heads) * head_dim or qkv.stride(1) != 1:
+        _fail("qkv must be [tokens, (n_q + 2 n_kv) * head_dim] with contiguous rows")
+    n = qkv.shape[0]
+    kv = _pages(k_pages, v_pages, ctx, False)
+    if kv.n_kv_heads != n_kv_heads or kv.head_dim != head_dim or k_pages.dtype != qkv.dtype:
+        _fail("the cache's heads or type differ from qkv's")
+    if q is None:
+        q = torch.empty((n, n_q_heads, head_dim), dtype=qkv.dtype, device=qkv.device)
+    elif q.shape != (n, n_q_heads, head_dim) or q.dtype != qkv.dtype or q.device != qkv.device or q.stride(2) != 1 or (
+            n_q_heads > 1 and q.stride(1) != head_dim):
+        _fail("q must be [tokens, n_q, head_dim] of qkv's type and device with contiguous heads")
+    rot = 0
+    if inv_freq is not None:
+        rot = 2 * inv_freq.numel()
+    a = _RopeArgs(qkv.data_ptr(), q.data_ptr(), n, qkv.stride(0), q.stride(0),
+                  _array(positions, "positions", "torch.int32", n, ctx) if rot else None,
+                  _array(slots, "slots", "torch.int32", n, ctx),
+                  _array(inv_freq, "inv_freq", "torch.float64", rot // 2, ctx) if rot else None,
+                  None if q_norm is None else _array(q_norm, "q_norm", "torch.float32", head_dim, ctx),
+                  None if k_norm is None else _array(k_norm, "k_norm", "torch.float32", head_dim, ctx),
+                  n_q_heads, rot, 1 if interleaved else 0, eps, rope_scale)
+    check(_native.lib().pyxis_cuda_qk_norm_rope_dev(ctx.handle, C.byref(a), C.byref(kv), _stream(stream, qkv.device)))
+    return q
+
+
+def tree_attention_dev(q, k_pages, v_pages, block_table, context_len, q_start, tree_mask=None, *, max_tree: int,
+                       max_context: int | None = None, scale: float | None = None, out=None, workspace=None, stream=None):
+    """Attention of ``q`` [rows, n_q, head_dim] over the pages (pyxis_cuda_tree_attention_dev):
+    sequence s owns rows ``q_start[s]`` .. ``q_start[s + 1] - 1`` (at most ``max_tree`` <= 64), whose
+    row j sees positions below ``context_len[s]`` and the drafts i with bit i of ``tree_mask`` (int64
+    or uint64 [rows]; None: drafts 0 .. j) at positions ``context_len[s]`` + i of the pages in
+    ``block_table`` [sequences, width].  ``max_context`` bounds the contexts, for the split of the work
+    (default: what the table holds); ``scale`` defaults to 1 / sqrt(head_dim).  Rows outside every
+    sequence are left as they are (in a new ``out``: uninitialised)."""
+    import torch
+
+    ctx = _where(q)
+    kv = _pages(k_pages, v_pages, ctx, False)
+    if q.dim() != 3 or q.shape[2] != kv.head_dim or q.stride(2) != 1 or q.dtype != k_pages.dtype:
+        _fail("q must be [rows, n_q, head_dim] of the cache's type")
+    rows, n_q, hd = q.shape
+    if out is None:
+        out = torch.empty((rows, n_q, hd), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.stride(2) != 1:
+        _fail("out must have q's shape, type and device")
+    if block_table.dim() != 2 or block_table.stride(1) != 1 or str(block_table.dtype) != "torch.int32" or \
+            block_table.device != q.device:
+        _fail("block_table must be int32 [sequences, pages] with contiguous rows on q's device")
+    n_seq, width = block_table.shape
+    mask = None
+    if tree_mask is not None:
+        mask = _array(tree_mask, "tree_mask", "torch.uint64" if str(tree_mask.dtype) == "torch.uint64" else "torch.int64",
+                      rows, ctx)
+    a = _TreeArgs(q.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1), out.stride(0), out.stride(1), rows, n_seq,
+                  _array(q_start, "q_start", "torch.int32", n_seq + 1, ctx),
+                  _array(context_len, "context_len", "torch.int32", n_seq, ctx), block_table.data_ptr(), mask,
+                  block_table.stride(0), width, n_q, max_tree, width * kv.page_size if max_context is None else max_context,
+                  hd ** -0.5 if scale is None else scale)
+    ws, ws_bytes = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
+    check(_native.lib().pyxis_cuda_tree_attention_dev(ctx.handle, C.byref(a), C.byref(kv), ws, ws_bytes,
+                                                      _stream(stream, q.device)))
+    return out
+
+
+def kv_copy_pages_dev(k_pages, v_pages, src, dst, stream=None) -> None:
+    """Copies pages ``src[i]`` to ``dst[i]`` (int32) of ``k_pages`` / ``v_pages`` [layers, pages,
+    page_size, n_kv, head_dim] in every layer (pyxis_cuda_kv_copy_pages_dev)."""
+    ctx = _where(k_pages)
+    kv = _pages(k_pages, v_pages, ctx, True)
+    n = src.numel()
+    if dst.numel() != n:
+        _fail("src and dst differ in length")
+    check(_native.lib().pyxis_cuda_kv_copy_pages_dev(
+        ctx.handle, C.byref(kv), _array(src, "src", "torch.int32", n, ctx), _array(dst, "dst", "torch.int32", n, ctx), n,
+        _stream(stream, k_pages.device)))
+
+
+def kv_compact_dev(k_pages, v_pages, block_table, context_len, accepted, new_len=None, stream=None):
+    """Moves the cache entries of each sequence's ``accepted`` nodes (bits, int64 or uint64
+    [sequences]) to positions ``context_len[s]``, ``context_len[s]`` + 1, ... in every layer and
+    returns ``new_len`` int32 [sequences] = context_len + their number (pyxis_cuda_kv_compact_dev)."""
+    import torch
+
+    ctx = _where(k_pages)
+    kv = _pages(k_pages, v_pages, ctx, True)
+    if block_table.dim() != 2 or block_table.stride(1) != 1 or str(block_table.dtype) != "torch.int32" or \
+            block_table.device != k_pages.device:
+        _fail("block_table must be int32 [sequences, pages] with contiguous rows on the cache's device")
+    n_seq, width = block_table.shape
+    if new_len is None:
+        new_len = torch.empty(n_seq, dtype=torch.int32, device=k_pages.device)
+    bits = "torch.uint64" if str(accepted.dtype) == "torch.uint64" else "torch.int64"
+    check(_native.lib().pyxis_cuda_kv_compact_dev(
+        ctx.handle, C.byref(kv), block_table.data_ptr(), block_table.stride(0), width,
+        _array(context_len, "context_len", "torch.int32", n_seq, ctx), _array(accepted, "accepted", bits, n_seq, ctx), n_seq,
+        _array(new_len, "new_len", "torch.int32", n_seq, ctx), _stream(stream, k_pages.device)))
+    return new_len
+
+
+def sample_dev(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, idx=None, prob=None, stream=None):
+    """One token per row of ``logits`` [M, n] (float32 or bfloat16) from ``uniforms`` float32 [M] in
+    [0, 1) (pyxis_cuda_sample_dev).  Each parameter is a number for all rows or a device tensor [M]
+    (float32; ``top_k`` int32).  Temperature 0 is the greedy choice.  Returns (idx int32 [M],
+    prob float32 [M]: the token's share of the kept weights)."""
+    import torch
+
+    if logits.dim() == 1:
+        logits = logits.unsqueeze(0)
+    ctx = _where(logits)
+    M, n = logits.shape
+    if n > 1 and logits.stride(1) != 1:
+        _fail("the logits of a row must be contiguous")
+    p = _SampleParams(None, None, None, None, 1.0, 0, 1.0, 0.0)
+    for name, value, kind in (("temperature", temperature, "torch.float32"), ("top_k", top_k, "torch.int32"),
+                              ("top_p", top_p, "torch.float32"), ("min_p", min_p, "torch.float32")):
+        if isinstance(value, torch.Tensor):
+            setattr(p, name, _array(value, name, kind, M, ctx))
+        else:
+            setattr(p, name + "_all", value)
+    if idx is None:
+        idx = torch.empty(M, dtype=torch.int32, device=logits.device)
+    if prob is None:
+        prob = torch.empty(M, dtype=torch.float32, device=logits.device)
+    check(_native.lib().pyxis_cuda_sample_dev(
+        ctx.handle, logits.data_ptr(), _dtype(logits), M, n, logits.stride(0), _array(uniforms, "uniforms", "torch.float32", M, ctx),
+        C.byref(p), _array(idx, "idx", "torch.int32", M, ctx), _array(prob, "prob", "torch.float32", M, ctx),
+        _stream(stream, logits.device)))
+    return idx, prob
+
+
+class PagePool:
+    """Host-side bookkeeping of a cache's pages: the block tables of sequences over ``num_pages`` pages
+    of ``page_size`` slots, each page counted by the tables that name it.
+
+        table = pool.allocate(tokens)          pages for a new sequence
+        pool.grow(table, tokens)               more of them, in place
+        child, src, dst = pool.fork(table, n)  a table sharing the full pages of the first n tokens; the
+                                               partly filled one is copied: kv_copy_pages_dev(.., src, dst)
+        pool.shrink(table, tokens)             gives back the pages past the first ``tokens`` slots
+        pool.free(table)
+
+    Raises PyxisError (PYXIS_ENOMEM) when too few pages are free, without taking any."""
+
+    def __init__(self, num_pages: int, page_size: int):
+        if num_pages <= 0 or page_size <= 0:
+            _fail(f"{num_pages} pages of {page_size} slots")
+        self.num_pages, self.page_size = num_pages, page_size
+        self._free = list(range(num_pages - 1, -1, -1))
+        self._uses = [0] * num_pages
+
+    @property
+    def available(self) -> int:
+        return len(self._free)
+
+    def _pages_for(self, tokens: int) -> int:
+        if tokens < 0:
+            _fail(f"{tokens} tokens")
+        return -(-tokens // self.page_size)
+
+    def _take(self, n: int) -> list[int]:
+        if n > len(self._free):
+            raise PyxisError(_native.PYXIS_ENOMEM, f"{n} pages needed, {len(self._free)} free")
+        got = [self._free.pop() for _ in range(n)]
+        for p in got:
+            self._uses[p] = 1
+        return got
+
+    def _drop(self, pages) -> None:
+        for p in pages:
+            if self._uses[p] <= 0:
+                _fail(f"page {p} is free already")
+            self._uses[p] -= 1
+            if self._uses[p] == 0:
+                self._free.append(p)
+
+    def allocate(self, tokens: int) -> list[int]:
+        return self._take(self._pages_for(tokens))
+
+    def grow(self, table: list[int], tokens: int) -> None:
+        table.extend(self._take(max(0, self._pages_for(tokens) - len(table))))
+
+    def shrink(self, table: list[int], tokens: int) -> None:
+        keep = self._pages_for(tokens)
+        if tokens % self.page_size and keep <= len(table) and self._uses[table[keep - 1]] > 1:
+            _fail(f"page {table[keep - 1]} is shared and would be written again: fork at {tokens} tokens instead")
+        self._drop(table[keep:])
+        del table[keep:]
+
+    def free(self, table: list[int]) -> None:
+        self._drop(table)
+        table.clear()
+
+    def fork(self, table: list[int], tokens: int) -> tuple[list[int], list[int], list[int]]:
+        if self._pages_for(tokens) > len(table):
+            _fail(f"a fork at {tokens} tokens of a table of {len(table)} pages")
+        full = tokens // self.page_size
+        new = self._take(self._pages_for(tokens) - full)
+        for p in table[:full]:
+            self._uses[p] += 1
+        return table[:full] + new, table[full : full + len(new)], list(new)
