@@ -15,14 +15,16 @@ cudaError_t launch_qk_norm_rope(const pyxis_qk_norm_rope_args &a, const pyxis_kv
 
 // How a call's keys are split over the GPU, from sizes the host knows.
 struct TreePlan {
+    bool tensor;    // on the tensor cores, which split the keys on the device
     int row_tile;   // query rows (nodes x heads of one kv head) of a CTA
     int row_tiles;  // CTAs over the rows of one (sequence, kv head)
     int splits;     // CTAs over the keys
 };
 TreePlan plan_tree_attention(const pyxis_tree_attention_args &a, const pyxis_kv_pages &kv, int num_sms);
-size_t tree_attention_workspace(const TreePlan &p, const pyxis_tree_attention_args &a, const pyxis_kv_pages &kv);
+size_t tree_attention_workspace(const TreePlan &p, const pyxis_tree_attention_args &a, const pyxis_kv_pages &kv,
+                                int num_sms);
 cudaError_t launch_tree_attention(const pyxis_tree_attention_args &a, const pyxis_kv_pages &kv, const TreePlan &p,
-                                  void *workspace, int *err, cudaStream_t st);
+                                  void *workspace, int *err, int num_sms, cudaStream_t st);
 
 cudaError_t launch_kv_copy_pages(const pyxis_kv_pages &kv, const int32_t *src, const int32_t *dst, size_t n, int num_sms,
                                  cudaStream_t st);

@@ -169,7 +169,7 @@ int pyxis_cuda_qk_norm_rope_dev(pyxis_cuda_ctx *ctx, const pyxis_qk_norm_rope_ar
 size_t pyxis_cuda_tree_attention_workspace_size(pyxis_cuda_ctx *ctx, const pyxis_tree_attention_args *a,
                                                 const pyxis_kv_pages *kv) {
     if (!ctx || check_tree(a, kv) != PYXIS_OK || a->n_seq == 0 || a->n_rows == 0) return 0;
-    return tree_attention_workspace(plan_tree_attention(*a, *kv, ctx->num_sms), *a, *kv);
+    return tree_attention_workspace(plan_tree_attention(*a, *kv, ctx->num_sms), *a, *kv, ctx->num_sms);
 }
 
 int pyxis_cuda_tree_attention_dev(pyxis_cuda_ctx *ctx, const pyxis_tree_attention_args *a, const pyxis_kv_pages *kv,
@@ -191,7 +191,7 @@ int pyxis_cuda_tree_attention_dev(pyxis_cuda_ctx *ctx, const pyxis_tree_attentio
     DeviceGuard g(ctx->device);
     cudaStream_t st = pick_stream(ctx, stream);
     const TreePlan plan = plan_tree_attention(*a, *kv, ctx->num_sms);
-    const size_t need = tree_attention_workspace(plan, *a, *kv);
+    const size_t need = tree_attention_workspace(plan, *a, *kv, ctx->num_sms);
     if (need && workspace) {
         if (workspace_bytes < need || !aligned(workspace, 256))
             return fail(PYXIS_EINVAL, "tree attention workspace: %zu bytes, 256-byte aligned, are needed", need);
@@ -199,7 +199,8 @@ int pyxis_cuda_tree_attention_dev(pyxis_cuda_ctx *ctx, const pyxis_tree_attentio
         if (const int rc = context_workspace(ctx, need, st)) return rc;
         workspace = ctx->ws;
     }
-    return cuda_status(launch_tree_attention(*a, *kv, plan, workspace, ctx->d_err, st), "tree attention launch");
+    return cuda_status(launch_tree_attention(*a, *kv, plan, workspace, ctx->d_err, ctx->num_sms, st),
+                       "tree attention launch");
 }
 
 int pyxis_cuda_kv_copy_pages_dev(pyxis_cuda_ctx *ctx, const pyxis_kv_pages *kv, const int32_t *src, const int32_t *dst,

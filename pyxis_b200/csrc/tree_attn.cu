@@ -24,43 +24,14 @@
 #include "common.cuh"
 #include "serve.h"
 #include "tc_ptx.cuh"
+#include "tree_attn.cuh"
 
 namespace pyxis {
 namespace {
 
 constexpr int kBlock = 32;  // keys of a warp's block: one per lane
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr uint64_t kTimeoutNs = 2000000000ull;
 enum { kErrLoad = 0x701, kErrDrain = 0x702 };
-
-struct TreeParams {
-    const char *q, *k, *v;
-    char *out;
-    long long q_row, q_head, out_row, out_head;              // bytes
-    long long page_stride, slot_stride, head_stride;         // bytes
-    const int32_t *q_start, *context_len, *block_table;
-    const unsigned long long *tree_mask;
-    long long table_stride, capacity;                        // capacity: positions that a table row names
-    int n_rows, n_q, n_kv, group, page_size, num_pages, max_tree, splits, row_tiles;
-    float scale2;                                            // scale * log2 e
-    float *part_o, *part_ml;                                 // [row][head][split][HD], [..][2] (splits > 1)
-    int *err;
-};
-
-// A sequence's rows and keys, from device memory and clamped to what the buffers hold.
-struct SeqShape {
-    int row0, nodes;
-    long long ctx, total;
-};
-PYXIS_DEVINL SeqShape seq_shape(const TreeParams &p, int seq) {
-    SeqShape s;
-    s.row0 = min(max(p.q_start[seq], 0), p.n_rows);
-    const int end = min(max(p.q_start[seq + 1], s.row0), p.n_rows);
-    s.nodes = min(end - s.row0, p.max_tree);
-    s.ctx = min((long long)max(p.context_len[seq], 0), p.capacity);
-    s.total = min(s.ctx + s.nodes, p.capacity);
-    return s;
-}
 
 PYXIS_DEVINL float redux_max(float v) {
     float r;
@@ -82,9 +53,6 @@ PYXIS_DEVINL float2 ld2(const __nv_bfloat16 *p) {
 }
 PYXIS_DEVINL float to_f32(float x) { return x; }
 PYXIS_DEVINL float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
-PYXIS_DEVINL void store(float *p, float x) { *p = x; }
-PYXIS_DEVINL void store(__nv_bfloat16 *p, float x) { *p = __float2bfloat16_rn(x); }
-
 template <typename T, int HD, int RT>
 struct TreeCfg {
     static constexpr int kPitch = HD * (int)sizeof(T) + 16;          // bytes of a K or V row in shared memory
@@ -400,6 +368,7 @@ cudaError_t run_tree(const TreeParams &p, int row_tile, size_t n_seq, cudaStream
 
 TreePlan plan_tree_attention(const pyxis_tree_attention_args &a, const pyxis_kv_pages &kv, int num_sms) {
     TreePlan t;
+    t.tensor = tree_attention_tc_supported(a, kv);
     const long long rows = (long long)a.max_tree * (a.n_q_heads / kv.n_kv_heads);
     t.row_tile = 2;
     while (t.row_tile < 32 && t.row_tile < rows) t.row_tile *= 2;
@@ -419,12 +388,14 @@ TreePlan plan_tree_attention(const pyxis_tree_attention_args &a, const pyxis_kv_
     return t;
 }
 
-size_t tree_attention_workspace(const TreePlan &t, const pyxis_tree_attention_args &a, const pyxis_kv_pages &kv) {
+size_t tree_attention_workspace(const TreePlan &t, const pyxis_tree_attention_args &a, const pyxis_kv_pages &kv,
+                                int num_sms) {
+    if (t.tensor) return tree_attention_tc_workspace(kv, num_sms);
     return t.splits == 1 ? 0 : a.n_rows * a.n_q_heads * t.splits * (size_t)(kv.head_dim + 2) * 4;
 }
 
 cudaError_t launch_tree_attention(const pyxis_tree_attention_args &a, const pyxis_kv_pages &kv, const TreePlan &t,
-                                  void *workspace, int *err, cudaStream_t st) {
+                                  void *workspace, int *err, int num_sms, cudaStream_t st) {
     const long long es = kv.dtype == PYXIS_DTYPE_F32 ? 4 : 2;
     TreeParams p;
     p.q = (const char *)a.q;
@@ -454,9 +425,10 @@ cudaError_t launch_tree_attention(const pyxis_tree_attention_args &a, const pyxi
     p.splits = t.splits;
     p.row_tiles = t.row_tiles;
     p.scale2 = a.scale * kLog2e;
+    p.err = err;
+    if (t.tensor) return launch_tree_attention_tc(p, a, kv, workspace, num_sms, st);
     p.part_ml = (float *)workspace;
     p.part_o = p.part_ml ? p.part_ml + a.n_rows * a.n_q_heads * t.splits * 2 : nullptr;
-    p.err = err;
     if (kv.dtype == PYXIS_DTYPE_F32)
         return kv.head_dim == 128 ? run_tree<float, 128>(p, t.row_tile, a.n_seq, st)
                                   : run_tree<float, 64>(p, t.row_tile, a.n_seq, st);

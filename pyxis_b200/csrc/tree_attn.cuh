@@ -1,0 +1,53 @@
+// tree_attn.cuh -- what the tree-attention kernels (tree_attn.cu on the CUDA cores, tree_attn_tc.cu
+// on the tensor cores) share: their parameters and a sequence's shape.
+#pragma once
+
+#include <cuda_bf16.h>
+
+#include "common.cuh"
+#include "serve.h"
+
+namespace pyxis {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct TreeParams {
+    const char *q, *k, *v;
+    char *out;
+    long long q_row, q_head, out_row, out_head;              // bytes
+    long long page_stride, slot_stride, head_stride;         // bytes
+    const int32_t *q_start, *context_len, *block_table;
+    const unsigned long long *tree_mask;
+    long long table_stride, capacity;                        // capacity: positions that a table row names
+    int n_rows, n_q, n_kv, group, page_size, num_pages, max_tree, splits, row_tiles;
+    float scale2;                                            // scale * log2 e
+    float *part_o, *part_ml;                                 // [row][head][split][HD], [..][2] (splits > 1)
+    int *err;
+};
+
+// A sequence's rows and keys, from device memory and clamped to what the buffers hold.
+struct SeqShape {
+    int row0, nodes;
+    long long ctx, total;
+};
+PYXIS_DEVINL SeqShape seq_shape(const TreeParams &p, int seq) {
+    SeqShape s;
+    s.row0 = min(max(p.q_start[seq], 0), p.n_rows);
+    const int end = min(max(p.q_start[seq + 1], s.row0), p.n_rows);
+    s.nodes = min(end - s.row0, p.max_tree);
+    s.ctx = min((long long)max(p.context_len[seq], 0), p.capacity);
+    s.total = min(s.ctx + s.nodes, p.capacity);
+    return s;
+}
+
+PYXIS_DEVINL void store(float *p, float x) { *p = x; }
+PYXIS_DEVINL void store(__nv_bfloat16 *p, float x) { *p = __float2bfloat16_rn(x); }
+
+// The tensor-core form (bf16 pages of a size that tiles 128 keys): whether it takes the call, its
+// workspace, its launch.
+bool tree_attention_tc_supported(const pyxis_tree_attention_args &a, const pyxis_kv_pages &kv);
+size_t tree_attention_tc_workspace(const pyxis_kv_pages &kv, int num_sms);
+cudaError_t launch_tree_attention_tc(const TreeParams &p, const pyxis_tree_attention_args &a, const pyxis_kv_pages &kv,
+                                     void *workspace, int num_sms, cudaStream_t st);
+
+}  // namespace pyxis
