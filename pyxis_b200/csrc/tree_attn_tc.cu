@@ -65,7 +65,14 @@ struct TcParams {
     int tile_pages;     // boxes per tile
     int vec_q, vec_out; // 16-byte accesses to q's and out's rows
     uint32_t q_sign;    // flips q's signs for a negative scale
-    float *part_o, *part_ml;  // [CTA][2][128][HD], [..][2]
+    float *part_o, *part_ml;  // [CTA][2][HD][128], [CTA][2][128][2]
+    struct Shared *shared;    // [CTA]
+};
+
+// A unit that begins in a CTA and goes on in the next ones, up to CTA `last` (-1: the CTA has none).
+// Its sums are in slot 1 of the first CTA and slot 0 of the others.
+struct Shared {
+    int last, row0, kvh, r0, rows;
 };
 
 PYXIS_DEVINL void tma_load_4d(void *dst, const void *tmap, int x, int y, int z, int w, uint64_t *bar) {
@@ -96,6 +103,34 @@ PYXIS_DEVINL float ex2(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
+}
+
+// 16 consecutive 32-bit columns of this warp's 32 TMEM lanes (complete after tmem_wait_st).
+PYXIS_DEVINL void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+
+PYXIS_DEVINL uint32_t pack_bf16(float lo, float hi) {
+    const __nv_bfloat162 x = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&x);
+}
+// 2 N consecutive bf16 of an output row.
+template <int N>
+PYXIS_DEVINL void write_row(char *dst, const uint32_t (&u)[N], int vec) {
+    if (vec) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) reinterpret_cast<uint4 *>(dst)[i / 4] = make_uint4(u[i], u[i + 1], u[i + 2], u[i + 3]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            reinterpret_cast<uint16_t *>(dst)[2 * i] = (uint16_t)u[i];
+            reinterpret_cast<uint16_t *>(dst)[2 * i + 1] = (uint16_t)(u[i] >> 16);
+        }
+    }
 }
 
 // Units of a sequence: (kv head, 128-row tile); key tiles of each.
@@ -163,18 +198,24 @@ struct Walk {
     PYXIS_DEVINL bool whole() const { return tb == 0 && te == w.tiles; }
 };
 
-// Sum of the sequences' work, and where tile `at` of it lies.  All threads of the block (up to 1024).
-PYXIS_DEVINL long long block_total(const TreeParams &p, int n_seq, long long *warp_sum) {
-    long long total = 0;
-    for (int s = threadIdx.x; s < n_seq; s += blockDim.x) total += seq_work(p, s).work();
+// Inclusive sum over the block's threads; *all is the sum of all of them.
+PYXIS_DEVINL long long block_scan(long long x, long long *warp_sum, long long *all) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    if ((threadIdx.x & 31) == 0) warp_sum[threadIdx.x >> 5] = total;
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
     __syncthreads();
-    total = 0;
-    for (int w = 0; w < (int)(blockDim.x + 31) / 32; ++w) total += warp_sum[w];
+    if (lane == 31) warp_sum[warp] = x;
     __syncthreads();
-    return total;
+    *all = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) {
+        if (w < warp) x += warp_sum[w];
+        *all += warp_sum[w];
+    }
+    return x;
 }
 
 template <int HD>
@@ -224,32 +265,29 @@ __global__ void __launch_bounds__(kThreads, 1)
     pdl_trigger();
 
     // ---- this CTA's tiles
-    const long long total = block_total(p, a.n_seq, warp_sum);
+    long long total = 0, mine = 0, incl = 0, sum;
+    for (int s0 = 0; s0 < a.n_seq; s0 += kThreads) {
+        const int s = s0 + threadIdx.x;
+        mine = s < a.n_seq ? seq_work(p, s).work() : 0;
+        incl = block_scan(mine, warp_sum, &sum);
+        total += sum;
+    }
     const int g = shares(total, gridDim.x), c = blockIdx.x;
     const long long lo = c < g ? first_tile(total, c, g) : 0, count = c < g ? first_tile(total, c + 1, g) - lo : 0;
+    if (threadIdx.x == 0) a.shared[c].last = -1;
     if (count > 0) {
         long long before = 0;
         for (int s0 = 0; s0 < a.n_seq; s0 += kThreads) {
             const int s = s0 + threadIdx.x;
-            const long long mine = s < a.n_seq ? seq_work(p, s).work() : 0;
-            long long incl = mine;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const long long x = __shfl_up_sync(0xffffffffu, incl, o);
-                if (lane >= o) incl += x;
-            }
-            if (lane == 31) warp_sum[warp] = incl;
-            __syncthreads();
-            long long sum = 0;
-            for (int w = 0; w < kThreads / 32; ++w) {
-                if (w < warp) incl += warp_sum[w];
-                sum += warp_sum[w];
+            if (a.n_seq > kThreads) {  // else they are still at hand
+                mine = s < a.n_seq ? seq_work(p, s).work() : 0;
+                incl = block_scan(mine, warp_sum, &sum);
             }
             const long long first = before + incl - mine;
             if (mine > 0 && lo >= first && lo < first + mine) start_seq = s, start_off = lo - first;
             before += sum;
-            __syncthreads();
         }
+        __syncthreads();
         Walk w;
         w.begin(p, start_seq, start_off, count);
         if (warp == kProdWarp) {
@@ -372,7 +410,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int row = quad * 32 + lane, tid = threadIdx.x - kSmWarp0 * 32;
             const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
             const uint32_t tO = tmem_base + lane_off + kOCol;
-            const float c2 = fabsf(p.scale2);
+            const float c2 = fmaxf(fabsf(p.scale2), 1e-37f);  // a masked score stays -inf with scale 0, too
             auto wait = [&](uint64_t *bar, long long phase) -> bool {
                 return __all_sync(0xffffffffu, tc::mbar_wait_bounded(bar, (uint32_t)(phase & 1), abort_flag, p.err, kErrSoft,
                                                                      kTimeoutNs));
@@ -386,23 +424,31 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int rows = min(sh.nodes * p.group - r0, kRows);
                 const bool active = quad * 32 < rows;  // the warp has rows
                 // ---- Q of the segment; the last segment's MMAs are done (odone)
-                for (int i = tid; i < rows * (HD / 8); i += kSmWarps * 32) {
-                    const int r = i / (HD / 8), ch = i % (HD / 8);
-                    const int t = (r0 + r) / p.group, h = kvh * p.group + (r0 + r) % p.group;
-                    const char *src = p.q + (sh.row0 + t) * p.q_row + h * p.q_head + ch * 16;
-                    uint4 x;
-                    if (a.vec_q) {
-                        x = *reinterpret_cast<const uint4 *>(src);
-                    } else {
-                        uint32_t u[4];
+                constexpr int kCh = HD / 8, kQUnroll = kCh;  // 16-byte chunks of a row, loads in flight
+                for (int i0 = tid; i0 < rows * kCh; i0 += kSmWarps * 32 * kQUnroll) {
+                    uint4 x[kQUnroll];
 #pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            u[k] = (uint32_t)reinterpret_cast<const uint16_t *>(src)[2 * k] |
-                                   (uint32_t)reinterpret_cast<const uint16_t *>(src)[2 * k + 1] << 16;
-                        x = make_uint4(u[0], u[1], u[2], u[3]);
+                    for (int k = 0; k < kQUnroll; ++k) {
+                        const int i = i0 + k * kSmWarps * 32, r = r0 + i / kCh, t = r / p.group;
+                        if (i >= rows * kCh) break;
+                        const char *src = p.q + (sh.row0 + t) * p.q_row + (kvh * p.group + r - t * p.group) * p.q_head +
+                                          (i % kCh) * 16;
+                        if (a.vec_q) {
+                            x[k] = *reinterpret_cast<const uint4 *>(src);
+                        } else {
+                            const uint16_t *e = reinterpret_cast<const uint16_t *>(src);
+                            x[k] = make_uint4((uint32_t)e[0] | (uint32_t)e[1] << 16, (uint32_t)e[2] | (uint32_t)e[3] << 16,
+                                              (uint32_t)e[4] | (uint32_t)e[5] << 16, (uint32_t)e[6] | (uint32_t)e[7] << 16);
+                        }
                     }
-                    x.x ^= a.q_sign, x.y ^= a.q_sign, x.z ^= a.q_sign, x.w ^= a.q_sign;
-                    *reinterpret_cast<uint4 *>(smem + L::q + (ch >> 3) * L::kPanel + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = x;
+#pragma unroll
+                    for (int k = 0; k < kQUnroll; ++k) {
+                        const int i = i0 + k * kSmWarps * 32, r = i / kCh, ch = i % kCh;
+                        if (i >= rows * kCh) break;
+                        x[k].x ^= a.q_sign, x[k].y ^= a.q_sign, x[k].z ^= a.q_sign, x[k].w ^= a.q_sign;
+                        *reinterpret_cast<uint4 *>(smem + L::q + (ch >> 3) * L::kPanel + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) =
+                            x[k];
+                    }
                 }
                 tc::fence_proxy_async_smem();
                 __syncwarp();
@@ -455,26 +501,34 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (!ok) break;
                     if (active) {
                         tc::tc_fence_after();
-                        auto seen = [&](int col) -> bool {
-                            const long long d = k0 + col - sh.ctx;
-                            return d < 0 || (d < sh.nodes && k0 + col < sh.total && ((mask >> d) & 1));
-                        };
-                        float mt = -INFINITY;
+                        float s[4][32];
 #pragma unroll
-                        for (int ch = 0; ch < kTile / 32; ++ch) {
-                            float s[32];
-                            tc::tmem_ld32(tS + (uint32_t)(ch * 32), s);
-                            if (tail) {
-#pragma unroll
-                                for (int i = 0; i < 32; ++i) s[i] = seen(ch * 32 + i) ? s[i] : -INFINITY;
+                        for (int ch = 0; ch < 4; ++ch)
+                            tc::tmem_ld32_async(tS + (uint32_t)(ch * 32), reinterpret_cast<uint32_t(&)[32]>(s[ch]));
+                        tc::tmem_wait_ld();
+                        if (tail) {
+                            // bit i: the row sees key k0 + i -- the context, and the drafts of its mask
+                            const long long d0 = sh.ctx - k0;  // the first draft's column
+                            const int avail = (int)(sh.total - sh.ctx);
+                            const unsigned long long m = avail >= 64 ? mask : mask & ((1ull << avail) - 1);
+                            unsigned long long v0 = ~0ull, v1 = ~0ull;
+                            if (d0 < 128) {
+                                const int d = d0 < -64 ? -64 : (int)d0;
+                                v0 = d >= 64 ? ~0ull : d > 0 ? ((1ull << d) - 1) | m << d : d > -64 ? m >> -d : 0;
+                                v1 = d > 64 ? ((1ull << (d - 64)) - 1) | m << (d - 64) : d == 64 ? m : d > 0 ? m >> (64 - d) : 0;
                             }
-                            float x[4] = {s[0], s[1], s[2], s[3]};
+                            const uint32_t vis[4] = {(uint32_t)v0, (uint32_t)(v0 >> 32), (uint32_t)v1, (uint32_t)(v1 >> 32)};
 #pragma unroll
-                            for (int i = 4; i < 32; ++i) x[i & 3] = fmaxf(x[i & 3], s[i]);
-                            mt = fmaxf(mt, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
+                            for (int ch = 0; ch < 4; ++ch)
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) s[ch][i] = (vis[ch] & (1u << i)) ? s[ch][i] : -INFINITY;
                         }
-                        mt *= c2;
-                        if (c2 == 0.f) mt = 0.f;  // 0 * inf
+                        float x[4] = {s[0][0], s[1][0], s[2][0], s[3][0]};
+#pragma unroll
+                        for (int i = 1; i < 32; ++i)
+#pragma unroll
+                            for (int ch = 0; ch < 4; ++ch) x[ch] = fmaxf(x[ch], s[ch][i]);
+                        const float mt = c2 * fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
                         const bool raise = mt > m_run + kRaise || (m_run == -INFINITY && mt > m_run);
                         if (__any_sync(0xffffffffu, raise)) {
                             const float alpha = raise ? ex2(m_run - mt) : 1.0f;
@@ -498,36 +552,22 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                         const float base = m_run == -INFINITY ? 0.f : m_run;
                         const float2 c22 = f2(c2, c2), base2 = f2(-base, -base);
-                        float2 sum = f2(0.f, 0.f);
+                        float2 sum[4];
 #pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-                            uint32_t pk[32];
+                        for (int ch = 0; ch < 4; ++ch) {
+                            uint32_t pk[16];
+                            sum[ch] = f2(0.f, 0.f);
 #pragma unroll
-                            for (int ch = 0; ch < 2; ++ch) {
-                                const int col = half * 64 + ch * 32;
-                                float s[32];
-                                tc::tmem_ld32(tS + (uint32_t)col, s);
-                                if (tail) {
-#pragma unroll
-                                    for (int i = 0; i < 32; ++i) s[i] = seen(col + i) ? s[i] : -INFINITY;
-                                }
-#pragma unroll
-                                for (int i = 0; i < 32; i += 2) {
-                                    const float2 x = ffma2(f2(s[i], s[i + 1]), c22, base2);
-                                    float p0 = ex2(x.x), p1 = ex2(x.y);
-                                    if (tail) {  // -inf * 0 is not a weight
-                                        p0 = s[i] == -INFINITY ? 0.f : p0;
-                                        p1 = s[i + 1] == -INFINITY ? 0.f : p1;
-                                    }
-                                    const __nv_bfloat162 h = __floats2bfloat162_rn(p0, p1);
-                                    const uint32_t u = *reinterpret_cast<const uint32_t *>(&h);
-                                    pk[ch * 16 + i / 2] = u;
-                                    sum = fadd2(sum, f2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u)));
-                                }
+                            for (int i = 0; i < 32; i += 2) {
+                                const float2 y = ffma2(f2(s[ch][i], s[ch][i + 1]), c22, base2);
+                                const uint32_t u = pack_bf16(ex2(y.x), ex2(y.y));
+                                pk[i / 2] = u;
+                                sum[ch] = fadd2(sum[ch], f2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u)));
                             }
-                            tc::tmem_st32(tS + (uint32_t)(half * 32), pk);
+                            tmem_st16(tS + (uint32_t)(ch * 16), pk);
                         }
-                        l += sum.x + sum.y;
+                        sum[0] = fadd2(fadd2(sum[0], sum[1]), fadd2(sum[2], sum[3]));
+                        l += sum[0].x + sum[0].y;
                         tc::tmem_wait_st();
                         tc::tc_fence_before();
                     }
@@ -547,8 +587,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const int t = (r0 + row) / p.group, h = kvh * p.group + (r0 + row) % p.group;
                     const float inv = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
                     const long long at = ((long long)(c * 2 + (w.from_before ? 0 : 1)) * kRows + row);
-                    char *dst = whole ? p.out + (sh.row0 + t) * p.out_row + h * p.out_head
-                                      : reinterpret_cast<char *>(a.part_o + at * HD);
+                    char *dst = p.out + (sh.row0 + t) * p.out_row + h * p.out_head;
+                    float *part = a.part_o + (at - row) * HD + row;  // column-major: a warp's rows are adjacent
 #pragma unroll 1
                     for (int ch = 0; ch < HD / 32; ++ch) {
                         float o[32];
@@ -571,29 +611,19 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if (row < rows && whole) {
                             uint32_t u[16];
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) {
-                                const __nv_bfloat162 x = __floats2bfloat162_rn(o[2 * i] * inv, o[2 * i + 1] * inv);
-                                u[i] = *reinterpret_cast<const uint32_t *>(&x);
-                            }
-                            if (a.vec_out) {
-#pragma unroll
-                                for (int i = 0; i < 16; i += 4)
-                                    reinterpret_cast<uint4 *>(dst + ch * 64)[i / 4] = make_uint4(u[i], u[i + 1], u[i + 2], u[i + 3]);
-                            } else {
-#pragma unroll
-                                for (int i = 0; i < 16; ++i) {
-                                    reinterpret_cast<uint16_t *>(dst + ch * 64)[2 * i] = (uint16_t)u[i];
-                                    reinterpret_cast<uint16_t *>(dst + ch * 64)[2 * i + 1] = (uint16_t)(u[i] >> 16);
-                                }
-                            }
+                            for (int i = 0; i < 16; ++i) u[i] = pack_bf16(o[2 * i] * inv, o[2 * i + 1] * inv);
+                            write_row(dst + ch * 64, u, a.vec_out);
                         } else if (row < rows) {
 #pragma unroll
-                            for (int i = 0; i < 32; i += 4)
-                                reinterpret_cast<float4 *>(dst + ch * 128)[i / 4] = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                            for (int i = 0; i < 32; ++i) part[(ch * 32 + i) * kRows] = o[i];
                         }
                         __syncwarp();  // tcgen05.ld is the whole warp's
                     }
                     if (!whole && row < rows) a.part_ml[at * 2] = m_run, a.part_ml[at * 2 + 1] = l;
+                    if (!whole && !w.from_before && row == 0) {
+                        const long long end = lo + count + (w.w.tiles - w.te) - 1;  // the unit's last tile
+                        a.shared[c] = Shared{(int)(((end + 1) * g + total - 1) / total) - 1, sh.row0, kvh, r0, rows};
+                    }
                     tc::tc_fence_before();
                 }
             }
@@ -605,45 +635,53 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == kMmaWarp) tc::tmem_dealloc(tmem_base, kTmemCols);
 }
 
-// Joins the units that several CTAs shared: a warp per (node, query head) of sequence blockIdx.y;
-// `grid` is the first kernel's.
+// Joins the unit that CTA blockIdx.x of the first kernel left unfinished, kJoinCols columns: a row per
+// thread.  Many small blocks and several CTAs' sums in flight per thread: a unit shared by all the
+// SMs' CTAs is read at L2 speed, not one latency per CTA.
+constexpr int kJoinCols = 8, kJoinUnroll = 4;
 template <int HD>
-__global__ void __launch_bounds__(256) tree_join_tc_kernel(const TcParams a, int grid) {
-    constexpr int kCols = HD / 32;
-    __shared__ long long warp_sum[8];
+__global__ void __launch_bounds__(kRows) tree_join_tc_kernel(const TcParams a) {
     const TreeParams &p = a.t;
     pdl_wait();
     pdl_trigger();
-    const int seq = blockIdx.y, lane = threadIdx.x & 31, item = blockIdx.x * 8 + (threadIdx.x >> 5);
-    const long long total = block_total(p, a.n_seq, warp_sum), before = block_total(p, seq, warp_sum);
-    const SeqWork w = seq_work(p, seq);
-    const int t = item / p.n_q, head = item % p.n_q;
-    if (t >= w.sh.nodes) return;
-    const int r = t * p.group + head % p.group, unit = head / p.group * w.row_tiles + r / kRows;
-    const int g = shares(total, grid);
-    const long long begin = before + unit * w.tiles, last = begin + w.tiles - 1;
-    const int c0 = (int)(((begin + 1) * g + total - 1) / total) - 1, c1 = (int)(((last + 1) * g + total - 1) / total) - 1;
-    if (c0 == c1) return;  // written by its CTA
-    const auto slot = [&](int c) -> long long {
-        return (long long)(c * 2 + (first_tile(total, c, g) > begin ? 0 : 1)) * kRows + r % kRows;
-    };
-    float m = -INFINITY;
-    for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, a.part_ml[slot(c) * 2]);
+    const int c0 = blockIdx.x, row = threadIdx.x, col = blockIdx.y * kJoinCols;
+    const Shared u = a.shared[c0];
+    if (u.last < 0 || row >= u.rows) return;
+    const auto slot = [&](int c) -> long long { return c == c0 ? c * 2 + 1 : c * 2; };
+    const auto ml_of = [&](int c) { return reinterpret_cast<const float2 *>(a.part_ml)[slot(c) * kRows + row]; };
+    float o[kJoinCols] = {}, l = 0.f, m = -INFINITY;
+    for (int c = c0; c <= u.last; c += kJoinUnroll) {
+        float2 ml[kJoinUnroll];
+        float x[kJoinUnroll][kJoinCols];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float base = m == -INFINITY ? 0.f : m;
-    float o[kCols] = {}, l = 0.f;
-#pragma unroll 4
-    for (int c = c0; c <= c1; ++c) {
-        const long long s = slot(c);
-        const float f = exp2f(a.part_ml[s * 2] - base);
-        l = fmaf(f, a.part_ml[s * 2 + 1], l);
+        for (int k = 0; k < kJoinUnroll; ++k) {
+            ml[k] = c + k <= u.last ? ml_of(c + k) : make_float2(-INFINITY, 0.f);
 #pragma unroll
-        for (int i = 0; i < kCols; ++i) o[i] = fmaf(f, a.part_o[s * HD + lane * kCols + i], o[i]);
+            for (int i = 0; i < kJoinCols; ++i)
+                x[k][i] = c + k <= u.last ? a.part_o[(slot(c + k) * HD + col + i) * kRows + row] : 0.f;
+        }
+        float top = m;
+#pragma unroll
+        for (int k = 0; k < kJoinUnroll; ++k) top = fmaxf(top, ml[k].x);
+        const float base = top == -INFINITY ? 0.f : top, old = ex2(m - base);
+        m = top;
+        l *= old;
+#pragma unroll
+        for (int i = 0; i < kJoinCols; ++i) o[i] *= old;
+#pragma unroll
+        for (int k = 0; k < kJoinUnroll; ++k) {
+            const float f = ex2(ml[k].x - base);
+            l = fmaf(f, ml[k].y, l);
+#pragma unroll
+            for (int i = 0; i < kJoinCols; ++i) o[i] = fmaf(f, x[k][i], o[i]);
+        }
     }
-    __nv_bfloat16 *dst = reinterpret_cast<__nv_bfloat16 *>(p.out + (w.sh.row0 + t) * p.out_row + head * p.out_head) + lane * kCols;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int t = (u.r0 + row) / p.group, head = u.kvh * p.group + (u.r0 + row) % p.group;
+    uint32_t w[kJoinCols / 2];
 #pragma unroll
-    for (int i = 0; i < kCols; ++i) store(dst + i, l == 0.f ? 0.f : o[i] / l);
+    for (int i = 0; i < kJoinCols / 2; ++i) w[i] = pack_bf16(o[2 * i] * inv, o[2 * i + 1] * inv);
+    write_row(p.out + (u.row0 + t) * p.out_row + head * p.out_head + col * 2, w, a.vec_out);
 }
 
 // [page][slot][head][64-column panel] of K or V
@@ -673,22 +711,22 @@ cudaError_t run_tc(const CUtensorMap &k, const CUtensorMap &v, const TcParams &a
     PdlScope pdl;
     e = launch_kernel(kern, dim3(grid), dim3(kThreads), Smem<HD>::bytes, st, k, v, a);
     if (e != cudaSuccess) return e;
-    return launch_kernel(tree_join_tc_kernel<HD>, dim3((a.t.max_tree * a.t.n_q + 7) / 8, a.n_seq), dim3(256), 0, st, a, grid);
+    return launch_kernel(tree_join_tc_kernel<HD>, dim3(grid, HD / kJoinCols), dim3(kRows), 0, st, a);
 }
 
 }  // namespace
 
 // Boxes of whole 8-row swizzle groups: a page of 8 to 128 slots that tiles 128 keys, or a multiple of
-// 128 slots.  Strides within the tensor map's 2^40 bytes, sequences within the join's grid.
+// 128 slots.  Strides within the tensor map's 2^40 bytes.
 bool tree_attention_tc_supported(const pyxis_tree_attention_args &a, const pyxis_kv_pages &kv) {
     const int64_t most = (int64_t)1 << 38;
     return kv.dtype == PYXIS_DTYPE_BF16 && kv.page_size % 8 == 0 &&
-           (kTile % kv.page_size == 0 || kv.page_size % kTile == 0) && a.n_seq <= 65535 && kv.page_stride < most &&
+           (kTile % kv.page_size == 0 || kv.page_size % kTile == 0) && kv.page_stride < most &&
            kv.slot_stride < most && kv.head_stride < most;
 }
 
 size_t tree_attention_tc_workspace(const pyxis_kv_pages &kv, int num_sms) {
-    return (size_t)num_sms * 2 * kRows * (kv.head_dim + 2) * 4;
+    return (size_t)num_sms * (2 * kRows * (kv.head_dim + 2) * 4 + sizeof(Shared));
 }
 
 cudaError_t launch_tree_attention_tc(const TreeParams &p, const pyxis_tree_attention_args &args, const pyxis_kv_pages &kv,
@@ -706,6 +744,7 @@ cudaError_t launch_tree_attention_tc(const TreeParams &p, const pyxis_tree_atten
     a.q_sign = p.scale2 < 0.f ? 0x80008000u : 0u;
     a.part_o = (float *)workspace;
     a.part_ml = a.part_o + (size_t)num_sms * 2 * kRows * kv.head_dim;
+    a.shared = reinterpret_cast<Shared *>(a.part_ml + (size_t)num_sms * 2 * kRows * 2);
     CUtensorMap k, v;
     if (!make_map(&k, kv.k, kv, a.box_rows) || !make_map(&v, kv.v, kv, a.box_rows)) return cudaErrorInvalidValue;
     return kv.head_dim == 128 ? run_tc<128>(k, v, a, num_sms, st) : run_tc<64>(k, v, a, num_sms, st);
