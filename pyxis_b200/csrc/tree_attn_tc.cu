@@ -13,9 +13,11 @@
 // sequences load all SMs alike.  A unit inside one CTA is written out at once; one that several
 // CTAs share leaves unnormalised partial sums (at most two per CTA) that a second kernel joins.
 //
-// Warps: 0 producer, 1 MMA issuer (and TMEM owner), 2-5 softmax, a row per thread.
-//   producer   a tile's pages by TMA (one box per page and 64 columns, 128-byte swizzle) through a
-//              ring of tiles in the order S_0, S_1, O_0, S_2, O_1, ... of the MMAs
+// Warps: 0 and 2 producers (of K and Q, and of V), 1 MMA issuer (and TMEM owner), 4-11 softmax: a row
+// per thread, half of a tile's keys per warp.
+//   producers  a tile's pages by TMA (one box per page and 64 columns, 128-byte swizzle) through a
+//              ring of tiles in the order S_0, S_1, O_0, S_2, O_1, ... of the MMAs; the next segment's
+//              Q rows by cp.async while the current one runs
 //   MMA        S_j into one of three TMEM buffers; O += P_j V_j with P_j from TMEM and V_j as an
 //              MN-major operand, as it lies in the cache
 //   softmax    reads S_j, masks the tiles that hold drafts or end inside, writes P_j over S_j.  The
@@ -34,27 +36,28 @@ namespace pyxis {
 namespace {
 
 constexpr int kRows = 128, kTile = 128;
-constexpr int kProdWarp = 0, kMmaWarp = 1, kSmWarp0 = 2, kSmWarps = 4;
+constexpr int kProdWarp = 0, kMmaWarp = 1, kProdWarpV = 2, kSmWarp0 = 4, kSmWarps = 8;
 constexpr int kThreads = (kSmWarp0 + kSmWarps) * 32;
 constexpr int kSBufs = 3;
 constexpr uint32_t kTmemCols = 512, kOCol = kSBufs * kTile;
 constexpr uint64_t kTimeoutNs = 2000000000ull;
 constexpr float kRaise = 8.0f;
 constexpr int kMinTiles = 2;  // tiles per CTA before the next CTA gets any
-enum { kErrProd = 0x711, kErrMma = 0x712, kErrSoft = 0x713, kErrDrain = 0x714 };
+enum { kErrProd = 0x711, kErrMma = 0x712, kErrSoft = 0x713, kErrDrain = 0x714, kErrAlign = 0x715 };
 
 template <int HD>
 struct Smem {
     static constexpr int kDB = HD / 64;                  // 64-column panels of a row
     static constexpr uint32_t kPanel = kTile * 128;      // 128 rows x 128 B
     static constexpr uint32_t kEntry = kDB * kPanel;     // a tile of K or of V
-    static constexpr int kRing = HD == 128 ? 6 : 12;
-    static constexpr uint32_t q = 0;
-    static constexpr uint32_t ring = q + kEntry;
+    static constexpr int kRing = HD == 128 ? 5 : 12;
+    static constexpr uint32_t q = 0;  // two buffers: the next segment's rows come while this one runs
+    static constexpr uint32_t ring = q + 2 * kEntry;
     static constexpr uint32_t bar = ring + kRing * kEntry;
-    static constexpr int kBars = 2 * kRing + 2 + 3 * kSBufs;
+    static constexpr int kBars = 2 * kRing + 5 + 3 * kSBufs;
     static constexpr uint32_t misc = bar + kBars * 8;
-    static constexpr uint32_t bytes = misc + 64 + 1024;  // + alignment slack
+    static constexpr uint32_t red = misc + 64;               // [2 tiles][2 halves][128 rows] f32
+    static constexpr uint32_t bytes = red + 2 * 2 * kRows * 4;
 };
 static_assert(Smem<128>::bytes <= 232448 && Smem<64>::bytes <= 232448, "227 KB of shared memory per CTA");
 
@@ -63,6 +66,7 @@ struct TcParams {
     int n_seq;
     int box_rows;       // rows of a TMA box: a page, or a tile of a larger page
     int tile_pages;     // boxes per tile
+    int page_tiles;     // tiles per page (1 for pages of up to 128 slots)
     int vec_q, vec_out; // 16-byte accesses to q's and out's rows
     uint32_t q_sign;    // flips q's signs for a negative scale
     float *part_o, *part_ml;  // [CTA][2][HD][128], [CTA][2][128][2]
@@ -98,6 +102,8 @@ PYXIS_DEVINL uint64_t desc_mn_sw128(uint32_t smem_addr, uint32_t panel) {
     d |= (uint64_t)2 << 61;
     return d;
 }
+PYXIS_DEVINL void named_bar(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
+
 // 2^x, denormal results as zero (a weight below 2^-126 of the largest).
 PYXIS_DEVINL float ex2(float x) {
     float r;
@@ -137,15 +143,15 @@ PYXIS_DEVINL void write_row(char *dst, const uint32_t (&u)[N], int vec) {
 struct SeqWork {
     SeqShape sh;
     int row_tiles, units;
-    long long tiles;
-    PYXIS_DEVINL long long work() const { return units * tiles; }
+    int tiles;
+    PYXIS_DEVINL long long work() const { return (long long)units * tiles; }
 };
 PYXIS_DEVINL SeqWork seq_work(const TreeParams &p, int seq) {
     SeqWork w;
     w.sh = seq_shape(p, seq);
     w.row_tiles = (w.sh.nodes * p.group + kRows - 1) / kRows;
     w.units = w.row_tiles * p.n_kv;
-    w.tiles = (w.sh.total + kTile - 1) / kTile;
+    w.tiles = (int)((w.sh.total + kTile - 1) / kTile);
     if (w.tiles < 1) w.tiles = 1;  // rows without keys still get their zeros
     return w;
 }
@@ -161,15 +167,16 @@ PYXIS_DEVINL long long first_tile(long long total, int c, int g) { return total 
 struct Walk {
     SeqWork w;
     int seq, unit;
-    long long tile, left;  // next tile of the unit, tiles left to this CTA
-    long long tb, te;      // the segment
+    long long left;        // tiles left to this CTA
+    int tile;              // next tile of the unit
+    int tb, te;            // the segment
     bool from_before;      // its unit began in an earlier CTA
     bool first;
     PYXIS_DEVINL void begin(const TreeParams &p, int seq0, long long offset, long long count) {
         seq = seq0;
         w = seq_work(p, seq);
         unit = (int)(offset / w.tiles);
-        tile = offset - unit * w.tiles;
+        tile = (int)(offset - (long long)unit * w.tiles);
         left = count;
         first = true;
     }
@@ -188,7 +195,7 @@ struct Walk {
         from_before = tile > 0;  // only the CTA's first segment can start inside a unit
         first = false;
         tb = tile;
-        te = w.tiles - tile < left ? w.tiles : tile + left;
+        te = w.tiles - tile < left ? w.tiles : tile + (int)left;
         left -= te - tb;
         tile = te;
         return true;
@@ -224,18 +231,23 @@ __global__ void __launch_bounds__(kThreads, 1)
                              const TcParams a) {
     using L = Smem<HD>;
     constexpr int kDB = L::kDB, kRing = L::kRing;
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    extern __shared__ __align__(1024) uint8_t smem[];
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::bar);
-    uint64_t *full = bars, *empty = bars + kRing, *qfull = bars + 2 * kRing, *drain = qfull + 1;
+    uint64_t *full = bars, *empty = bars + kRing, *qfull = bars + 2 * kRing, *qempty = qfull + 2, *drain = qempty + 2;
     // per score buffer: sfull (S_j landed), pfull (P_j written, V_j fit to be multiplied), odone (P_j V_j done)
     uint64_t *sfull = drain + 1, *pfull = sfull + kSBufs, *odone = pfull + kSBufs;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + L::misc);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::misc + 4);
-    volatile int *bad = reinterpret_cast<volatile int *>(smem + L::misc + 8);  // [2]: a draft's value was not finite
-    __shared__ long long warp_sum[kThreads / 32], start_off;
-    __shared__ int start_seq;
+    volatile int *bad = reinterpret_cast<volatile int *>(smem + L::misc + 8);  // [2]: 1 + the last segment of that parity with a draft's value that is not finite
+    long long &start_off = *reinterpret_cast<long long *>(smem + L::misc + 16);
+    int &start_seq = *reinterpret_cast<int *>(smem + L::misc + 24);
+    float *red = reinterpret_cast<float *>(smem + L::red);
+    long long *warp_sum = reinterpret_cast<long long *>(smem + L::ring);  // before the ring is used
     const TreeParams &p = a.t;
+    if (tc::smem_u32(smem) & 1023) {  // the swizzled tiles' alignment; there is no static shared memory before them
+        if (threadIdx.x == 0) atomicCAS(p.err, 0, kErrAlign);
+        return;
+    }
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
@@ -243,7 +255,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc::mbar_init(&full[s], 1);
             tc::mbar_init(&empty[s], 1);
         }
-        tc::mbar_init(qfull, kSmWarps);
+        for (int b = 0; b < 2; ++b) {
+            tc::mbar_init(&qfull[b], 1);
+            tc::mbar_init(&qempty[b], 1);
+        }
         tc::mbar_init(drain, 1);
         for (int b = 0; b < kSBufs; ++b) {
             tc::mbar_init(&sfull[b], 1);
@@ -290,56 +305,108 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncthreads();
         Walk w;
         w.begin(p, start_seq, start_off, count);
-        if (warp == kProdWarp) {
-            // ---------------------------------------------------------------- TMA producer
-            int e = 0;
+        if (warp == kProdWarp || warp == kProdWarpV) {
+            // ---------------------------------------------------------------- producers: K and Q, V
+            const bool is_k = warp == kProdWarp;
+            int e0 = 0, newest = -1;  // ring places of earlier segments; the latest place filled
             bool ok = true;
+            Walk ahead = w;  // one segment ahead: whose Q is loaded next
+            int qseg = 0;
+            bool q_pending = false;
+            auto wait = [&](uint64_t *bar, int phase) -> bool {
+                return __all_sync(0xffffffffu, tc::mbar_wait_bounded(bar, (uint32_t)(phase & 1), abort_flag, p.err, kErrProd,
+                                                                     kTimeoutNs));
+            };
+            // Q of the next segment, 16 bytes per copy, in the 128-byte swizzle; rows past the unit's
+            // are left as they are (their lanes' results are never written)
+            auto load_q = [&]() -> bool {
+                if (!ahead.next(p, a.n_seq)) return true;
+                const int b = qseg & 1;
+                if (!wait(&qempty[b], qseg / 2 - 1)) return false;
+                uint8_t *dst = smem + L::q + b * L::kEntry;
+                constexpr int kCh = HD / 8;  // 16-byte chunks of a row; a lane keeps its chunk
+                const int r0 = ahead.row0(), rows = min(ahead.w.sh.nodes * p.group - r0, kRows), ch = lane % kCh;
+                const char *head0 = p.q + ahead.w.sh.row0 * p.q_row + ahead.kvh() * p.group * p.q_head + ch * 16;
+                for (int r = lane / kCh; r < rows; r += 32 / kCh) {
+                    const int t = (r0 + r) / p.group, h = r0 + r - t * p.group;
+                    const char *src = head0 + t * p.q_row + h * p.q_head;
+                    uint8_t *at = dst + (ch >> 3) * L::kPanel + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
+                    if (a.vec_q) {
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(tc::smem_u32(at)), "l"(src) : "memory");
+                    } else {
+                        const uint16_t *e = reinterpret_cast<const uint16_t *>(src);
+                        uint32_t x[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) x[k] = ((uint32_t)e[2 * k] | (uint32_t)e[2 * k + 1] << 16) ^ a.q_sign;
+                        *reinterpret_cast<uint4 *>(at) = make_uint4(x[0], x[1], x[2], x[3]);
+                    }
+                }
+                q_pending = true;
+                return true;
+            };
+            auto finish_q = [&]() {
+                if (!q_pending) return;
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                tc::fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&qfull[qseg & 1]);
+                ++qseg;
+                q_pending = false;
+            };
+            if (is_k) ok = load_q();
             while (ok && w.next(p, a.n_seq)) {
-                const int T = (int)(w.te - w.tb), kvh = w.kvh();
+                const int T = w.te - w.tb, kvh = w.kvh();
                 const int32_t *table = p.block_table + w.seq * p.table_stride;
-                // this lane's page of tile tb + j (-1: none), and how many of the tile's pages exist
+                // how many of the pages of tile tb + j exist, and this lane's
                 auto page_count = [&](int j) -> int {
-                    const long long rest = w.w.sh.total - (w.tb + j) * kTile;
-                    if (rest <= 0 || j >= T) return 0;
-                    const long long n = (rest + a.box_rows - 1) / a.box_rows;
-                    return (int)(n < a.tile_pages ? n : a.tile_pages);
+                    if (j >= T) return 0;
+                    const long long rest = w.w.sh.total - (long long)(w.tb + j) * kTile;
+                    if (rest >= kTile) return a.tile_pages;
+                    return rest <= 0 ? 0 : ((int)rest + a.box_rows - 1) / a.box_rows;
                 };
                 auto page_of = [&](int j) -> int {
                     if (lane >= page_count(j)) return 0;
-                    const int id = __ldg(table + ((w.tb + j) * kTile + lane * a.box_rows) / p.page_size);
+                    const int t = w.tb + j;
+                    const int id = __ldg(table + (a.page_tiles == 1 ? t * a.tile_pages + lane : t / a.page_tiles));
                     return min(max(id, 0), p.num_pages - 1);
                 };
-                auto issue = [&](bool is_k, int j, int page) -> bool {
-                    const int s = e % kRing;
-                    if (e >= kRing && !__all_sync(0xffffffffu, tc::mbar_wait_bounded(&empty[s], (uint32_t)((e / kRing - 1) & 1),
-                                                                                      abort_flag, p.err, kErrProd, kTimeoutNs)))
-                        return false;
+                auto issue = [&](int j, int page) -> bool {
+                    const int e = e0 + (is_k ? (j == 0 ? 0 : 2 * j - 1) : (j == T - 1 ? 2 * T - 1 : 2 * j + 2));
+                    const int slot = e % kRing;
+                    if (!wait(&empty[slot], e / kRing - 1)) return false;
                     const int n = page_count(j);
-                    if (lane == 0) tc::mbar_arrive_expect_tx(&full[s], (uint32_t)(n * a.box_rows * HD * 2));
+                    if (lane == 0) tc::mbar_arrive_expect_tx(&full[slot], (uint32_t)(n * a.box_rows * HD * 2));
                     __syncwarp();
                     if (lane < n) {
-                        uint8_t *dst = smem + L::ring + s * L::kEntry + lane * a.box_rows * 128;
-                        const int slot = (int)(((w.tb + j) * kTile + lane * a.box_rows) % p.page_size);
+                        uint8_t *dst = smem + L::ring + slot * L::kEntry + lane * a.box_rows * 128;
+                        const int row = a.page_tiles == 1 ? 0 : (w.tb + j) % a.page_tiles * kTile;
 #pragma unroll
                         for (int x = 0; x < kDB; ++x)
-                            tma_load_4d(dst + x * L::kPanel, is_k ? &tm_k : &tm_v, x * 64, kvh, slot, page, &full[s]);
+                            tma_load_4d(dst + x * L::kPanel, is_k ? &tm_k : &tm_v, x * 64, kvh, row, page, &full[slot]);
                     }
-                    ++e;
+                    newest = e;
                     return true;
                 };
-                int prev = 0, cur = page_of(0), next = page_of(1);
-                ok = issue(true, 0, cur);
-                for (int j = 1; ok && j < T; ++j) {
-                    prev = cur, cur = next, next = page_of(j + 1);
-                    ok = issue(true, j, cur) && issue(false, j - 1, prev);
+                int cur = page_of(0);
+                for (int j = 0; ok && j < T; ++j) {
+                    const int next = page_of(j + 1);
+                    ok = issue(j, cur);
+                    cur = next;
+                    if (is_k) {
+                        if (j > 0 || T == 1) finish_q();  // a tile's time after load_q
+                        if (ok && j == 2) ok = load_q();
+                    }
                 }
-                ok = ok && issue(false, T - 1, cur);
+                if (is_k) {
+                    finish_q();
+                    if (ok && T <= 2) ok = load_q();
+                }
+                e0 += 2 * T;
             }
             if (*abort_flag && lane == 0) {  // let the copies already issued land before the CTA exits
                 volatile int no_abort = 0;
-                for (int x = e > kRing ? e - kRing : 0; x < e; ++x)
-                    tc::mbar_wait_bounded(&full[x % kRing], (uint32_t)((x / kRing) & 1), &no_abort, p.err, kErrDrain,
-                                          100000000ull);
+                for (int e = max(0, newest - kRing + 1); e <= newest; ++e)
+                    tc::mbar_wait_bounded(&full[e % kRing], (uint32_t)((e / kRing) & 1), &no_abort, p.err, kErrDrain, 100000000ull);
             }
         } else if (warp == kMmaWarp) {
             // ---------------------------------------------------------------- MMA issuer
@@ -349,133 +416,107 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const uint64_t k_d = tc::desc_sw128(tc::smem_u32(smem + L::ring));
                 const uint64_t v_d = desc_mn_sw128(tc::smem_u32(smem + L::ring), L::kPanel);
                 const uint32_t tO = tmem_base + kOCol;
-                int e = 0, seg = 0;
-                long long n0 = 0;  // tiles of earlier segments
+                int slot = 0, fills = 0;   // ring
+                int sb = 0, suse = 0;      // score buffer of the next S, and how often it was used
+                int ob = 0, ouse = 0;      // of the next O
+                auto wait = [&](uint64_t *bar, int phase) -> bool {
+                    return tc::mbar_wait_bounded(bar, (uint32_t)(phase & 1), abort_flag, p.err, kErrMma, kTimeoutNs);
+                };
                 bool ok = true;
-                auto score = [&](long long n) -> bool {
-                    const int b = (int)(n % kSBufs), s = e % kRing;
-                    const long long use = n / kSBufs;
-                    // the buffer's earlier probabilities have been multiplied
-                    if (use > 0 && !tc::mbar_wait_bounded(&odone[b], (uint32_t)((use - 1) & 1), abort_flag, p.err, kErrMma,
-                                                          kTimeoutNs))
-                        return false;
-                    if (!tc::mbar_wait_bounded(&full[s], (uint32_t)((e / kRing) & 1), abort_flag, p.err, kErrMma, kTimeoutNs))
-                        return false;
+                auto score = [&](uint64_t qd) -> bool {
+                    // the buffer's earlier probabilities have been multiplied, and K is there
+                    if (!wait(&odone[sb], suse - 1) || !wait(&full[slot], fills)) return false;
                     tc::tc_fence_after();
-                    const uint32_t tS = tmem_base + (uint32_t)(b * kTile);
+                    const uint32_t tS = tmem_base + (uint32_t)(sb * kTile);
+                    const uint64_t kd = k_d + (uint64_t)(slot * (L::kEntry >> 4));
 #pragma unroll
                     for (int x = 0; x < kDB; ++x)
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk)
-                            tc::mma_f16(tS, q_d + (uint64_t)(x * (L::kPanel >> 4) + kk * 2),
-                                        k_d + (uint64_t)(s * (L::kEntry >> 4) + x * (L::kPanel >> 4) + kk * 2), idesc_s,
-                                        (uint32_t)(x | kk));
-                    tc::mma_commit(&empty[s]);
-                    tc::mma_commit(&sfull[b]);
-                    ++e;
+                            tc::mma_f16(tS, qd + (uint64_t)(x * (L::kPanel >> 4) + kk * 2),
+                                        kd + (uint64_t)(x * (L::kPanel >> 4) + kk * 2), idesc_s, (uint32_t)(x | kk));
+                    tc::mma_commit(&empty[slot]);
+                    tc::mma_commit(&sfull[sb]);
+                    if (++slot == kRing) slot = 0, ++fills;
+                    if (++sb == kSBufs) sb = 0, ++suse;
                     return true;
                 };
-                auto output = [&](long long n, bool add) -> bool {
-                    const int b = (int)(n % kSBufs), s = e % kRing;
-                    const long long use = n / kSBufs;
-                    if (!tc::mbar_wait_bounded(&full[s], (uint32_t)((e / kRing) & 1), abort_flag, p.err, kErrMma, kTimeoutNs) ||
-                        !tc::mbar_wait_bounded(&pfull[b], (uint32_t)(use & 1), abort_flag, p.err, kErrMma, kTimeoutNs))
-                        return false;
+                auto output = [&](bool add) -> bool {
+                    if (!wait(&full[slot], fills) || !wait(&pfull[ob], ouse)) return false;
                     tc::tc_fence_after();
-                    const uint32_t tS = tmem_base + (uint32_t)(b * kTile);
+                    const uint32_t tS = tmem_base + (uint32_t)(ob * kTile);
+                    const uint64_t vd = v_d + (uint64_t)(slot * (L::kEntry >> 4));
 #pragma unroll
                     for (int kk = 0; kk < kTile / 16; ++kk)  // 16 keys: 8 columns of P, 16 rows of V
-                        tc::mma_f16_ts(tO, tS + (uint32_t)(kk * 8), v_d + (uint64_t)(s * (L::kEntry >> 4) + kk * (2048 >> 4)),
-                                       idesc_o, (uint32_t)(add || kk > 0));
-                    tc::mma_commit(&empty[s]);
-                    tc::mma_commit(&odone[b]);
-                    ++e;
+                        tc::mma_f16_ts(tO, tS + (uint32_t)(kk * 8), vd + (uint64_t)(kk * (2048 >> 4)), idesc_o,
+                                       (uint32_t)(add || kk > 0));
+                    tc::mma_commit(&empty[slot]);
+                    tc::mma_commit(&odone[ob]);
+                    if (++slot == kRing) slot = 0, ++fills;
+                    if (++ob == kSBufs) ob = 0, ++ouse;
                     return true;
                 };
-                for (; ok && w.next(p, a.n_seq); ++seg) {
-                    const int T = (int)(w.te - w.tb);
-                    ok = tc::mbar_wait_bounded(qfull, (uint32_t)(seg & 1), abort_flag, p.err, kErrMma, kTimeoutNs) && score(n0);
-                    for (int j = 1; ok && j < T; ++j) ok = score(n0 + j) && output(n0 + j - 1, j > 1);
-                    ok = ok && output(n0 + T - 1, T > 1);
-                    n0 += T;
+                for (int seg = 0; ok && w.next(p, a.n_seq); ++seg) {
+                    const int T = w.te - w.tb;
+                    const uint64_t qd = q_d + (uint64_t)((seg & 1) * (L::kEntry >> 4));
+                    ok = wait(&qfull[seg & 1], seg >> 1) && score(qd);
+                    for (int j = 1; ok && j < T; ++j) {
+                        ok = score(qd);
+                        if (ok && j == T - 1) tc::mma_commit(&qempty[seg & 1]);
+                        ok = ok && output(j > 1);
+                    }
+                    if (ok && T == 1) tc::mma_commit(&qempty[seg & 1]);
+                    ok = ok && output(T > 1);
                 }
                 // every MMA this thread issued must complete before TMEM is released
                 tc::mma_commit(drain);
                 volatile int no_abort = 0;
                 tc::mbar_wait_bounded(drain, 0, &no_abort, p.err, kErrDrain, kTimeoutNs);
             }
-        } else {
+        } else if (warp >= kSmWarp0) {
             // ---------------------------------------------------------------- softmax
-            const int quad = warp & 3;  // TMEM lanes 32 quad .. 32 quad + 31
+            const int quad = warp & 3;                 // TMEM lanes 32 quad .. 32 quad + 31
+            const int half = (warp - kSmWarp0) >> 2;   // keys [64 half, +64) of each tile, columns [HD/2 half, +HD/2) of O
             const int row = quad * 32 + lane, tid = threadIdx.x - kSmWarp0 * 32;
             const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
-            const uint32_t tO = tmem_base + lane_off + kOCol;
+            const uint32_t tO = tmem_base + lane_off + kOCol, tOh = tO + (uint32_t)(half * (HD / 2));
             const float c2 = fmaxf(fabsf(p.scale2), 1e-37f);  // a masked score stays -inf with scale 0, too
-            auto wait = [&](uint64_t *bar, long long phase) -> bool {
+            auto wait = [&](uint64_t *bar, int phase) -> bool {
                 return __all_sync(0xffffffffu, tc::mbar_wait_bounded(bar, (uint32_t)(phase & 1), abort_flag, p.err, kErrSoft,
                                                                      kTimeoutNs));
             };
-            long long n0 = 0;
-            int seg = 0;
+            int b = 0, use = 0;    // score buffer and how often it was used
+            int n0 = 0, seg = 0;   // tiles of earlier segments
+            int swaps = 0;         // exchanges with the rows' other warp: they alternate between two buffers
             bool ok = true;
-            for (; ok && w.next(p, a.n_seq); ++seg) {
-                const int T = (int)(w.te - w.tb), kvh = w.kvh(), r0 = w.row0();
+            for (; w.next(p, a.n_seq); ++seg) {
+                const int T = w.te - w.tb, kvh = w.kvh(), r0 = w.row0();
                 const SeqShape &sh = w.w.sh;
                 const int rows = min(sh.nodes * p.group - r0, kRows);
                 const bool active = quad * 32 < rows;  // the warp has rows
-                // ---- Q of the segment; the last segment's MMAs are done (odone)
-                constexpr int kCh = HD / 8, kQUnroll = kCh;  // 16-byte chunks of a row, loads in flight
-                for (int i0 = tid; i0 < rows * kCh; i0 += kSmWarps * 32 * kQUnroll) {
-                    uint4 x[kQUnroll];
-#pragma unroll
-                    for (int k = 0; k < kQUnroll; ++k) {
-                        const int i = i0 + k * kSmWarps * 32, r = r0 + i / kCh, t = r / p.group;
-                        if (i >= rows * kCh) break;
-                        const char *src = p.q + (sh.row0 + t) * p.q_row + (kvh * p.group + r - t * p.group) * p.q_head +
-                                          (i % kCh) * 16;
-                        if (a.vec_q) {
-                            x[k] = *reinterpret_cast<const uint4 *>(src);
-                        } else {
-                            const uint16_t *e = reinterpret_cast<const uint16_t *>(src);
-                            x[k] = make_uint4((uint32_t)e[0] | (uint32_t)e[1] << 16, (uint32_t)e[2] | (uint32_t)e[3] << 16,
-                                              (uint32_t)e[4] | (uint32_t)e[5] << 16, (uint32_t)e[6] | (uint32_t)e[7] << 16);
-                        }
-                    }
-#pragma unroll
-                    for (int k = 0; k < kQUnroll; ++k) {
-                        const int i = i0 + k * kSmWarps * 32, r = i / kCh, ch = i % kCh;
-                        if (i >= rows * kCh) break;
-                        x[k].x ^= a.q_sign, x[k].y ^= a.q_sign, x[k].z ^= a.q_sign, x[k].w ^= a.q_sign;
-                        *reinterpret_cast<uint4 *>(smem + L::q + (ch >> 3) * L::kPanel + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) =
-                            x[k];
-                    }
-                }
-                tc::fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) tc::mbar_arrive(qfull);
                 unsigned long long mask = 0;
                 if (row < rows) {
                     const int t = (r0 + row) / p.group;
                     mask = p.tree_mask ? p.tree_mask[sh.row0 + t] : (2ull << t) - 1;
                 }
                 float m_run = -INFINITY, l = 0.f;
-                for (int j = 0; ok && j < T; ++j) {
-                    const long long n = n0 + j;
-                    const int b = (int)(n % kSBufs);
-                    const long long k0 = (w.tb + j) * kTile;
+                // after a failed wait the loops run on without work, so that the barriers of a row's two
+                // warps keep their counts
+                for (int j = 0; j < T; ++j) {
+                    const long long k0 = (long long)(w.tb + j) * kTile;
+                    const int pb = b == 0 ? kSBufs - 1 : b - 1, puse = b == 0 ? use - 1 : use;  // the tile before
                     const uint32_t tS = tmem_base + lane_off + (uint32_t)(b * kTile);
                     const bool tail = k0 + kTile > sh.ctx;
-                    if (tail) {
+                    if (tail && ok) {
                         // V_j: rows that hold no key become zero (their weights are zero, but what lies
                         // there may be anything), and so do a draft's values that are not finite: the
                         // rows that do see the draft get them back below
-                        const long long ve = 2 * n0 + (j == T - 1 ? 2 * T - 1 : 2 * j + 2);
+                        const int ve = 2 * n0 + (j == T - 1 ? 2 * T - 1 : 2 * j + 2);  // its place in the ring's order
                         ok = wait(&full[ve % kRing], ve / kRing);
-                        if (!ok) break;
                         uint8_t *v = smem + L::ring + (ve % kRing) * L::kEntry;
                         const int valid = (int)min((long long)kTile, max(sh.total - k0, 0ll));
                         const int drafts = (int)min((long long)valid, max(sh.ctx - k0, 0ll));  // first draft's row
-                        for (int i = tid; i < (kTile - drafts) * (HD / 8); i += kSmWarps * 32) {
+                        for (int i = tid; ok && i < (kTile - drafts) * (HD / 8); i += kSmWarps * 32) {
                             const int r = drafts + i / (HD / 8), ch = i % (HD / 8);
                             uint4 *at = reinterpret_cast<uint4 *>(v + (ch >> 3) * L::kPanel + r * 128 + ((ch & 7) << 4));
                             if (r >= valid) {
@@ -492,69 +533,72 @@ __global__ void __launch_bounds__(kThreads, 1)
                             }
                             if (any) {
                                 *at = x;
-                                bad[seg & 1] = 1;
+                                bad[seg & 1] = seg + 1;
                             }
                         }
                         tc::fence_proxy_async_smem();
                     }
-                    ok = wait(&sfull[b], n / kSBufs);
-                    if (!ok) break;
+                    ok = ok && wait(&sfull[b], use);
                     if (active) {
+                        float s[2][32];
+                        float mt = -INFINITY;
+                        if (ok) {
                         tc::tc_fence_after();
-                        float s[4][32];
 #pragma unroll
-                        for (int ch = 0; ch < 4; ++ch)
-                            tc::tmem_ld32_async(tS + (uint32_t)(ch * 32), reinterpret_cast<uint32_t(&)[32]>(s[ch]));
+                        for (int ch = 0; ch < 2; ++ch)
+                            tc::tmem_ld32_async(tS + (uint32_t)(half * 64 + ch * 32), reinterpret_cast<uint32_t(&)[32]>(s[ch]));
                         tc::tmem_wait_ld();
                         if (tail) {
-                            // bit i: the row sees key k0 + i -- the context, and the drafts of its mask
-                            const long long d0 = sh.ctx - k0;  // the first draft's column
+                            // bit i: the row sees key k0 + 64 half + i -- the context, and the drafts of its mask
+                            const long long d0 = sh.ctx - k0 - half * 64;  // the first draft's column
                             const int avail = (int)(sh.total - sh.ctx);
                             const unsigned long long m = avail >= 64 ? mask : mask & ((1ull << avail) - 1);
-                            unsigned long long v0 = ~0ull, v1 = ~0ull;
-                            if (d0 < 128) {
-                                const int d = d0 < -64 ? -64 : (int)d0;
-                                v0 = d >= 64 ? ~0ull : d > 0 ? ((1ull << d) - 1) | m << d : d > -64 ? m >> -d : 0;
-                                v1 = d > 64 ? ((1ull << (d - 64)) - 1) | m << (d - 64) : d == 64 ? m : d > 0 ? m >> (64 - d) : 0;
-                            }
-                            const uint32_t vis[4] = {(uint32_t)v0, (uint32_t)(v0 >> 32), (uint32_t)v1, (uint32_t)(v1 >> 32)};
+                            const unsigned long long vis = d0 >= 64 ? ~0ull : d0 > 0 ? ((1ull << d0) - 1) | m << d0 : d0 > -64 ? m >> -d0 : 0;
 #pragma unroll
-                            for (int ch = 0; ch < 4; ++ch)
+                            for (int ch = 0; ch < 2; ++ch)
 #pragma unroll
-                                for (int i = 0; i < 32; ++i) s[ch][i] = (vis[ch] & (1u << i)) ? s[ch][i] : -INFINITY;
+                                for (int i = 0; i < 32; ++i)
+                                    s[ch][i] = ((uint32_t)(vis >> (ch * 32)) & (1u << i)) ? s[ch][i] : -INFINITY;
                         }
-                        float x[4] = {s[0][0], s[1][0], s[2][0], s[3][0]};
+                        float x[4] = {s[0][0], s[0][1], s[1][0], s[1][1]};
 #pragma unroll
-                        for (int i = 1; i < 32; ++i)
+                        for (int i = 2; i < 32; ++i)
 #pragma unroll
-                            for (int ch = 0; ch < 4; ++ch) x[ch] = fmaxf(x[ch], s[ch][i]);
-                        const float mt = c2 * fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+                            for (int ch = 0; ch < 2; ++ch) x[ch * 2 + (i & 1)] = fmaxf(x[ch * 2 + (i & 1)], s[ch][i]);
+                        mt = c2 * fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+                        }
+                        // the row's maximum over both halves; past this barrier both have read S, so P may
+                        // be written over it
+                        float *rd = red + (swaps++ & 1) * 2 * kRows;
+                        rd[half * kRows + row] = mt;
+                        named_bar(1 + quad, 64);
+                        mt = fmaxf(mt, rd[(1 - half) * kRows + row]);
                         const bool raise = mt > m_run + kRaise || (m_run == -INFINITY && mt > m_run);
+                        if (ok) {
                         if (__any_sync(0xffffffffu, raise)) {
                             const float alpha = raise ? ex2(m_run - mt) : 1.0f;
                             if (raise) m_run = mt, l *= alpha;
                             if (j > 0) {
                                 // O of the tiles before, in TMEM, once they are all in
-                                ok = wait(&odone[(n - 1) % kSBufs], (n - 1) / kSBufs);
-                                if (!ok) break;
+                                ok = wait(&odone[pb], puse);
                                 tc::tc_fence_after();
 #pragma unroll
-                                for (int ch = 0; ch < HD / 32; ++ch) {
+                                for (int ch = 0; ch < HD / 64; ++ch) {
                                     uint32_t o[32];
-                                    tc::tmem_ld32_async(tO + (uint32_t)(ch * 32), o);
+                                    tc::tmem_ld32_async(tOh + (uint32_t)(ch * 32), o);
                                     tc::tmem_wait_ld();
 #pragma unroll
                                     for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-                                    tc::tmem_st32(tO + (uint32_t)(ch * 32), o);
+                                    tc::tmem_st32(tOh + (uint32_t)(ch * 32), o);
                                 }
                                 tc::tmem_wait_st();
                             }
                         }
                         const float base = m_run == -INFINITY ? 0.f : m_run;
                         const float2 c22 = f2(c2, c2), base2 = f2(-base, -base);
-                        float2 sum[4];
+                        float2 sum[2];
 #pragma unroll
-                        for (int ch = 0; ch < 4; ++ch) {
+                        for (int ch = 0; ch < 2; ++ch) {
                             uint32_t pk[16];
                             sum[ch] = f2(0.f, 0.f);
 #pragma unroll
@@ -564,40 +608,43 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 pk[i / 2] = u;
                                 sum[ch] = fadd2(sum[ch], f2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u)));
                             }
-                            tmem_st16(tS + (uint32_t)(ch * 16), pk);
+                            tmem_st16(tS + (uint32_t)(half * 32 + ch * 16), pk);
                         }
-                        sum[0] = fadd2(fadd2(sum[0], sum[1]), fadd2(sum[2], sum[3]));
+                        sum[0] = fadd2(sum[0], sum[1]);
                         l += sum[0].x + sum[0].y;
                         tc::tmem_wait_st();
                         tc::tc_fence_before();
+                        }
                     }
-                    // the next segment's flag: every warp has read it (two segments ago, before it
-                    // loaded this one's Q), none is past this segment before this arrival
-                    if (j == T - 1 && tid == 0) bad[(seg + 1) & 1] = 0;
                     __syncwarp();
                     if (lane == 0) tc::mbar_arrive(&pfull[b]);
+                    if (++b == kSBufs) b = 0, ++use;
                 }
-                if (!ok) break;
                 n0 += T;
-                ok = wait(&odone[(n0 - 1) % kSBufs], (n0 - 1) / kSBufs);
-                if (!ok) break;
+                ok = ok && wait(&odone[b == 0 ? kSBufs - 1 : b - 1], b == 0 ? use - 1 : use);
                 if (active) {
+                    float *rd = red + (swaps++ & 1) * 2 * kRows;
+                    rd[half * kRows + row] = l;
+                    named_bar(1 + quad, 64);
+                    l += rd[(1 - half) * kRows + row];
+                }
+                if (active && ok) {
                     tc::tc_fence_after();
-                    const bool fix = bad[seg & 1] != 0, whole = w.whole();
+                    const bool fix = bad[seg & 1] == seg + 1, whole = w.whole();
                     const int t = (r0 + row) / p.group, h = kvh * p.group + (r0 + row) % p.group;
                     const float inv = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
                     const long long at = ((long long)(c * 2 + (w.from_before ? 0 : 1)) * kRows + row);
                     char *dst = p.out + (sh.row0 + t) * p.out_row + h * p.out_head;
                     float *part = a.part_o + (at - row) * HD + row;  // column-major: a warp's rows are adjacent
 #pragma unroll 1
-                    for (int ch = 0; ch < HD / 32; ++ch) {
+                    for (int ch = half * (HD / 64); ch < (half + 1) * (HD / 64); ++ch) {
                         float o[32];
                         tc::tmem_ld32(tO + (uint32_t)(ch * 32), o);
                         // the drafts' values that are not finite, for the rows that see them
                         if (fix && row < rows)
                             for (int d = 0; d < sh.nodes; ++d) {
                                 const long long pos = sh.ctx + d;
-                                if (!((mask >> d) & 1) || pos >= sh.total || pos < w.tb * kTile || pos >= w.te * kTile) continue;
+                                if (!((mask >> d) & 1) || pos >= sh.total || pos < (long long)w.tb * kTile || pos >= (long long)w.te * kTile) continue;
                                 const int page = min(max(p.block_table[w.seq * p.table_stride + pos / p.page_size], 0),
                                                      p.num_pages - 1);
                                 const __nv_bfloat16 *v = reinterpret_cast<const __nv_bfloat16 *>(
@@ -619,8 +666,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                         __syncwarp();  // tcgen05.ld is the whole warp's
                     }
-                    if (!whole && row < rows) a.part_ml[at * 2] = m_run, a.part_ml[at * 2 + 1] = l;
-                    if (!whole && !w.from_before && row == 0) {
+                    if (!whole && half == 0 && row < rows) a.part_ml[at * 2] = m_run, a.part_ml[at * 2 + 1] = l;
+                    if (!whole && half == 0 && !w.from_before && row == 0) {
                         const long long end = lo + count + (w.w.tiles - w.te) - 1;  // the unit's last tile
                         a.shared[c] = Shared{(int)(((end + 1) * g + total - 1) / total) - 1, sh.row0, kvh, r0, rows};
                     }
@@ -736,12 +783,13 @@ cudaError_t launch_tree_attention_tc(const TreeParams &p, const pyxis_tree_atten
     a.n_seq = (int)args.n_seq;
     a.box_rows = std::min(kv.page_size, kTile);
     a.tile_pages = kTile / a.box_rows;
+    a.page_tiles = std::max(1, kv.page_size / kTile);
     const auto vec = [](const void *base, int64_t row, int64_t head) {
         return (reinterpret_cast<uintptr_t>(base) & 15) == 0 && row % 8 == 0 && head % 8 == 0;
     };
-    a.vec_q = vec(args.q, args.q_row, args.q_head);
-    a.vec_out = vec(args.out, args.out_row, args.out_head);
     a.q_sign = p.scale2 < 0.f ? 0x80008000u : 0u;
+    a.vec_q = a.q_sign == 0 && vec(args.q, args.q_row, args.q_head);
+    a.vec_out = vec(args.out, args.out_row, args.out_head);
     a.part_o = (float *)workspace;
     a.part_ml = a.part_o + (size_t)num_sms * 2 * kRows * kv.head_dim;
     a.shared = reinterpret_cast<Shared *>(a.part_ml + (size_t)num_sms * 2 * kRows * 2);
