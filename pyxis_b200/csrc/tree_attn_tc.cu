@@ -104,6 +104,13 @@ PYXIS_DEVINL uint64_t desc_mn_sw128(uint32_t smem_addr, uint32_t panel) {
 }
 PYXIS_DEVINL void named_bar(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
 
+// True in one lane of the (converged) warp.
+PYXIS_DEVINL bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
+    return r != 0;
+}
+
 // 2^x, denormal results as zero (a weight below 2^-126 of the largest).
 PYXIS_DEVINL float ex2(float x) {
     float r;
@@ -410,7 +417,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         } else if (warp == kMmaWarp) {
             // ---------------------------------------------------------------- MMA issuer
-            if (lane == 0) {
+            if (elect_one()) {
                 constexpr uint32_t idesc_s = idesc_bf16(kRows, kTile, false), idesc_o = idesc_bf16(kRows, HD, true);
                 const uint64_t q_d = tc::desc_sw128(tc::smem_u32(smem + L::q));
                 const uint64_t k_d = tc::desc_sw128(tc::smem_u32(smem + L::ring));
