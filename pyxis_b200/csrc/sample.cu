@@ -7,11 +7,17 @@
 // nothing is sorted and no mask is kept; three times at most one element of the order is located
 // -- by count (the k-th), by weight (p Z_k) and by weight (u Z).
 //
-// A cluster of CTAs holds a row in shared memory (one pass over HBM) and histograms it by
-// (max - x) / temperature in bins of 1/64 nat, weights and counts.  The leader CTA finds the bin
-// that holds the element sought, the cluster gathers the bin's elements into the leader's shared
-// memory, and the leader sorts and scans them.  A bin of more elements than that holds (flat or
-// heavily tied rows) is first cut down by histograms over the 64-bit (value, index) key.
+// A cluster of CTAs holds a row in shared memory (one pass over HBM).  Elements are located in two
+// steps: the cluster gathers a small set that holds the element into the leader CTA's shared memory,
+// and the leader narrows that set down by histograms over the 64-bit (value, index) key until a
+// warp can rank what is left.  The set is
+//   - with top_k up to kMaxTopK: everything from the k-th largest of the threads' maxima up (each of
+//     them is an element of its own, so the k-th largest element is not below it); about k elements,
+//     and the other filters and the draw are settled among them without another pass;
+//   - else: the bin of a histogram of the row (weights by (max - x) / temperature, 1/32 nat a bin)
+//     that the running sum over the bins names, one gather per element sought.
+// A set that is too large (flat or heavily tied rows) is cut down first, by the cluster's
+// histograms over the same key.
 //
 // Weights are exp() in f64 rounded to 2^-44 (less for rows of over 2^18 tokens, so that a row's sum
 // stays below 2^63): integer sums are exact in any order, so neither the atomics' order nor the
@@ -19,6 +25,7 @@
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include "common.cuh"
@@ -31,11 +38,14 @@ namespace cg = cooperative_groups;
 
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
-constexpr int kBins = 2048;        // 1/64 nat each: 32 nats, past which a weight rounds to 0
-constexpr int kCand = 2048;        // elements of a bin that the leader sorts
-constexpr int kMaxCluster = 8;
+constexpr int kBins = 1024;  // 1/32 nat each: 32 nats, past which a weight rounds to 0
 constexpr int kPerThread = kBins / kThreads;
-constexpr float kBinsPerNat = 64.0f;
+constexpr float kBinsPerNat = 32.0f;
+constexpr int kCand = 2048;  // elements that the leader takes
+constexpr int kMaxTopK = 1024;
+constexpr int kRank = 32;    // elements that a warp ranks
+constexpr int kMaxCluster = 8;
+constexpr int kTable = 256;  // 2^(-j / 256)
 
 struct SampleArgs {
     const void *logits;
@@ -46,37 +56,41 @@ struct SampleArgs {
     int32_t top_k_all;
     int32_t *idx;
     float *prob;
-    int shift;       // weights are multiples of 2^-shift
-    int last_bin;    // elements of later bins have weight 0
-    unsigned cap;    // elements of a segment that shared memory holds
+    int shift;     // weights are multiples of 2^-shift
+    int last_bin;  // elements of later bins have weight 0
+    unsigned cap;  // elements of a segment that shared memory holds
 };
 
-// What the leader tells the cluster about the element being located.
-struct Control {
-    int skip;                        // the prefix is the whole row
-    int bin;                         // first-level bin
-    unsigned count;                  // elements in [lo, hi] of the bin
-    unsigned long long lo, hi;       // key range
-    unsigned long long ex_mass;      // weight and count before the range
-    unsigned ex_count;
+using u64 = unsigned long long;
+
+struct Histogram {
+    unsigned lo[kBins], hi[kBins], cnt[kBins];  // weight as two words, count
+};
+
+// A part of the order: keys lo .. hi, and the weight and count of what comes before it.
+struct Range {
+    u64 lo, hi, ex_mass;
+    unsigned ex_count, count;
 };
 
 struct Shared {
     union {
-        unsigned long long cand[kCand];
-        struct {
-            unsigned lo[kBins], hi[kBins], cnt[kBins];
-        } sub;  // histogram of a key range
+        u64 cand[kCand];
+        Histogram sub;  // of a key range, while the cluster cuts a set down
     };
-    unsigned lo[kBins], hi[kBins], cnt[kBins];  // the row's histogram (leader): weight as two words, count
-    unsigned long long scan[kWarps];
+    Histogram row;      // of the row; then, in the leader, of the candidates' key range
+    double table[kTable];
+    u64 scan[kWarps];
     unsigned scan_cnt[kWarps];
-    unsigned long long rank_min[kMaxCluster], rank_max[kMaxCluster], rank_mass[kMaxCluster];
+    u64 rank_min[kMaxCluster], rank_max[kMaxCluster], rank_mass[kMaxCluster];
     float rank_top[kMaxCluster];
-    Control ctl[3];
+    Range ctl[4];       // what the leader tells the cluster: per element sought
+    int bin[4];         // its bin (the last bin of a top-k set), -1: nothing to seek
     unsigned ncand;
-    unsigned long long found_mass, found_w, found_key;
-    int which;
+    Range narrow;
+    u64 few[kRank];
+    unsigned nfew;
+    u64 found_mass, found_w, found_key;
 };
 
 PYXIS_DEVINL float widen(float x) { return x; }
@@ -84,52 +98,61 @@ PYXIS_DEVINL float widen(__nv_bfloat16 x) { return __bfloat162float(x); }
 
 // Order-preserving key of a finite or infinite value and its index: larger values first, then
 // smaller indexes; -0 ties with +0.
-PYXIS_DEVINL unsigned long long key_of(float v, unsigned idx) {
+PYXIS_DEVINL u64 key_of(float v, unsigned idx) {
     if (v == 0.0f) v = 0.0f;
     const unsigned u = __float_as_uint(v);
     const unsigned ord = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-    return ((unsigned long long)ord << 32) | (0xFFFFFFFFu - idx);
+    return ((u64)ord << 32) | (0xFFFFFFFFu - idx);
 }
-PYXIS_DEVINL float value_of(unsigned long long key) {
+PYXIS_DEVINL float value_of(u64 key) {
     const unsigned ord = (unsigned)(key >> 32);
     return __uint_as_float((ord & 0x80000000u) ? (ord & 0x7FFFFFFFu) : ~ord);
 }
 
 // 64-bit add into two 32-bit words of (this or another CTA's) shared memory: the carry goes with
 // the value the low word had, so the pair is exact once all adds are done.
-PYXIS_DEVINL void add_wide(unsigned *lo, unsigned *hi, unsigned long long w) {
+PYXIS_DEVINL void add_wide(unsigned *lo, unsigned *hi, u64 w) {
     const unsigned wl = (unsigned)w;
     const unsigned old = atomicAdd(lo, wl);
     const unsigned c = (unsigned)(w >> 32) + (old + wl < old ? 1u : 0u);
     if (c) atomicAdd(hi, c);
 }
+PYXIS_DEVINL u64 wide(const Histogram &h, int b) { return ((u64)h.hi[b] << 32) | h.lo[b]; }
 
 struct Row {
-    float top;        // largest logit
-    float bin_scale;  // bins per unit of logit
-    double inv_t;
-    bool greedy;
+    float top;            // largest logit
+    float bin_scale;      // bins per unit of logit
+    double steps;         // 2^(1/256) steps per unit of logit
     int shift, last_bin;
+    const double *table;
     // the bin of x, or -1 if its weight is 0
     PYXIS_DEVINL int bin(float x) const {
         if (x == top) return 0;
-        if (greedy) return -1;
         const float f = (top - x) * bin_scale;
         return f < (float)(last_bin + 1) ? (int)f : -1;  // NaN and infinite distances: -1
     }
-    PYXIS_DEVINL unsigned long long weight(float x) const {
+    // exp((x - top) / temperature) 2^shift, rounded: 2^(-k / 256) from the table, times exp of the
+    // rest, |rest| <= ln 2 / 512, by its Taylor polynomial (cubic: off by 2^-47 of the weight)
+    PYXIS_DEVINL u64 weight(float x) const {
         if (x == top) return 1ull << shift;
-        const double e = exp(-((double)top - (double)x) * inv_t);
-        return (unsigned long long)__double2ll_rn(e * (double)(1ull << shift));
+        const double u = ((double)top - (double)x) * steps;
+        constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: rounds to a whole number
+        const double m = u + kRound;
+        const int k = __double2loint(m);  // valid bins: u < 2^14
+        const double rest = ((m - kRound) - u) * (0.69314718055994530942 / kTable);
+        double e = fma(rest, fma(rest, fma(rest, 1.0 / 6.0, 0.5), 1.0), 1.0) * table[k & (kTable - 1)];
+        // times 2^(shift - k / 256), then rounded to a whole number in the low bits
+        e *= __hiloint2double((1023 + shift - (k >> 8)) << 20, 0);
+        return (u64)__double_as_longlong(e + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
     }
 };
 
 // Inclusive sums over the CTA's threads.
-PYXIS_DEVINL void block_scan(unsigned long long &mass, unsigned &cnt, Shared &s) {
+PYXIS_DEVINL void block_scan(u64 &mass, unsigned &cnt, Shared &s) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const unsigned long long m = __shfl_up_sync(0xffffffffu, mass, o);
+        const u64 m = __shfl_up_sync(0xffffffffu, mass, o);
         const unsigned c = __shfl_up_sync(0xffffffffu, cnt, o);
         if (lane >= o) mass += m, cnt += c;
     }
@@ -138,9 +161,146 @@ PYXIS_DEVINL void block_scan(unsigned long long &mass, unsigned &cnt, Shared &s)
     __syncthreads();
     for (int w = 0; w < warp; ++w) mass += s.scan[w], cnt += s.scan_cnt[w];
 }
+PYXIS_DEVINL u64 block_sum(u64 x, Shared &s) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) s.scan[threadIdx.x >> 5] = x;
+    __syncthreads();
+    x = 0;
+    for (int w = 0; w < kWarps; ++w) x += s.scan[w];
+    return x;
+}
+// Smallest and largest of the threads' keys.
+PYXIS_DEVINL void block_range(u64 &lo, u64 &hi, Shared &s) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const u64 x = __shfl_xor_sync(0xffffffffu, lo, o), y = __shfl_xor_sync(0xffffffffu, hi, o);
+        lo = x < lo ? x : lo;
+        hi = y > hi ? y : hi;
+    }
+    __shared__ u64 lows[kWarps], highs[kWarps];
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) lows[threadIdx.x >> 5] = lo, highs[threadIdx.x >> 5] = hi;
+    __syncthreads();
+    for (int w = 0; w < kWarps; ++w) {
+        lo = lows[w] < lo ? lows[w] : lo;
+        hi = highs[w] > hi ? highs[w] : hi;
+    }
+}
+
+PYXIS_DEVINL void clear(Histogram &h) {
+    for (int b = threadIdx.x; b < kBins; b += kThreads) h.lo[b] = h.hi[b] = h.cnt[b] = 0;
+}
+PYXIS_DEVINL int shift_for(u64 lo, u64 hi) {  // (hi - key) >> shift is a bin
+    int sh = 0;
+    while (((hi - lo) >> sh) >= kBins) ++sh;
+    return sh;
+}
+
+// The bin of a key-range histogram where the running count (by_count) or weight passes t becomes
+// the range; *out is written by one thread (after a barrier: in may be *out).
+PYXIS_DEVINL void pick_bin(const Histogram &h, const Range &in, int sh, bool by_count, u64 t, Range *out, Shared &s) {
+    u64 m = 0;
+    unsigned c = 0;
+#pragma unroll
+    for (int j = 0; j < kPerThread; ++j) m += wide(h, threadIdx.x * kPerThread + j), c += h.cnt[threadIdx.x * kPerThread + j];
+    const Range r = in;
+    u64 em = m;
+    unsigned ec = c;
+    block_scan(em, ec, s);
+    em += r.ex_mass - m, ec += r.ex_count - c;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kPerThread; ++j) {
+        const int b = threadIdx.x * kPerThread + j;
+        const u64 before = by_count ? ec : em, size = by_count ? h.cnt[b] : wide(h, b);
+        if (t >= before && t - before < size) {
+            const u64 hi = r.hi - ((u64)b << sh), width = (1ull << sh) - 1;
+            *out = Range{hi - r.lo > width ? hi - width : r.lo, hi, em, ec, h.cnt[b]};
+        }
+        em += wide(h, b), ec += h.cnt[b];
+    }
+    __syncthreads();
+}
+
+// Leader: among the candidates, whose first follows ex_mass and ex_count, the element where the
+// running count or weight passes t: its weight, its key and the running weight with it.
+PYXIS_DEVINL void locate(Shared &s, const Row &r, unsigned n, u64 ex_mass, unsigned ex_count, bool by_count, u64 t) {
+    u64 lo = ~0ull, hi = 0;
+    for (unsigned i = threadIdx.x; i < n; i += kThreads) {
+        const u64 k = s.cand[i];
+        lo = k < lo ? k : lo;
+        hi = k > hi ? k : hi;
+    }
+    block_range(lo, hi, s);
+    if (threadIdx.x == 0) s.narrow = Range{lo, hi, ex_mass, ex_count, n};
+    __syncthreads();
+    while (s.narrow.count > kRank) {
+        lo = s.narrow.lo, hi = s.narrow.hi;
+        const int sh = shift_for(lo, hi);
+        clear(s.row);
+        __syncthreads();
+        for (unsigned i = threadIdx.x; i < n; i += kThreads) {
+            const u64 k = s.cand[i];
+            if (k < lo || k > hi) continue;
+            const int b = (int)((hi - k) >> sh);
+            add_wide(&s.row.lo[b], &s.row.hi[b], r.weight(value_of(k)));
+            atomicAdd(&s.row.cnt[b], 1u);
+        }
+        __syncthreads();
+        pick_bin(s.row, s.narrow, sh, by_count, t, &s.narrow, s);
+    }
+    if (threadIdx.x == 0) s.nfew = 0;
+    __syncthreads();
+    lo = s.narrow.lo, hi = s.narrow.hi;
+    for (unsigned i = threadIdx.x; i < n; i += kThreads) {
+        const u64 k = s.cand[i];
+        if (k >= lo && k <= hi) s.few[atomicAdd(&s.nfew, 1u)] = k;
+    }
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        const unsigned few = s.nfew, lane = threadIdx.x;
+        const u64 k = lane < few ? s.few[lane] : 0;
+        const u64 w = lane < few ? r.weight(value_of(k)) : 0;
+        u64 before = s.narrow.ex_mass;
+        unsigned rank = s.narrow.ex_count;
+        for (unsigned i = 0; i < few; ++i) {
+            const u64 ki = __shfl_sync(0xffffffffu, k, i), wi = __shfl_sync(0xffffffffu, w, i);
+            if (ki > k) before += wi, ++rank;
+        }
+        if (lane < few && (by_count ? rank == t : t >= before && t - before < w)) {
+            s.found_mass = before + w;
+            s.found_w = w;
+            s.found_key = k;
+        }
+    }
+    __syncthreads();
+}
+
+// What the filters and the draw ask for, the same for every CTA of a row.
+struct Params {
+    int top_k;
+    double top_p, min_p, u;
+    PYXIS_DEVINL u64 top_p_target(u64 prefix) const {  // the first element with a running weight >= p prefix
+        const double goal = ceil(top_p * (double)prefix);
+        return goal > 1.0 ? (u64)goal - 1 : 0;
+    }
+    PYXIS_DEVINL u64 draw_target(u64 kept) const {
+        const double v = u > 0.0 ? u : 0.0;  // NaN: 0
+        const u64 t = v < 1.0 ? (u64)(v * (double)kept) : kept;
+        return t < kept ? t : kept - 1;
+    }
+};
+
+PYXIS_DEVINL void write_result(const SampleArgs &a, size_t row, const Shared &s, u64 kept) {
+    if (threadIdx.x != 0) return;
+    a.idx[row] = (int32_t)(0xFFFFFFFFu - (unsigned)(s.found_key & 0xFFFFFFFFu));
+    if (a.prob) a.prob[row] = (float)((double)s.found_w / (double)kept);
+}
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a) {
+__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a) {
     extern __shared__ __align__(16) unsigned char smem[];
     Shared &s = *reinterpret_cast<Shared *>(smem);
     T *vals = reinterpret_cast<T *>(smem + (sizeof(Shared) + 15) / 16 * 16);
@@ -150,7 +310,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a) {
     const size_t row = blockIdx.y;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
-    // this CTA's segment of the row
+    // ---- this CTA's segment of the row, and the threads' maxima
     const size_t per = (a.n + ranks - 1) / ranks;
     const size_t beg = rank * per < a.n ? rank * per : a.n, end = beg + per < a.n ? beg + per : a.n;
     const T *src = reinterpret_cast<const T *>(a.logits) + row * a.ld + beg;
@@ -161,25 +321,27 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a) {
     T *own = vals + phase;
     auto value = [&](unsigned i) -> float { return widen(i < held ? own[i] : src[i]); };
 
-    for (int b = tid; b < kBins; b += kThreads) s.lo[b] = s.hi[b] = s.cnt[b] = 0;
-    if (tid == 0) s.ncand = 0;
-    float top = -INFINITY;
+    float mine = -INFINITY;
     const unsigned head = min(held, (V - phase) % V), vecs = (held - head) / V;
-    if (tid < head) own[tid] = src[tid], top = fmaxf(top, widen(src[tid]));
-    for (unsigned i = head + vecs * V + tid; i < held; i += kThreads) own[i] = src[i], top = fmaxf(top, widen(src[i]));
-    for (unsigned i = held + tid; i < len; i += kThreads) top = fmaxf(top, widen(src[i]));
     {
         const uint4 *g = reinterpret_cast<const uint4 *>(src + head);
         uint4 *d = reinterpret_cast<uint4 *>(own + head);
-#pragma unroll 4
+#pragma unroll 8
         for (unsigned i = tid; i < vecs; i += kThreads) {
             const uint4 x = __ldg(g + i);
             d[i] = x;
             const T *e = reinterpret_cast<const T *>(&x);
 #pragma unroll
-            for (unsigned j = 0; j < V; ++j) top = fmaxf(top, widen(e[j]));
+            for (unsigned j = 0; j < V; ++j) mine = fmaxf(mine, widen(e[j]));
         }
     }
+    if (tid < (int)head) own[tid] = src[tid], mine = fmaxf(mine, widen(src[tid]));
+    for (unsigned i = head + vecs * V + tid; i < held; i += kThreads) own[i] = src[i], mine = fmaxf(mine, widen(src[i]));
+    for (unsigned i = held + tid; i < len; i += kThreads) mine = fmaxf(mine, widen(src[i]));
+    clear(s.row);
+    if (tid == 0) s.ncand = 0;
+    if (tid < kTable) s.table[tid] = exp2(-(double)tid / kTable);
+    float top = mine;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     float *wtop = reinterpret_cast<float *>(s.scan);
@@ -194,16 +356,6 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a) {
     Row r;
     r.top = s.rank_top[0];
     for (unsigned i = 1; i < ranks; ++i) r.top = fmaxf(r.top, s.rank_top[i]);
-    const float t32 = a.temperature ? a.temperature[row] : 0.f;
-    const double temperature = a.temperature ? (double)t32 : a.temperature_all;
-    r.greedy = !(temperature > 0.0);
-    r.inv_t = r.greedy ? 0.0 : 1.0 / temperature;
-    r.bin_scale = (float)(kBinsPerNat * r.inv_t);
-    r.shift = a.shift;
-    r.last_bin = a.last_bin;
-    const int top_k = r.greedy ? 0 : a.top_k ? a.top_k[row] : a.top_k_all;
-    const double top_p = r.greedy ? 1.0 : a.top_p ? (double)a.top_p[row] : a.top_p_all;
-    const double min_p = r.greedy ? 0.0 : a.min_p ? (double)a.min_p[row] : a.min_p_all;
     if (!(r.top > -INFINITY)) {  // the same for the whole cluster
         if (rank == 0 && tid == 0) {
             a.idx[row] = -1;
@@ -211,162 +363,224 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a) {
         }
         return;
     }
+    const double temperature = a.temperature ? (double)a.temperature[row] : a.temperature_all;
+    if (!(temperature > 0.0)) {  // greedy: the first maximum
+        u64 best = 0, least = ~0ull;
+        for (unsigned i = tid; i < len; i += kThreads)
+            if (value(i) == r.top) {
+                best = key_of(r.top, (unsigned)(beg + i));
+                break;
+            }
+        block_range(least, best, s);
+        if (tid == 0) leader.rank_max[rank] = best;
+        cluster.sync();
+        if (rank == 0 && tid == 0) {
+            for (unsigned i = 0; i < ranks; ++i) best = s.rank_max[i] > best ? s.rank_max[i] : best;
+            a.idx[row] = (int32_t)(0xFFFFFFFFu - (unsigned)(best & 0xFFFFFFFFu));
+            if (a.prob) a.prob[row] = 1.0f;
+        }
+        return;
+    }
+    r.bin_scale = (float)(kBinsPerNat / temperature);
+    r.steps = kTable * 1.44269504088896340736 / temperature;
+    r.shift = a.shift;
+    r.last_bin = a.last_bin;
+    r.table = s.table;
+    Params q;
+    q.top_k = a.top_k ? a.top_k[row] : a.top_k_all;
+    q.top_p = a.top_p ? (double)a.top_p[row] : a.top_p_all;
+    q.min_p = a.min_p ? (double)a.min_p[row] : a.min_p_all;
+    q.u = (double)a.u[row];
+    const double least = fmin(q.min_p, 1.0) * (double)(1ull << r.shift);  // weights that min_p keeps
+
+    // every element of bins first .. last of key lo .. hi into the leader's candidates
+    auto gather = [&](int first, int last, u64 lo, u64 hi) {
+        for (unsigned i = tid; i < len; i += kThreads) {
+            const float x = value(i);
+            const int b = r.bin(x);
+            if (b < first || b > last) continue;
+            const u64 k = key_of(x, (unsigned)(beg + i));
+            if (k < lo || k > hi) continue;
+            const unsigned at = atomicAdd(&leader.ncand, 1u);
+            if (at < kCand) leader.cand[at] = k;
+        }
+    };
+
+    // ---- a set that settles everything: the whole row, or what top_k can keep
+    const bool small = a.n <= kCand;
+    if (small || (q.top_k > 0 && q.top_k <= kMaxTopK)) {
+        if (!small) {
+            const int b = r.bin(mine);
+            if (b >= 0) atomicAdd(&leader.row.cnt[b], 1u);
+            cluster.sync();
+        }
+        if (rank == 0) {
+            if (tid == 0) s.bin[3] = r.last_bin;
+            __syncthreads();
+            if (!small) {
+                u64 unused = 0;
+                unsigned c = 0;
+#pragma unroll
+                for (int j = 0; j < kPerThread; ++j) c += s.row.cnt[tid * kPerThread + j];
+                unsigned incl = c;
+                block_scan(unused, incl, s);
+                unsigned before = incl - c;
+#pragma unroll
+                for (int j = 0; j < kPerThread; ++j) {
+                    const unsigned x = s.row.cnt[tid * kPerThread + j];
+                    if (before < (unsigned)q.top_k && before + x >= (unsigned)q.top_k) s.bin[3] = tid * kPerThread + j;
+                    before += x;
+                }
+            }
+        }
+        cluster.sync();
+        gather(0, leader.bin[3], 0, ~0ull);
+        cluster.sync();
+        const unsigned n = leader.ncand;
+        if (n <= kCand) {
+            if (rank != 0) {
+                cluster.sync();  // the leader's count has been read
+                return;
+            }
+            u64 total = 0, above = 0;
+            for (unsigned i = tid; i < n; i += kThreads) {
+                const u64 w = r.weight(value_of(s.cand[i]));
+                total += w;
+                if ((double)w >= least) above += w;
+            }
+            cluster.sync();
+            total = block_sum(total, s);
+            if (q.top_k > 0 && (unsigned)q.top_k < n) {
+                locate(s, r, n, 0, 0, true, (u64)q.top_k - 1);
+                total = s.found_mass;
+                __syncthreads();
+            }
+            u64 kept = total;
+            if (q.min_p > 0.0) {
+                above = block_sum(above, s);
+                kept = above < kept ? above : kept;
+            }
+            if (q.top_p < 1.0) {
+                locate(s, r, n, 0, 0, false, q.top_p_target(total));
+                kept = s.found_mass < kept ? s.found_mass : kept;
+                __syncthreads();
+            }
+            locate(s, r, n, 0, 0, false, q.draw_target(kept));
+            write_result(a, row, s, kept);
+            return;
+        }
+        cluster.sync();  // everyone has read the count
+        clear(s.row);
+        cluster.sync();
+    }
 
     // ---- the histogram of the row, in the leader
     {
-        const double least = fmin(min_p, 1.0) * (double)(1ull << r.shift);
-        unsigned long long above = 0;  // weight of the elements that min_p keeps
+        u64 above = 0;  // weight of the elements that min_p keeps
+        const bool count = q.top_k > 0;
         for (unsigned i = tid; i < len; i += kThreads) {
             const float x = value(i);
             const int b = r.bin(x);
             if (b < 0) continue;
-            const unsigned long long w = r.weight(x);
+            const u64 w = r.weight(x);
             if ((double)w >= least) above += w;
-            add_wide(&s.lo[b], &s.hi[b], w);
-            atomicAdd(&s.cnt[b], 1u);
+            add_wide(&s.row.lo[b], &s.row.hi[b], w);
+            if (count) atomicAdd(&s.row.cnt[b], 1u);
         }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) above += __shfl_xor_sync(0xffffffffu, above, o);
-        __syncthreads();
-        if (lane == 0) s.scan[warp] = above;
-        __syncthreads();
-        if (tid == 0) {
-            for (int w = 1; w < kWarps; ++w) above += s.scan[w];
-            leader.rank_mass[rank] = above;
-        }
+        above = block_sum(above, s);
+        if (tid == 0) leader.rank_mass[rank] = above;
         if (rank != 0)
-            for (int b = tid; b < kBins; b += kThreads)
-                if (s.cnt[b]) {
-                    add_wide(&leader.lo[b], &leader.hi[b], ((unsigned long long)s.hi[b] << 32) | s.lo[b]);
-                    atomicAdd(&leader.cnt[b], s.cnt[b]);
-                }
+            for (int b = tid; b < kBins; b += kThreads) {
+                const u64 w = wide(s.row, b);
+                if (w) add_wide(&leader.row.lo[b], &leader.row.hi[b], w);
+                if (s.row.cnt[b]) atomicAdd(&leader.row.cnt[b], s.row.cnt[b]);
+            }
     }
     cluster.sync();
 
     // ---- leader: running sums over the bins (thread t holds bins kPerThread t ..)
-    unsigned long long bin_mass[kPerThread], ex_mass = 0;
-    unsigned bin_cnt[kPerThread], ex_cnt = 0;
-    unsigned long long total = 0, kept = 0;
-    unsigned total_cnt = 0;
+    u64 bin_mass[kPerThread], ex_mass = 0, total = 0, kept = 0;
+    unsigned bin_cnt[kPerThread], ex_cnt = 0, total_cnt = 0;
     if (rank == 0) {
-        unsigned long long m = 0;
+        u64 m = 0;
         unsigned c = 0;
 #pragma unroll
         for (int j = 0; j < kPerThread; ++j) {
-            const int b = tid * kPerThread + j;
-            bin_mass[j] = ((unsigned long long)s.hi[b] << 32) | s.lo[b];
-            bin_cnt[j] = s.cnt[b];
+            bin_mass[j] = wide(s.row, tid * kPerThread + j);
+            bin_cnt[j] = s.row.cnt[tid * kPerThread + j];
             m += bin_mass[j];
             c += bin_cnt[j];
         }
         ex_mass = m, ex_cnt = c;
         block_scan(ex_mass, ex_cnt, s);
-        if (tid == kThreads - 1) s.found_mass = ex_mass, s.which = (int)ex_cnt;
+        if (tid == kThreads - 1) s.found_mass = ex_mass, s.nfew = ex_cnt;
         __syncthreads();
         total = s.found_mass;
-        total_cnt = (unsigned)s.which;
+        total_cnt = s.nfew;
         ex_mass -= m, ex_cnt -= c;
         kept = total;
-        if (min_p > 0.0) {
-            unsigned long long above = 0;
+        if (q.min_p > 0.0) {
+            u64 above = 0;
             for (unsigned i = 0; i < ranks; ++i) above += s.rank_mass[i];
             kept = above < kept ? above : kept;
         }
         __syncthreads();
     }
-
-    unsigned long long prefix = total;  // weight of the top-k prefix
+    u64 prefix = total;  // weight of the top-k prefix
     // stage 0: top-k, 1: top-p, 2: the draw.  Each locates the first element whose running count
-    // (stage 0) or weight exceeds `t`.
+    // (stage 0) or weight exceeds t.
     for (int stage = 0; stage < 3; ++stage) {
-        if (stage == 0 && top_k <= 0) continue;
-        if (stage == 1 && !(top_p < 1.0)) continue;
-        Control &ctl = s.ctl[stage];
-        unsigned long long t = 0;
+        if (stage == 0 && q.top_k <= 0) continue;
+        if (stage == 1 && !(q.top_p < 1.0)) continue;
+        u64 t = 0;
         if (rank == 0) {
-            bool skip = false;
-            if (stage == 0) {
-                t = (unsigned long long)top_k - 1;
-                skip = t >= total_cnt;
-            } else if (stage == 1) {
-                const double goal = ceil(top_p * (double)prefix);
-                t = goal > 1.0 ? (unsigned long long)goal - 1 : 0;
-                skip = t >= total;
-            } else {
-                double u = (double)a.u[row];
-                u = r.greedy || !(u > 0.0) ? 0.0 : u;
-                t = u < 1.0 ? (unsigned long long)(u * (double)kept) : kept;
-                if (t >= kept) t = kept - 1;
-            }
-            if (tid == 0) ctl.skip = skip, s.ncand = 0;
-            if (!skip) {
-                unsigned long long m = ex_mass;
-                unsigned c = ex_cnt;
+            t = stage == 0 ? (u64)q.top_k - 1 : stage == 1 ? q.top_p_target(prefix) : q.draw_target(kept);
+            if (tid == 0) s.bin[stage] = -1, s.ncand = 0;
+            __syncthreads();
+            u64 m = ex_mass;
+            unsigned c = ex_cnt;
 #pragma unroll
-                for (int j = 0; j < kPerThread; ++j) {
-                    const unsigned long long before = stage == 0 ? c : m, size = stage == 0 ? bin_cnt[j] : bin_mass[j];
-                    if (t >= before && t - before < size) {
-                        ctl.bin = tid * kPerThread + j;
-                        ctl.count = bin_cnt[j];
-                        ctl.lo = 0, ctl.hi = ~0ull;
-                        ctl.ex_mass = m, ctl.ex_count = c;
-                    }
-                    m += bin_mass[j], c += bin_cnt[j];
+            for (int j = 0; j < kPerThread; ++j) {
+                const u64 before = stage == 0 ? c : m, size = stage == 0 ? bin_cnt[j] : bin_mass[j];
+                if (t >= before && t - before < size) {
+                    s.bin[stage] = tid * kPerThread + j;
+                    s.ctl[stage] = Range{0, ~0ull, m, c, bin_cnt[j]};
                 }
+                m += bin_mass[j], c += bin_cnt[j];
             }
         }
         cluster.sync();
-        const Control &shared_ctl = leader.ctl[stage];
-        if (shared_ctl.skip) continue;
-        const int bin = shared_ctl.bin;
-        unsigned count = shared_ctl.count;
-        unsigned long long lo = 0, hi = ~0ull;
+        const int bin = leader.bin[stage];
+        if (bin < 0) continue;  // top-k keeps the whole row
+        gather(bin, bin, 0, ~0ull);
+        cluster.sync();
+        unsigned count = leader.ncand;
         if (count > kCand) {
-            // the bin's range of keys
-            unsigned long long kmin = ~0ull, kmax = 0;
+            // the bin's range of keys; then each round leaves 1 / kBins of it, down to single keys
+            u64 lo = ~0ull, hi = 0;
             for (unsigned i = tid; i < len; i += kThreads) {
                 const float x = value(i);
                 if (r.bin(x) != bin) continue;
-                const unsigned long long k = key_of(x, (unsigned)(beg + i));
-                kmin = k < kmin ? k : kmin;
-                kmax = k > kmax ? k : kmax;
+                const u64 k = key_of(x, (unsigned)(beg + i));
+                lo = k < lo ? k : lo;
+                hi = k > hi ? k : hi;
             }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) {
-                const unsigned long long x = __shfl_xor_sync(0xffffffffu, kmin, o), y = __shfl_xor_sync(0xffffffffu, kmax, o);
-                kmin = x < kmin ? x : kmin;
-                kmax = y > kmax ? y : kmax;
-            }
-            __syncthreads();
-            if (lane == 0) s.scan[warp] = kmin;
-            __syncthreads();
-            if (tid == 0) {
-                for (int w = 0; w < kWarps; ++w) kmin = s.scan[w] < kmin ? s.scan[w] : kmin;
-                leader.rank_min[rank] = kmin;
-            }
-            __syncthreads();
-            if (lane == 0) s.scan[warp] = kmax;
-            __syncthreads();
-            if (tid == 0) {
-                for (int w = 0; w < kWarps; ++w) kmax = s.scan[w] > kmax ? s.scan[w] : kmax;
-                leader.rank_max[rank] = kmax;
-            }
+            block_range(lo, hi, s);
+            if (tid == 0) leader.rank_min[rank] = lo, leader.rank_max[rank] = hi;
             cluster.sync();
             lo = ~0ull, hi = 0;
             for (unsigned i = 0; i < ranks; ++i) {
                 lo = leader.rank_min[i] < lo ? leader.rank_min[i] : lo;
                 hi = leader.rank_max[i] > hi ? leader.rank_max[i] : hi;
             }
-            // each round leaves 1/kBins of the range, down to single keys
             while (count > kCand) {
-                int sh = 0;
-                while (((hi - lo) >> sh) >= kBins) ++sh;
-                for (int b = tid; b < kBins; b += kThreads) s.sub.lo[b] = s.sub.hi[b] = s.sub.cnt[b] = 0;
+                const int sh = shift_for(lo, hi);
+                clear(s.sub);
                 cluster.sync();
                 for (unsigned i = tid; i < len; i += kThreads) {
                     const float x = value(i);
                     if (r.bin(x) != bin) continue;
-                    const unsigned long long k = key_of(x, (unsigned)(beg + i));
+                    const u64 k = key_of(x, (unsigned)(beg + i));
                     if (k < lo || k > hi) continue;
                     const unsigned b = (unsigned)((hi - k) >> sh);
                     add_wide(&s.sub.lo[b], &s.sub.hi[b], r.weight(x));
@@ -376,106 +590,37 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a) {
                 if (rank != 0)
                     for (int b = tid; b < kBins; b += kThreads)
                         if (s.sub.cnt[b]) {
-                            add_wide(&leader.sub.lo[b], &leader.sub.hi[b],
-                                     ((unsigned long long)s.sub.hi[b] << 32) | s.sub.lo[b]);
+                            add_wide(&leader.sub.lo[b], &leader.sub.hi[b], wide(s.sub, b));
                             atomicAdd(&leader.sub.cnt[b], s.sub.cnt[b]);
                         }
                 cluster.sync();
                 if (rank == 0) {
-                    unsigned long long m = 0;
-                    unsigned c = 0;
-#pragma unroll
-                    for (int j = 0; j < kPerThread; ++j) {
-                        const int b = tid * kPerThread + j;
-                        m += ((unsigned long long)s.sub.hi[b] << 32) | s.sub.lo[b];
-                        c += s.sub.cnt[b];
-                    }
-                    unsigned long long em = m;
-                    unsigned ec = c;
-                    block_scan(em, ec, s);
-                    em += ctl.ex_mass - m, ec += ctl.ex_count - c;
-                    __syncthreads();  // ctl is rewritten below
-#pragma unroll
-                    for (int j = 0; j < kPerThread; ++j) {
-                        const int b = tid * kPerThread + j;
-                        const unsigned long long bm = ((unsigned long long)s.sub.hi[b] << 32) | s.sub.lo[b];
-                        const unsigned long long before = stage == 0 ? ec : em, size = stage == 0 ? s.sub.cnt[b] : bm;
-                        if (t >= before && t - before < size) {
-                            ctl.hi = hi - ((unsigned long long)b << sh);
-                            const unsigned long long width = (1ull << sh) - 1;
-                            ctl.lo = ctl.hi - lo > width ? ctl.hi - width : lo;
-                            ctl.count = s.sub.cnt[b];
-                            ctl.ex_mass = em, ctl.ex_count = ec;
-                        }
-                        em += bm, ec += s.sub.cnt[b];
-                    }
+                    if (tid == 0) s.ctl[stage].lo = lo, s.ctl[stage].hi = hi, s.ncand = 0;
+                    __syncthreads();
+                    pick_bin(s.sub, s.ctl[stage], sh, stage == 0, t, &s.ctl[stage], s);
                 }
                 cluster.sync();
-                lo = shared_ctl.lo, hi = shared_ctl.hi, count = shared_ctl.count;
+                lo = leader.ctl[stage].lo, hi = leader.ctl[stage].hi, count = leader.ctl[stage].count;
             }
+            gather(bin, bin, lo, hi);
+            cluster.sync();
         }
-        // ---- gather the elements of the range into the leader, sort and scan them there
-        for (unsigned i = tid; i < len; i += kThreads) {
-            const float x = value(i);
-            if (r.bin(x) != bin) continue;
-            const unsigned long long k = key_of(x, (unsigned)(beg + i));
-            if (k < lo || k > hi) continue;
-            const unsigned at = atomicAdd(&leader.ncand, 1u);
-            if (at < kCand) leader.cand[at] = k;
-        }
-        cluster.sync();
         if (rank == 0) {
-            int size = 32;
-            while (size < (int)count) size <<= 1;
-            for (int i = (int)count + tid; i < size; i += kThreads) s.cand[i] = 0;
-            __syncthreads();
-            for (int k = 2; k <= size; k <<= 1)
-                for (int j = k >> 1; j > 0; j >>= 1) {
-                    for (int i = tid; i < size / 2; i += kThreads) {
-                        const int x = 2 * i - (i & (j - 1)), y = x + j;  // j is a power of two
-                        const unsigned long long p = s.cand[x], q = s.cand[y];
-                        if ((p < q) == ((x & k) == 0)) s.cand[x] = q, s.cand[y] = p;
-                    }
-                    __syncthreads();
-                }
-            // running weights; thread t holds `each` consecutive candidates
-            const int each = (size + kThreads - 1) / kThreads;
-            unsigned long long w[kCand / kThreads], m = 0;
-            for (int j = 0; j < each; ++j) {
-                const int i = tid * each + j;
-                w[j] = i < (int)count ? r.weight(value_of(s.cand[i])) : 0;
-                m += w[j];
-            }
-            unsigned long long em = m;
-            unsigned unused = 0;
-            block_scan(em, unused, s);
-            em += ctl.ex_mass - m;
-            for (int j = 0; j < each; ++j) {
-                const int i = tid * each + j;
-                if (i < (int)count &&
-                    (stage == 0 ? (unsigned long long)ctl.ex_count + i == t : t >= em && t - em < w[j])) {
-                    s.found_mass = em + w[j];
-                    s.found_w = w[j];
-                    s.found_key = s.cand[i];
-                }
-                em += w[j];
-            }
-            __syncthreads();
-            const unsigned long long cum = s.found_mass;
+            locate(s, r, count, s.ctl[stage].ex_mass, s.ctl[stage].ex_count, stage == 0, t);
+            const u64 cum = s.found_mass;
             if (stage == 0) prefix = cum;
-            if (stage < 2) {
-                if (cum < kept) kept = cum;
-            } else if (tid == 0) {
-                a.idx[row] = (int32_t)(0xFFFFFFFFu - (unsigned)(s.found_key & 0xFFFFFFFFu));
-                if (a.prob) a.prob[row] = r.greedy ? 1.0f : (float)((double)s.found_w / (double)kept);
-            }
+            if (stage < 2)
+                kept = cum < kept ? cum : kept;
+            else
+                write_result(a, row, s, kept);
             __syncthreads();
         }
     }
+    cluster.sync();  // no CTA leaves while another may still read the leader's
 }
 
 template <typename T>
-cudaError_t run_sample(SampleArgs &a, size_t M, int ranks, cudaStream_t st) {
+cudaError_t run_sample(SampleArgs &a, size_t M, int num_sms, cudaStream_t st) {
     auto kern = sample_kernel<T>;
     static std::atomic<uint64_t> done{0};
     constexpr size_t fixed = (sizeof(Shared) + 15) / 16 * 16, most = 200 * 1024;
@@ -483,8 +628,13 @@ cudaError_t run_sample(SampleArgs &a, size_t M, int ranks, cudaStream_t st) {
         return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
     });
     if (e != cudaSuccess) return e;
+    // one CTA per 4096 tokens, up to eight; fewer where the rows fill the GPU (two CTAs an SM) without
+    // them and two such segments still fit an SM
+    int ranks = 1;
+    while (ranks < kMaxCluster && (size_t)ranks * 4096 < a.n) ranks *= 2;
+    while (ranks > 1 && M * ranks > (size_t)num_sms * 2 && (a.n / (ranks / 2)) * sizeof(T) + fixed < 112 * 1024) ranks /= 2;
     const size_t per = (a.n + ranks - 1) / ranks, room = (most - fixed) / sizeof(T) - 16 / sizeof(T);
-    a.cap = (unsigned)(per < room ? per : room);
+    a.cap = (unsigned)std::min(per, room);
     const size_t bytes = fixed + (a.cap + 16 / sizeof(T)) * sizeof(T);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ranks, (unsigned)M);
@@ -504,7 +654,7 @@ cudaError_t run_sample(SampleArgs &a, size_t M, int ranks, cudaStream_t st) {
 }  // namespace
 
 cudaError_t launch_sample(const void *logits, int dtype, size_t M, size_t n, size_t ld, const float *uniforms,
-                          const pyxis_sample_params &p, int32_t *idx, float *prob, cudaStream_t st) {
+                          const pyxis_sample_params &p, int32_t *idx, float *prob, int num_sms, cudaStream_t st) {
     SampleArgs a;
     a.logits = logits;
     a.n = n;
@@ -525,10 +675,7 @@ cudaError_t launch_sample(const void *logits, int dtype, size_t M, size_t n, siz
     a.shift = bits > 18 ? 62 - bits : 44;
     // a weight below 2^-(shift + 1) rounds to 0: beyond (shift + 1) ln 2 nats, and a bin to spare
     a.last_bin = (int)((a.shift + 1) * 0.6931471805599453 * kBinsPerNat) + 1;
-    // one CTA per 4096 tokens, up to eight
-    int ranks = 1;
-    while (ranks < kMaxCluster && (size_t)ranks * 4096 < n) ranks *= 2;
-    return dtype == PYXIS_DTYPE_F32 ? run_sample<float>(a, M, ranks, st) : run_sample<__nv_bfloat16>(a, M, ranks, st);
+    return dtype == PYXIS_DTYPE_F32 ? run_sample<float>(a, M, num_sms, st) : run_sample<__nv_bfloat16>(a, M, num_sms, st);
 }
 
 }  // namespace pyxis

@@ -33,6 +33,6 @@ cudaError_t launch_kv_compact(const pyxis_kv_pages &kv, const int32_t *block_tab
                               int32_t *new_len, cudaStream_t st);
 
 cudaError_t launch_sample(const void *logits, int dtype, size_t M, size_t n, size_t ld, const float *uniforms,
-                          const pyxis_sample_params &p, int32_t *idx, float *prob, cudaStream_t st);
+                          const pyxis_sample_params &p, int32_t *idx, float *prob, int num_sms, cudaStream_t st);
 
 }  // namespace pyxis

@@ -246,7 +246,8 @@ int pyxis_cuda_sample_dev(pyxis_cuda_ctx *ctx, const void *logits, int dtype, si
     if (!aligned(logits, elem(dtype))) return fail(PYXIS_EINVAL, "logits are not aligned to their type");
     if (!ctx) return fail(PYXIS_EINVAL, "null context");
     DeviceGuard g(ctx->device);
-    return cuda_status(launch_sample(logits, dtype, M, n, ld, uniforms, *params, idx, prob, pick_stream(ctx, stream)),
+    return cuda_status(launch_sample(logits, dtype, M, n, ld, uniforms, *params, idx, prob, ctx->num_sms,
+                                     pick_stream(ctx, stream)),
                        "sample launch");
 }
 
