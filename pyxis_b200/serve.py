@@ -22,7 +22,7 @@ import ctypes as C
 
 import numpy as np
 
-from . import _native, _require_cuda
+from . import CUDA_STREAM_LEGACY, _native, _require_cuda
 from ._native import DTYPE_BF16, DTYPE_F32, PYXIS_EINVAL, PyxisError, check
 
 _vp, _sz, _i64 = C.c_void_p, C.c_size_t, C.c_int64
@@ -56,54 +56,76 @@ def _fail(msg: str):
     raise PyxisError(PYXIS_EINVAL, msg)
 
 
-_DTYPES: dict = {}
+class _Torch:
+    """What the calls use of torch and of the library, looked up once: a call is a few microseconds,
+    and the kernels of a small step are no longer."""
 
-
-def _dtype(t) -> int:
-    if not _DTYPES:
+    def __init__(self):
         import torch
-        _DTYPES.update({torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16})
-    d = _DTYPES.get(t.dtype)
-    if d is None:
-        _fail(f"dtype {t.dtype}: float32 or bfloat16 is needed")
-    return d
+        self.empty, self.Tensor = torch.empty, torch.Tensor
+        self.f32, self.f64, self.i32, self.i64 = torch.float32, torch.float64, torch.int32, torch.int64
+        self.masks = (torch.int64, torch.uint64)
+        self.types = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16}
+        self.contexts: dict = {}
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        self.raw_stream = raw or (lambda device: torch.cuda.current_stream(device).cuda_stream)
+        L = _native.lib()
+        self.rope, self.tree = L.pyxis_cuda_qk_norm_rope_dev, L.pyxis_cuda_tree_attention_dev
+        self.copy, self.compact, self.sample = (L.pyxis_cuda_kv_copy_pages_dev, L.pyxis_cuda_kv_compact_dev,
+                                                L.pyxis_cuda_sample_dev)
 
 
-def _where(t):
-    """(context, its device) of a CUDA tensor."""
-    if not t.is_cuda:
+_torch = None
+
+
+def _begin(t):
+    """(what the calls use, the tensor's device, its context) of a CUDA tensor."""
+    global _torch
+    if _torch is None:
+        _torch = _Torch()
+    d = t.get_device()
+    if d < 0:
         _fail(f"a CUDA tensor is needed, not one on {t.device}")
-    return _require_cuda(t.device.index or 0)
+    ctx = _torch.contexts.get(d)
+    if ctx is None:
+        ctx = _torch.contexts[d] = _require_cuda(d)
+    return _torch, d, ctx.handle
 
 
-def _stream(stream, device) -> int:
-    import torch
-    h = (stream or torch.cuda.current_stream(device)).cuda_stream
-    return h if h else 0x1  # torch's default stream, as the explicit handle of the legacy one
+def _stream(stream, device: int) -> int:
+    # torch's default stream is 0, which the library reads as its own: name the legacy stream instead
+    return (_torch.raw_stream(device) if stream is None else stream.cuda_stream) or CUDA_STREAM_LEGACY
 
 
-def _array(t, what: str, dtype: str, n: int, ctx) -> int:
+def _array(t, what: str, dtype, n: int, device: int) -> int:
     """Address of a contiguous device array of at least n elements."""
-    if not t.is_cuda or (t.device.index or 0) != ctx.device:
-        _fail(f"{what} must be on cuda:{ctx.device}")
-    if str(t.dtype) != dtype:
+    if t.get_device() != device:
+        _fail(f"{what} must be on cuda:{device}")
+    if t.dtype is not dtype and (dtype is not _torch.i64 or t.dtype not in _torch.masks):
         _fail(f"{what} must be {dtype}, not {t.dtype}")
     if t.numel() < n or not t.is_contiguous():
         _fail(f"{what} must hold {n} contiguous elements")
     return t.data_ptr()
 
 
-def _pages(k, v, ctx, layers: bool) -> _Pages:
-    dims = 5 if layers else 4
-    if k.dim() != dims or k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype:
-        _fail(f"k_pages and v_pages must be {dims}-dimensional tensors of one shape, layout and type")
-    if not k.is_cuda or k.device != v.device or (k.device.index or 0) != ctx.device:
-        _fail(f"cache pages must be on cuda:{ctx.device}")
-    s, n = k.stride(), k.shape
-    if s[-1] != 1:
-        _fail("the elements of a head must be contiguous")
-    return _Pages(k.data_ptr(), v.data_ptr(), _dtype(k), n[0] if layers else 1, n[-4], n[-3], n[-2], n[-1],
-                  s[0] if layers else 0, s[-4], s[-3], s[-2])
+def _table(t, what: str, device: int):
+    if t.dim() != 2 or t.stride(1) != 1 or t.dtype is not _torch.i32 or t.get_device() != device:
+        _fail(f"{what} must be int32 [sequences, pages] with contiguous rows on cuda:{device}")
+    return t.shape
+
+
+def _pages(k, v, device: int, layers: bool) -> _Pages:
+    n, s = k.shape, k.stride()
+    if len(n) != (5 if layers else 4) or n != v.shape or s != v.stride() or k.dtype is not v.dtype:
+        _fail(f"k_pages and v_pages must be {5 if layers else 4}-dimensional tensors of one shape, layout and type")
+    if k.get_device() != device or v.get_device() != device:
+        _fail(f"cache pages must be on cuda:{device}")
+    kind = _torch.types.get(k.dtype)
+    if kind is None or s[-1] != 1:
+        _fail(f"cache pages of {k.dtype}: float32 or bfloat16 with contiguous heads are needed")
+    if layers:
+        return _Pages(k.data_ptr(), v.data_ptr(), kind, n[0], n[1], n[2], n[3], n[4], s[0], s[1], s[2], s[3])
+    return _Pages(k.data_ptr(), v.data_ptr(), kind, 1, n[0], n[1], n[2], n[3], 0, s[0], s[1], s[2])
 
 
 ROPE_KINDS = {"plain": 0, "linear": 1, "ntk": 2, "yarn": 3}
@@ -134,31 +156,31 @@ def qk_norm_rope_dev(qkv, positions, inv_freq, n_q_heads: int, n_kv_heads: int, 
     on the device, or None for no rotation; ``q_norm`` / ``k_norm`` float32 [head_dim] or None;
     ``q``: a [tokens, n_q, head_dim] tensor with contiguous heads to write, ``qkv``'s own rows
     included."""
-    import torch
-
-    ctx = _where(qkv)
-    if qkv.dim() != 2 or qkv.shape[1] != (n_q_heads + 2 * n_kv_heads) * head_dim or qkv.stride(1) != 1:
+    T, dev, ctx = _begin(qkv)
+    shape, ld, dtype = qkv.shape, qkv.stride(), qkv.dtype
+    if len(shape) != 2 or shape[1] != (n_q_heads + 2 * n_kv_heads) * head_dim or ld[1] != 1:
         _fail("qkv must be [tokens, (n_q + 2 n_kv) * head_dim] with contiguous rows")
-    n = qkv.shape[0]
-    kv = _pages(k_pages, v_pages, ctx, False)
-    if kv.n_kv_heads != n_kv_heads or kv.head_dim != head_dim or k_pages.dtype != qkv.dtype:
+    n = shape[0]
+    kv = _pages(k_pages, v_pages, dev, False)
+    if kv.n_kv_heads != n_kv_heads or kv.head_dim != head_dim or k_pages.dtype is not dtype:
         _fail("the cache's heads or type differ from qkv's")
     if q is None:
-        q = torch.empty((n, n_q_heads, head_dim), dtype=qkv.dtype, device=qkv.device)
-    elif q.shape != (n, n_q_heads, head_dim) or q.dtype != qkv.dtype or q.device != qkv.device or q.stride(2) != 1 or (
-            n_q_heads > 1 and q.stride(1) != head_dim):
-        _fail("q must be [tokens, n_q, head_dim] of qkv's type and device with contiguous heads")
-    rot = 0
-    if inv_freq is not None:
-        rot = 2 * inv_freq.numel()
-    a = _RopeArgs(qkv.data_ptr(), q.data_ptr(), n, qkv.stride(0), q.stride(0),
-                  _array(positions, "positions", "torch.int32", n, ctx) if rot else None,
-                  _array(slots, "slots", "torch.int32", n, ctx),
-                  _array(inv_freq, "inv_freq", "torch.float64", rot // 2, ctx) if rot else None,
-                  None if q_norm is None else _array(q_norm, "q_norm", "torch.float32", head_dim, ctx),
-                  None if k_norm is None else _array(k_norm, "k_norm", "torch.float32", head_dim, ctx),
+        q = T.empty((n, n_q_heads, head_dim), dtype=dtype, device=qkv.device)
+        ld_q = n_q_heads * head_dim
+    else:
+        if q.shape != (n, n_q_heads, head_dim) or q.dtype is not dtype or q.get_device() != dev or q.stride(2) != 1 or (
+                n_q_heads > 1 and q.stride(1) != head_dim):
+            _fail("q must be [tokens, n_q, head_dim] of qkv's type and device with contiguous heads")
+        ld_q = q.stride(0)
+    rot = 0 if inv_freq is None else 2 * inv_freq.numel()
+    a = _RopeArgs(qkv.data_ptr(), q.data_ptr(), n, ld[0], ld_q, _array(positions, "positions", T.i32, n, dev) if rot else None,
+                  _array(slots, "slots", T.i32, n, dev), _array(inv_freq, "inv_freq", T.f64, rot // 2, dev) if rot else None,
+                  None if q_norm is None else _array(q_norm, "q_norm", T.f32, head_dim, dev),
+                  None if k_norm is None else _array(k_norm, "k_norm", T.f32, head_dim, dev),
                   n_q_heads, rot, 1 if interleaved else 0, eps, rope_scale)
-    check(_native.lib().pyxis_cuda_qk_norm_rope_dev(ctx.handle, C.byref(a), C.byref(kv), _stream(stream, qkv.device)))
+    rc = T.rope(ctx, C.byref(a), C.byref(kv), _stream(stream, dev))
+    if rc:
+        check(rc)
     return q
 
 
@@ -171,68 +193,62 @@ def tree_attention_dev(q, k_pages, v_pages, block_table, context_len, q_start, t
     ``block_table`` [sequences, width].  ``max_context`` bounds the contexts, for the split of the work
     (default: what the table holds); ``scale`` defaults to 1 / sqrt(head_dim).  Rows outside every
     sequence are left as they are (in a new ``out``: uninitialised)."""
-    import torch
-
-    ctx = _where(q)
-    kv = _pages(k_pages, v_pages, ctx, False)
-    if q.dim() != 3 or q.shape[2] != kv.head_dim or q.stride(2) != 1 or q.dtype != k_pages.dtype:
+    T, dev, ctx = _begin(q)
+    kv = _pages(k_pages, v_pages, dev, False)
+    shape, s, dtype = q.shape, q.stride(), q.dtype
+    if len(shape) != 3 or shape[2] != kv.head_dim or s[2] != 1 or dtype is not k_pages.dtype:
         _fail("q must be [rows, n_q, head_dim] of the cache's type")
-    rows, n_q, hd = q.shape
+    rows, n_q, hd = shape
     if out is None:
-        out = torch.empty((rows, n_q, hd), dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.stride(2) != 1:
+        out = T.empty((rows, n_q, hd), dtype=dtype, device=q.device)
+    elif out.shape != shape or out.dtype is not dtype or out.get_device() != dev or out.stride(2) != 1:
         _fail("out must have q's shape, type and device")
-    if block_table.dim() != 2 or block_table.stride(1) != 1 or str(block_table.dtype) != "torch.int32" or \
-            block_table.device != q.device:
-        _fail("block_table must be int32 [sequences, pages] with contiguous rows on q's device")
-    n_seq, width = block_table.shape
-    mask = None
-    if tree_mask is not None:
-        mask = _array(tree_mask, "tree_mask", "torch.uint64" if str(tree_mask.dtype) == "torch.uint64" else "torch.int64",
-                      rows, ctx)
-    a = _TreeArgs(q.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1), out.stride(0), out.stride(1), rows, n_seq,
-                  _array(q_start, "q_start", "torch.int32", n_seq + 1, ctx),
-                  _array(context_len, "context_len", "torch.int32", n_seq, ctx), block_table.data_ptr(), mask,
+    o = out.stride()
+    n_seq, width = _table(block_table, "block_table", dev)
+    a = _TreeArgs(q.data_ptr(), out.data_ptr(), s[0], s[1], o[0], o[1], rows, n_seq,
+                  _array(q_start, "q_start", T.i32, n_seq + 1, dev), _array(context_len, "context_len", T.i32, n_seq, dev),
+                  block_table.data_ptr(), None if tree_mask is None else _array(tree_mask, "tree_mask", T.i64, rows, dev),
                   block_table.stride(0), width, n_q, max_tree, width * kv.page_size if max_context is None else max_context,
                   hd ** -0.5 if scale is None else scale)
-    ws, ws_bytes = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
-    check(_native.lib().pyxis_cuda_tree_attention_dev(ctx.handle, C.byref(a), C.byref(kv), ws, ws_bytes,
-                                                      _stream(stream, q.device)))
+    if workspace is None:
+        rc = T.tree(ctx, C.byref(a), C.byref(kv), None, 0, _stream(stream, dev))
+    else:
+        if workspace.get_device() != dev or not workspace.is_contiguous():
+            _fail(f"the workspace must be contiguous on cuda:{dev}")
+        rc = T.tree(ctx, C.byref(a), C.byref(kv), workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+                    _stream(stream, dev))
+    if rc:
+        check(rc)
     return out
 
 
 def kv_copy_pages_dev(k_pages, v_pages, src, dst, stream=None) -> None:
     """Copies pages ``src[i]`` to ``dst[i]`` (int32) of ``k_pages`` / ``v_pages`` [layers, pages,
     page_size, n_kv, head_dim] in every layer (pyxis_cuda_kv_copy_pages_dev)."""
-    ctx = _where(k_pages)
-    kv = _pages(k_pages, v_pages, ctx, True)
+    T, dev, ctx = _begin(k_pages)
+    kv = _pages(k_pages, v_pages, dev, True)
     n = src.numel()
     if dst.numel() != n:
         _fail("src and dst differ in length")
-    check(_native.lib().pyxis_cuda_kv_copy_pages_dev(
-        ctx.handle, C.byref(kv), _array(src, "src", "torch.int32", n, ctx), _array(dst, "dst", "torch.int32", n, ctx), n,
-        _stream(stream, k_pages.device)))
+    rc = T.copy(ctx, C.byref(kv), _array(src, "src", T.i32, n, dev), _array(dst, "dst", T.i32, n, dev), n, _stream(stream, dev))
+    if rc:
+        check(rc)
 
 
 def kv_compact_dev(k_pages, v_pages, block_table, context_len, accepted, new_len=None, stream=None):
     """Moves the cache entries of each sequence's ``accepted`` nodes (bits, int64 or uint64
     [sequences]) to positions ``context_len[s]``, ``context_len[s]`` + 1, ... in every layer and
     returns ``new_len`` int32 [sequences] = context_len + their number (pyxis_cuda_kv_compact_dev)."""
-    import torch
-
-    ctx = _where(k_pages)
-    kv = _pages(k_pages, v_pages, ctx, True)
-    if block_table.dim() != 2 or block_table.stride(1) != 1 or str(block_table.dtype) != "torch.int32" or \
-            block_table.device != k_pages.device:
-        _fail("block_table must be int32 [sequences, pages] with contiguous rows on the cache's device")
-    n_seq, width = block_table.shape
+    T, dev, ctx = _begin(k_pages)
+    kv = _pages(k_pages, v_pages, dev, True)
+    n_seq, width = _table(block_table, "block_table", dev)
     if new_len is None:
-        new_len = torch.empty(n_seq, dtype=torch.int32, device=k_pages.device)
-    bits = "torch.uint64" if str(accepted.dtype) == "torch.uint64" else "torch.int64"
-    check(_native.lib().pyxis_cuda_kv_compact_dev(
-        ctx.handle, C.byref(kv), block_table.data_ptr(), block_table.stride(0), width,
-        _array(context_len, "context_len", "torch.int32", n_seq, ctx), _array(accepted, "accepted", bits, n_seq, ctx), n_seq,
-        _array(new_len, "new_len", "torch.int32", n_seq, ctx), _stream(stream, k_pages.device)))
+        new_len = T.empty(n_seq, dtype=T.i32, device=k_pages.device)
+    rc = T.compact(ctx, C.byref(kv), block_table.data_ptr(), block_table.stride(0), width,
+                   _array(context_len, "context_len", T.i32, n_seq, dev), _array(accepted, "accepted", T.i64, n_seq, dev), n_seq,
+                   _array(new_len, "new_len", T.i32, n_seq, dev), _stream(stream, dev))
+    if rc:
+        check(rc)
     return new_len
 
 
@@ -241,29 +257,29 @@ def sample_dev(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
     [0, 1) (pyxis_cuda_sample_dev).  Each parameter is a number for all rows or a device tensor [M]
     (float32; ``top_k`` int32).  Temperature 0 is the greedy choice.  Returns (idx int32 [M],
     prob float32 [M]: the token's share of the kept weights)."""
-    import torch
-
     if logits.dim() == 1:
         logits = logits.unsqueeze(0)
-    ctx = _where(logits)
+    T, dev, ctx = _begin(logits)
     M, n = logits.shape
-    if n > 1 and logits.stride(1) != 1:
-        _fail("the logits of a row must be contiguous")
-    p = _SampleParams(None, None, None, None, 1.0, 0, 1.0, 0.0)
-    for name, value, kind in (("temperature", temperature, "torch.float32"), ("top_k", top_k, "torch.int32"),
-                              ("top_p", top_p, "torch.float32"), ("min_p", min_p, "torch.float32")):
-        if isinstance(value, torch.Tensor):
-            setattr(p, name, _array(value, name, kind, M, ctx))
-        else:
-            setattr(p, name + "_all", value)
+    kind = T.types.get(logits.dtype)
+    if kind is None or (n > 1 and logits.stride(1) != 1):
+        _fail(f"logits of {logits.dtype}: float32 or bfloat16 with contiguous rows are needed")
+
+    def per_row(value, what, dtype):
+        return _array(value, what, dtype, M, dev) if isinstance(value, T.Tensor) else None
+
+    t, k, p, m = (per_row(temperature, "temperature", T.f32), per_row(top_k, "top_k", T.i32), per_row(top_p, "top_p", T.f32),
+                  per_row(min_p, "min_p", T.f32))
+    params = _SampleParams(t, k, p, m, temperature if t is None else 1.0, top_k if k is None else 0, top_p if p is None else 1.0,
+                           min_p if m is None else 0.0)
     if idx is None:
-        idx = torch.empty(M, dtype=torch.int32, device=logits.device)
+        idx = T.empty(M, dtype=T.i32, device=logits.device)
     if prob is None:
-        prob = torch.empty(M, dtype=torch.float32, device=logits.device)
-    check(_native.lib().pyxis_cuda_sample_dev(
-        ctx.handle, logits.data_ptr(), _dtype(logits), M, n, logits.stride(0), _array(uniforms, "uniforms", "torch.float32", M, ctx),
-        C.byref(p), _array(idx, "idx", "torch.int32", M, ctx), _array(prob, "prob", "torch.float32", M, ctx),
-        _stream(stream, logits.device)))
+        prob = T.empty(M, dtype=T.f32, device=logits.device)
+    rc = T.sample(ctx, logits.data_ptr(), kind, M, n, logits.stride(0), _array(uniforms, "uniforms", T.f32, M, dev), C.byref(params),
+                  _array(idx, "idx", T.i32, M, dev), _array(prob, "prob", T.f32, M, dev), _stream(stream, dev))
+    if rc:
+        check(rc)
     return idx, prob
 
 
