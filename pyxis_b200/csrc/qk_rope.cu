@@ -8,9 +8,11 @@
 // Bytes bound it: every element is read once and written once.  A head lies across HD / V lanes
 // with V = 16 bytes of elements each, so the norm is a shuffle sum and the rotation's partner a
 // shuffle away (halves) or in the same register vector (interleaved pairs).  The angles of a
-// token are the same for all its heads: the CTA forms them once, in 64 bits (position * frequency
-// has far more than 24 significant bits at far positions; reduced by multiples of pi/2 to
-// [-pi/4, pi/4] before it is rounded to f32), while the heads' loads are in flight.
+// token are the same for all its heads: a warp takes a token (or a part of its heads), forms the
+// angles once, in 64 bits (position * frequency has far more than 24 significant bits at far
+// positions; reduced by multiples of pi/2 to [-pi/4, pi/4] before it is rounded to f32), while the
+// first heads' loads are in flight, and keeps its factors in registers.  Warps share nothing, so
+// one's angles overlap the others' traffic.
 #include <cuda_bf16.h>
 
 #include "common.cuh"
@@ -20,8 +22,7 @@ namespace pyxis {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kUnroll = 4;      // heads in flight per lane group
-constexpr int kMaxTokens = 4;   // tokens per CTA
+constexpr int kUnroll = 4;  // accesses in flight per warp and kind
 
 // 16 bytes of T as f32.
 template <typename T>
@@ -77,7 +78,7 @@ struct RopeParams {
     char *q, *k, *v;
     long long ld_qkv, ld_q;                           // bytes
     long long page_stride, slot_stride, head_stride;  // bytes
-    int n_tokens, n_q, n_kv, page_size, num_slots, rot, interleaved, tokens_per_cta;
+    int n_tokens, n_q, n_kv, page_size, num_slots, rot, interleaved, parts;
     const int32_t *positions, *slots;
     const double *inv_freq;
     const float *q_norm, *k_norm;
@@ -87,91 +88,117 @@ struct RopeParams {
 template <typename T, int HD>
 __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const RopeParams p) {
     constexpr int V = Vec<T>::N, L = HD / V;  // lanes of a head
-    constexpr int kGroups = kThreads / L;
-    __shared__ float2 cs[kMaxTokens][HD / 2];
+    constexpr int kHeads = 32 / L, kHead = HD * (int)sizeof(T);  // heads of a warp's access
+    __shared__ float2 cs[kThreads / 32][HD / 2];
     pdl_wait();
     pdl_trigger();
-    const int t0 = blockIdx.x * p.tokens_per_cta;
-    const int nt = min(p.tokens_per_cta, p.n_tokens - t0);
-    const int heads = p.n_q + 2 * p.n_kv, items = nt * heads;
-    const int group = threadIdx.x / L, li = threadIdx.x % L;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int job = blockIdx.x * (kThreads / 32) + warp, t = job / p.parts, part = job - t * p.parts;
+    if (t >= p.n_tokens) return;
+    const int li = lane % L, sub = lane / L;
     const int half = p.rot / 2;
     const int off = half / V;  // lanes between the partners of the halves form
-    bool have_angles = false;
+    const bool first = li < off, turns = p.interleaved ? li * V < p.rot : li < 2 * off;
+    const int partner = first ? li + off : turns ? li - off : li;
+    const int step = p.parts * kHeads, h0 = part * kHeads + sub;  // this lane group's heads: h0, h0 + step, ...
+    const char *src = p.qkv + t * p.ld_qkv + li * 16;
+    const char *ksrc = src + p.n_q * kHead, *vsrc = ksrc + p.n_kv * kHead;
 
-    // item = token-major (token, head); the trip count is the same for every group of the CTA
-    for (int base = 0; base < items; base += kGroups * kUnroll) {
-        uint4 raw[kUnroll];
+    auto load = [&](const char *base, int h, int heads, uint4 (&raw)[kUnroll]) {
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
-            const int it = base + u * kGroups + group;
-            if (it < items)
-                raw[u] = *reinterpret_cast<const uint4 *>(p.qkv + (t0 + it / heads) * p.ld_qkv +
-                                                          (size_t)(it % heads) * HD * sizeof(T) + li * 16);
-            else
-                raw[u] = make_uint4(0, 0, 0, 0);
+            raw[u] = make_uint4(0, 0, 0, 0);
+            if (h + u * step < heads) raw[u] = *reinterpret_cast<const uint4 *>(base + (h + u * step) * kHead);
         }
-        if (!have_angles) {
-            for (int i = threadIdx.x; i < nt * half; i += kThreads) {
-                const int t = i / half, f = i - t * half;
-                float2 c = cos_sin(p.positions[t0 + t], p.inv_freq[f]);
-                cs[t][f] = make_float2(c.x * p.scale, c.y * p.scale);
+    };
+    uint4 raw[kUnroll];
+    load(src, h0, p.n_q, raw);  // on its way while the angles are formed
+    const int slot = p.slots[t];
+    // this lane's rotation factors: its pairs' (c, s), or with halves each of its elements' c and the
+    // partner's signed s
+    float2 f[V];
+    if (p.rot) {
+        const int pos = p.positions[t];
+        for (int i = lane; i < half; i += 32) {
+            const float2 c = cos_sin(pos, p.inv_freq[i]);
+            cs[warp][i] = make_float2(c.x * p.scale, c.y * p.scale);
+        }
+        __syncwarp();
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            f[e] = f2(1.f, 0.f);
+            if (p.interleaved) {
+                if (turns && e < V / 2) f[e] = cs[warp][li * (V / 2) + e];
+            } else if (turns) {
+                f[e] = cs[warp][(first ? li : li - off) * V + e];
+                f[e].y = first ? -f[e].y : f[e].y;
             }
-            __syncthreads();
-            have_angles = true;
         }
+    }
+    auto weights = [&](const float *w, float (&out)[V]) {
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            const int it = base + u * kGroups + group;
-            const int t = it < items ? it / heads : 0, h = it < items ? it - t * heads : 0;
-            const bool is_q = h < p.n_q, is_v = h >= p.n_q + p.n_kv;
-            float x[V];
-            Vec<T>::load(raw[u], x);
-            const float *w = is_v ? nullptr : is_q ? p.q_norm : p.k_norm;
+        for (int e = 0; e < V; ++e) out[e] = w ? __ldg(w + li * V + e) : 1.f;
+    };
+    // a head's norm and rotation
+    auto turn = [&](uint4 in, const float (&w)[V], bool norm) -> uint4 {
+        float x[V];
+        Vec<T>::load(in, x);
+        if (norm) {
             float ss = 0.f;
 #pragma unroll
             for (int e = 0; e < V; ++e) ss = fmaf(x[e], x[e], ss);
 #pragma unroll
             for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            if (w) {
-                const float f = rms_factor(ss, HD, p.eps);
+            const float r = rsqrtf(fmaf(ss, 1.0f / HD, p.eps));
 #pragma unroll
-                for (int e = 0; e < V; ++e) x[e] = rms_scale(x[e], f, __ldg(w + li * V + e));
-            }
+            for (int e = 0; e < V; ++e) x[e] *= r * w[e];
+        }
+        if (p.rot) {
             if (p.interleaved) {
-                if (!is_v && li * V < p.rot) {
 #pragma unroll
-                    for (int e = 0; e < V; e += 2) {
-                        const float2 c = cs[t][(li * V + e) / 2];
-                        const float a = x[e], b = x[e + 1];
-                        x[e] = rope_rot(a, b, c.x, c.y, true);
-                        x[e + 1] = rope_rot(b, a, c.x, c.y, false);
-                    }
+                for (int e = 0; e < V; e += 2) {
+                    const float a = x[e], b = x[e + 1];
+                    x[e] = fmaf(a, f[e / 2].x, -(b * f[e / 2].y));
+                    x[e + 1] = fmaf(b, f[e / 2].x, a * f[e / 2].y);
                 }
             } else {
-                const bool first = li < off, turns = li < 2 * off;
-                const int src = first ? li + off : turns ? li - off : li;
 #pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    const float other = __shfl_sync(0xffffffffu, x[e], src, L);
-                    if (!is_v && turns) {
-                        const float2 c = cs[t][(first ? li : li - off) * V + e];
-                        x[e] = rope_rot(x[e], other, c.x, c.y, first);
-                    }
-                }
+                for (int e = 0; e < V; ++e)
+                    x[e] = fmaf(x[e], f[e].x, __shfl_sync(0xffffffffu, x[e], partner, L) * f[e].y);
             }
-            if (it >= items) continue;
-            const uint4 out = is_v ? raw[u] : Vec<T>::store(x);
-            if (is_q) {
-                *reinterpret_cast<uint4 *>(p.q + (t0 + t) * p.ld_q + (size_t)h * HD * sizeof(T) + li * 16) = out;
-            } else {
-                const int slot = __ldg(p.slots + t0 + t);
-                if (slot >= 0 && slot < p.num_slots) {
-                    const int page = slot / p.page_size, kh = is_v ? h - p.n_q - p.n_kv : h - p.n_q;
-                    char *dst = (is_v ? p.v : p.k) + page * p.page_stride + (slot - page * p.page_size) * p.slot_stride +
-                                kh * p.head_stride;
-                    *reinterpret_cast<uint4 *>(dst + li * 16) = out;
-                }
+        }
+        return Vec<T>::store(x);
+    };
+
+    // queries, keys, values; the trip counts are the whole warp's
+    float w[V];
+    weights(p.q_norm, w);
+    for (int h = h0, base = part * kHeads; base < p.n_q; h += step * kUnroll, base += step * kUnroll) {
+        if (h != h0) load(src, h, p.n_q, raw);
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            if (base + u * step >= p.n_q) break;  // of the whole warp
+            const uint4 x = turn(raw[u], w, p.q_norm != nullptr);
+            if (h + u * step < p.n_q)
+                *reinterpret_cast<uint4 *>(p.q + t * p.ld_q + (h + u * step) * kHead + li * 16) = x;
+        }
+    }
+    if (slot < 0 || slot >= p.num_slots) return;
+    const int page = slot / p.page_size;
+    const long long at = page * p.page_stride + (slot - page * p.page_size) * p.slot_stride + li * 16;
+    weights(p.k_norm, w);
+    for (int h = h0, base = part * kHeads; base < p.n_kv; h += step * kUnroll, base += step * kUnroll) {
+        uint4 v[kUnroll];
+        load(ksrc, h, p.n_kv, raw);
+        load(vsrc, h, p.n_kv, v);
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            if (base + u * step >= p.n_kv) break;
+            const uint4 x = turn(raw[u], w, p.k_norm != nullptr);
+            if (h + u * step < p.n_kv) {
+                const long long to = at + (h + u * step) * p.head_stride;
+                *reinterpret_cast<uint4 *>(p.k + to) = x;
+                *reinterpret_cast<uint4 *>(p.v + to) = v[u];
             }
         }
     }
@@ -199,8 +226,9 @@ cudaError_t launch_qk_norm_rope(const pyxis_qk_norm_rope_args &a, const pyxis_kv
     p.num_slots = kv.num_pages * kv.page_size;
     p.rot = a.rotary_dim;
     p.interleaved = a.interleaved;
-    // one token per CTA until the tokens cover the GPU a few times over
-    p.tokens_per_cta = a.n_tokens <= (size_t)num_sms * 8 ? 1 : kMaxTokens;
+    // a token's heads are dealt to up to 8 warps while the tokens alone do not fill the GPU
+    p.parts = 1;
+    while (p.parts < 8 && a.n_tokens * p.parts * 2 <= (size_t)num_sms * 32) p.parts *= 2;
     p.positions = a.positions;
     p.slots = a.slots;
     p.inv_freq = a.inv_freq;
@@ -208,7 +236,7 @@ cudaError_t launch_qk_norm_rope(const pyxis_qk_norm_rope_args &a, const pyxis_kv
     p.k_norm = a.k_norm;
     p.eps = a.eps;
     p.scale = a.rope_scale;
-    const dim3 grid((unsigned)((a.n_tokens + p.tokens_per_cta - 1) / p.tokens_per_cta));
+    const dim3 grid((unsigned)((a.n_tokens * p.parts + kThreads / 32 - 1) / (kThreads / 32)));
     if (kv.dtype == PYXIS_DTYPE_F32)
         return kv.head_dim == 128 ? launch_kernel(qk_norm_rope_kernel<float, 128>, grid, dim3(kThreads), 0, st, p)
                                   : launch_kernel(qk_norm_rope_kernel<float, 64>, grid, dim3(kThreads), 0, st, p);
