@@ -1,6 +1,8 @@
 // paged.cu -- page copies (forks) and the compaction of accepted drafts in a paged KV cache
 // (the cache of src/kv_cache.rs:34-41 cut into pages; include/pyxis_serve.h).  Both only move
 // bytes: 16 bytes per thread and access, several accesses in flight.
+#include <algorithm>
+
 #include "common.cuh"
 #include "serve.h"
 
@@ -9,7 +11,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kCopyUnroll = 4;
-constexpr int kMoveUnroll = 16;  // moves of one column in flight
+constexpr int kMoveUnroll = 8;  // moves of one column in flight
 
 struct PageGeom {
     char *k, *v;
@@ -55,10 +57,12 @@ __global__ void __launch_bounds__(kThreads) kv_copy_pages_kernel(const PageGeom 
         if (first + u * kThreads < vecs) *reinterpret_cast<uint4 *>(to + at[u]) = x[u];
 }
 
-// grid (2 * layers, sequences); a thread takes 16-byte columns of the rows and moves each through
-// all of the sequence's moves in order.  A move's place is never a later move's source: node j of
-// rank r goes to r <= j, and later sources lie beyond j.  So a batch of loads may run ahead of its
-// stores, and one thread's order of accesses to its column is all the ordering needed.
+// grid (parts, sequences): the 16-byte columns of a sequence's rows, over all layers' keys and values,
+// are dealt to the threads of its parts.  A thread moves its column through all of the sequence's
+// moves in order.  A move's place is never a later move's source: node j of rank r goes to r <= j,
+// and later sources lie beyond j.  So a batch of loads may run ahead of its stores, and one thread's
+// order of accesses to its column is all the ordering needed.  Latency bounds it (the mask, the
+// table, then the rows): a CTA forms the moves once for several columns per thread.
 __global__ void __launch_bounds__(kThreads)
     kv_compact_kernel(const PageGeom g, const int32_t *__restrict__ table, long long table_stride, int table_width,
                       const int32_t *__restrict__ context_len, const unsigned long long *__restrict__ accepted,
@@ -89,10 +93,10 @@ __global__ void __launch_bounds__(kThreads)
         }
     }
     __syncthreads();
-    char *base = ((blockIdx.x & 1) ? g.v : g.k) + (long long)(blockIdx.x >> 1) * g.layer_stride;
-    for (int c = threadIdx.x; c < g.n_kv * g.row_vecs; c += kThreads) {
-        const int head = c / g.row_vecs;
-        char *col = base + head * g.head_stride + (c - head * g.row_vecs) * 16;
+    const int cols = g.n_kv * g.row_vecs, total = 2 * g.n_layers * cols;
+    for (int i = blockIdx.x * kThreads + threadIdx.x; i < total; i += gridDim.x * kThreads) {
+        const int plane = i / cols, c = i - plane * cols, head = c / g.row_vecs;
+        char *col = ((plane & 1) ? g.v : g.k) + (plane >> 1) * g.layer_stride + head * g.head_stride + (c - head * g.row_vecs) * 16;
         for (int m0 = 0; m0 < moves; m0 += kMoveUnroll) {
             uint4 x[kMoveUnroll];
 #pragma unroll
@@ -126,9 +130,12 @@ cudaError_t launch_kv_copy_pages(const pyxis_kv_pages &kv, const int32_t *src, c
 
 cudaError_t launch_kv_compact(const pyxis_kv_pages &kv, const int32_t *block_table, size_t table_stride,
                               size_t table_width, const int32_t *context_len, const uint64_t *accepted, size_t n_seq,
-                              int32_t *new_len, cudaStream_t st) {
-    return launch_kernel(kv_compact_kernel, dim3(2 * kv.n_layers, (unsigned)n_seq), dim3(kThreads), 0, st, geom(kv),
-                         block_table, (long long)table_stride, (int)table_width, context_len,
+                              int32_t *new_len, int num_sms, cudaStream_t st) {
+    const PageGeom g = geom(kv);
+    // about four CTAs an SM, and no more than one column per thread
+    const size_t total = (size_t)2 * kv.n_layers * kv.n_kv_heads * g.row_vecs;
+    const size_t parts = std::max<size_t>(1, std::min((total + kThreads - 1) / kThreads, (size_t)num_sms * 4 / n_seq));
+    return launch_kernel(kv_compact_kernel, dim3((unsigned)parts, (unsigned)n_seq), dim3(kThreads), 0, st, g, block_table, (long long)table_stride, (int)table_width, context_len,
                          (const unsigned long long *)accepted, new_len);
 }
 

@@ -30,7 +30,7 @@ cudaError_t launch_kv_copy_pages(const pyxis_kv_pages &kv, const int32_t *src, c
                                  cudaStream_t st);
 cudaError_t launch_kv_compact(const pyxis_kv_pages &kv, const int32_t *block_table, size_t table_stride,
                               size_t table_width, const int32_t *context_len, const uint64_t *accepted, size_t n_seq,
-                              int32_t *new_len, cudaStream_t st);
+                              int32_t *new_len, int num_sms, cudaStream_t st);
 
 cudaError_t launch_sample(const void *logits, int dtype, size_t M, size_t n, size_t ld, const float *uniforms,
                           const pyxis_sample_params &p, int32_t *idx, float *prob, int num_sms, cudaStream_t st);

@@ -221,6 +221,7 @@ int pyxis_cuda_kv_compact_dev(pyxis_cuda_ctx *ctx, const pyxis_kv_pages *kv, con
     if (n_seq == 0) return PYXIS_OK;
     if (!block_table || !context_len || !accepted || !new_len)
         return fail(PYXIS_EINVAL, "null block_table, context_len, accepted or new_len");
+    if ((long long)kv->n_layers * kv->n_kv_heads * kv->head_dim >= (1ll << 30)) return fail(PYXIS_EINVAL, "cache rows too long");
     if (n_seq > 65535 || table_width > (size_t)INT32_MAX) return fail(PYXIS_EINVAL, "more than 65535 sequences, or too wide a table");
     if (n_seq > 1 && table_stride < table_width)
         return fail(PYXIS_EINVAL, "block table rows of %zu with stride %zu", table_width, table_stride);
@@ -228,7 +229,7 @@ int pyxis_cuda_kv_compact_dev(pyxis_cuda_ctx *ctx, const pyxis_kv_pages *kv, con
     if (!ctx) return fail(PYXIS_EINVAL, "null context");
     DeviceGuard g(ctx->device);
     return cuda_status(launch_kv_compact(*kv, block_table, table_stride, table_width, context_len, accepted, n_seq, new_len,
-                                         pick_stream(ctx, stream)),
+                                         ctx->num_sms, pick_stream(ctx, stream)),
                        "kv_compact launch");
 }
 
