@@ -43,9 +43,9 @@ constexpr int kPerThread = kBins / kThreads;
 constexpr float kBinsPerNat = 32.0f;
 constexpr int kCand = 2048;  // elements that the leader takes
 constexpr int kMaxTopK = 1024;
-constexpr int kRank = 32;    // elements that a warp ranks
+constexpr int kRank = 128;   // elements that are ranked against one another
 constexpr int kMaxCluster = 8;
-constexpr int kTable = 256;  // 2^(-j / 256)
+constexpr int kTable = 256;  // steps of 2 in the exponentials' table
 
 struct SampleArgs {
     const void *logits;
@@ -79,7 +79,7 @@ struct Shared {
         Histogram sub;  // of a key range, while the cluster cuts a set down
     };
     Histogram row;      // of the row; then, in the leader, of the candidates' key range
-    double table[kTable];
+    double table[kTable];  // 2^(shift - j / 256)
     u64 scan[kWarps];
     unsigned scan_cnt[kWarps];
     u64 rank_min[kMaxCluster], rank_max[kMaxCluster], rank_mass[kMaxCluster];
@@ -88,13 +88,17 @@ struct Shared {
     int bin[4];         // its bin (the last bin of a top-k set), -1: nothing to seek
     unsigned ncand;
     Range narrow;
-    u64 few[kRank];
+    u64 few[kRank], few_w[kRank];
     unsigned nfew;
     u64 found_mass, found_w, found_key;
 };
 
 PYXIS_DEVINL float widen(float x) { return x; }
 PYXIS_DEVINL float widen(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T>
+PYXIS_DEVINL T lowest() {
+    return T(-INFINITY);
+}
 
 // Order-preserving key of a finite or infinite value and its index: larger values first, then
 // smaller indexes; -0 ties with +0.
@@ -127,23 +131,28 @@ struct Row {
     const double *table;
     // the bin of x, or -1 if its weight is 0
     PYXIS_DEVINL int bin(float x) const {
-        if (x == top) return 0;
         const float f = (top - x) * bin_scale;
-        return f < (float)(last_bin + 1) ? (int)f : -1;  // NaN and infinite distances: -1
+        const int b = f < (float)(last_bin + 1) ? (int)f : -1;  // NaN and infinite distances: -1
+        return x == top ? 0 : b;
     }
-    // exp((x - top) / temperature) 2^shift, rounded: 2^(-k / 256) from the table, times exp of the
-    // rest, |rest| <= ln 2 / 512, by its Taylor polynomial (cubic: off by 2^-47 of the weight)
+    // a bound: values below it are in later bins than b (the bins' own rounding is far within 1e-3 bins)
+    PYXIS_DEVINL float floor_of(int b) const {
+        return b >= last_bin || isinf(top) ? -INFINITY : top - (float)(b + 1) * (1.001f / bin_scale) - fabsf(top) * 1e-6f;
+    }
+    // exp((x - top) / temperature) 2^shift, rounded: 2^(shift - k / 256) from the table, times exp of
+    // the rest d ln 2 / 256, |d| <= 1/2, by its Taylor polynomial (cubic: off by 2^-47 of the weight)
     PYXIS_DEVINL u64 weight(float x) const {
-        if (x == top) return 1ull << shift;
-        const double u = ((double)top - (double)x) * steps;
+        constexpr double c = 0.69314718055994530942 / kTable;
         constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: rounds to a whole number
+        const double u = ((double)top - (double)x) * steps;
         const double m = u + kRound;
         const int k = __double2loint(m);  // valid bins: u < 2^14
-        const double rest = ((m - kRound) - u) * (0.69314718055994530942 / kTable);
-        double e = fma(rest, fma(rest, fma(rest, 1.0 / 6.0, 0.5), 1.0), 1.0) * table[k & (kTable - 1)];
-        // times 2^(shift - k / 256), then rounded to a whole number in the low bits
-        e *= __hiloint2double((1023 + shift - (k >> 8)) << 20, 0);
-        return (u64)__double_as_longlong(e + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
+        const double d = (m - kRound) - u;
+        double e = fma(d, fma(d, fma(d, c * c * c / 6.0, c * c / 2.0), c), 1.0) * table[k & (kTable - 1)];
+        e = __hiloint2double(__double2hiint(e) - ((k >> 8) << 20), __double2loint(e));  // 2^-(k / 256)
+        // to a whole number in the low bits
+        const u64 w = (u64)__double_as_longlong(e + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
+        return x == top ? 1ull << shift : w;
     }
 };
 
@@ -193,9 +202,9 @@ PYXIS_DEVINL void clear(Histogram &h) {
     for (int b = threadIdx.x; b < kBins; b += kThreads) h.lo[b] = h.hi[b] = h.cnt[b] = 0;
 }
 PYXIS_DEVINL int shift_for(u64 lo, u64 hi) {  // (hi - key) >> shift is a bin
-    int sh = 0;
-    while (((hi - lo) >> sh) >= kBins) ++sh;
-    return sh;
+    static_assert(kBins == 1 << 10, "");
+    const int bits = 64 - __clzll((long long)(hi - lo));
+    return bits > 10 ? bits - 10 : 0;
 }
 
 // The bin of a key-range histogram where the running count (by_count) or weight passes t becomes
@@ -222,6 +231,15 @@ PYXIS_DEVINL void pick_bin(const Histogram &h, const Range &in, int sh, bool by_
         em += wide(h, b), ec += h.cnt[b];
     }
     __syncthreads();
+}
+
+// Ranks n <= kRank keys of s.few against one another (weights in s.few_w): thread i < n gets the
+// weight and the number of those before its own.
+PYXIS_DEVINL void rank_few(const Shared &s, unsigned n, u64 &before, unsigned &rank) {
+    if (threadIdx.x >= n) return;
+    const u64 k = s.few[threadIdx.x];
+    for (unsigned i = 0; i < n; ++i)
+        if (s.few[i] > k) before += s.few_w[i], ++rank;
 }
 
 // Leader: among the candidates, whose first follows ex_mass and ex_count, the element where the
@@ -256,23 +274,21 @@ PYXIS_DEVINL void locate(Shared &s, const Row &r, unsigned n, u64 ex_mass, unsig
     lo = s.narrow.lo, hi = s.narrow.hi;
     for (unsigned i = threadIdx.x; i < n; i += kThreads) {
         const u64 k = s.cand[i];
-        if (k >= lo && k <= hi) s.few[atomicAdd(&s.nfew, 1u)] = k;
+        if (k < lo || k > hi) continue;
+        const unsigned at = atomicAdd(&s.nfew, 1u);
+        s.few[at] = k;
+        s.few_w[at] = r.weight(value_of(k));
     }
     __syncthreads();
-    if (threadIdx.x < 32) {
-        const unsigned few = s.nfew, lane = threadIdx.x;
-        const u64 k = lane < few ? s.few[lane] : 0;
-        const u64 w = lane < few ? r.weight(value_of(k)) : 0;
-        u64 before = s.narrow.ex_mass;
-        unsigned rank = s.narrow.ex_count;
-        for (unsigned i = 0; i < few; ++i) {
-            const u64 ki = __shfl_sync(0xffffffffu, k, i), wi = __shfl_sync(0xffffffffu, w, i);
-            if (ki > k) before += wi, ++rank;
-        }
-        if (lane < few && (by_count ? rank == t : t >= before && t - before < w)) {
+    u64 before = s.narrow.ex_mass;
+    unsigned rank = s.narrow.ex_count;
+    rank_few(s, s.nfew, before, rank);
+    if (threadIdx.x < s.nfew) {
+        const u64 w = s.few_w[threadIdx.x];
+        if (by_count ? rank == t : t >= before && t - before < w) {
             s.found_mass = before + w;
             s.found_w = w;
-            s.found_key = k;
+            s.found_key = s.few[threadIdx.x];
         }
     }
     __syncthreads();
@@ -319,10 +335,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     // shared memory holds the segment at the 16-byte phase it has in global memory
     const unsigned phase = (unsigned)((reinterpret_cast<uintptr_t>(src) & 15) / sizeof(T));
     T *own = vals + phase;
-    auto value = [&](unsigned i) -> float { return widen(i < held ? own[i] : src[i]); };
 
+    // (elements before and after it in its 16-byte vectors are -inf there)
     float mine = -INFINITY;
-    const unsigned head = min(held, (V - phase) % V), vecs = (held - head) / V;
+    const unsigned head = min(held, (V - phase) % V), vecs = (held - head) / V, all_vecs = (phase + held + V - 1) / V;
     {
         const uint4 *g = reinterpret_cast<const uint4 *>(src + head);
         uint4 *d = reinterpret_cast<uint4 *>(own + head);
@@ -335,12 +351,36 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
             for (unsigned j = 0; j < V; ++j) mine = fmaxf(mine, widen(e[j]));
         }
     }
+    const T none = lowest<T>();
+    if (tid < (int)phase) vals[tid] = none;
+    if (phase + held + tid < all_vecs * V) own[held + tid] = none;
     if (tid < (int)head) own[tid] = src[tid], mine = fmaxf(mine, widen(src[tid]));
     for (unsigned i = head + vecs * V + tid; i < held; i += kThreads) own[i] = src[i], mine = fmaxf(mine, widen(src[i]));
     for (unsigned i = held + tid; i < len; i += kThreads) mine = fmaxf(mine, widen(src[i]));
+    // fn(values, index of the first, how many) for every element: four at a time from shared memory,
+    // then one by one what it does not hold
+    auto scan = [&](auto &&fn) {
+        constexpr unsigned H = V / 4;
+        for (unsigned i = tid; i < all_vecs * H; i += kThreads) {
+            float x[4];
+            if constexpr (sizeof(T) == 4) {
+                const float4 v = reinterpret_cast<const float4 *>(vals)[i];
+                x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+            } else {
+                const uint2 v = reinterpret_cast<const uint2 *>(vals)[i];
+                x[0] = __uint_as_float(v.x << 16), x[1] = __uint_as_float(v.x & 0xFFFF0000u);
+                x[2] = __uint_as_float(v.y << 16), x[3] = __uint_as_float(v.y & 0xFFFF0000u);
+            }
+            fn(x, (int)(i * 4) - (int)phase);
+        }
+        for (unsigned i = held + tid; i < len; i += kThreads) {
+            const float x[4] = {widen(src[i]), -INFINITY, -INFINITY, -INFINITY};
+            fn(x, (int)i);
+        }
+    };
     clear(s.row);
     if (tid == 0) s.ncand = 0;
-    if (tid < kTable) s.table[tid] = exp2(-(double)tid / kTable);
+    if (tid < kTable) s.table[tid] = exp2(a.shift - (double)tid / kTable);
     float top = mine;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -366,11 +406,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     const double temperature = a.temperature ? (double)a.temperature[row] : a.temperature_all;
     if (!(temperature > 0.0)) {  // greedy: the first maximum
         u64 best = 0, least = ~0ull;
-        for (unsigned i = tid; i < len; i += kThreads)
-            if (value(i) == r.top) {
-                best = key_of(r.top, (unsigned)(beg + i));
-                break;
-            }
+        scan([&](const float (&x)[4], int i) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (x[j] == r.top) {
+                    const u64 k = key_of(r.top, (unsigned)(beg + i + j));
+                    best = k > best ? k : best;
+                }
+        });
         block_range(least, best, s);
         if (tid == 0) leader.rank_max[rank] = best;
         cluster.sync();
@@ -391,19 +434,24 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     q.top_p = a.top_p ? (double)a.top_p[row] : a.top_p_all;
     q.min_p = a.min_p ? (double)a.min_p[row] : a.min_p_all;
     q.u = (double)a.u[row];
-    const double least = fmin(q.min_p, 1.0) * (double)(1ull << r.shift);  // weights that min_p keeps
+    // weights that min_p keeps: w >= min_p 2^shift
+    const u64 least = q.min_p > 0.0 ? (u64)ceil(fmin(q.min_p, 1.0) * (double)(1ull << r.shift)) : 0;
 
     // every element of bins first .. last of key lo .. hi into the leader's candidates
     auto gather = [&](int first, int last, u64 lo, u64 hi) {
-        for (unsigned i = tid; i < len; i += kThreads) {
-            const float x = value(i);
-            const int b = r.bin(x);
-            if (b < first || b > last) continue;
-            const u64 k = key_of(x, (unsigned)(beg + i));
-            if (k < lo || k > hi) continue;
-            const unsigned at = atomicAdd(&leader.ncand, 1u);
-            if (at < kCand) leader.cand[at] = k;
-        }
+        const float floor = r.floor_of(last);
+        scan([&](const float (&x)[4], int i) {
+            if (!(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) >= floor)) return;  // most are far below
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int b = r.bin(x[j]);
+                if (b < first || b > last) continue;
+                const u64 k = key_of(x[j], (unsigned)(beg + i + j));
+                if (k < lo || k > hi) continue;
+                const unsigned at = atomicAdd(&leader.ncand, 1u);
+                if (at < kCand) leader.cand[at] = k;
+            }
+        });
     };
 
     // ---- a set that settles everything: the whole row, or what top_k can keep
@@ -442,13 +490,41 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
                 cluster.sync();  // the leader's count has been read
                 return;
             }
+            cluster.sync();
+            if (n <= kRank) {  // one ranking answers all three
+                u64 w = 0, before = 0;
+                unsigned at = 0;
+                if (tid < (int)n) s.few[tid] = s.cand[tid], s.few_w[tid] = w = r.weight(value_of(s.cand[tid]));
+                __syncthreads();
+                rank_few(s, n, before, at);
+                const bool in = tid < (int)n && (q.top_k <= 0 || at < (unsigned)q.top_k);  // top-k keeps it
+                const u64 total = block_sum(in ? w : 0, s);
+                u64 kept = total;
+                if (q.min_p > 0.0) {
+                    const u64 above = block_sum(in && w >= least ? w : 0, s);
+                    kept = above < kept ? above : kept;
+                }
+                if (q.top_p < 1.0) {
+                    const u64 t = q.top_p_target(total);
+                    if (in && t >= before && t - before < w) s.found_mass = before + w;
+                    __syncthreads();
+                    kept = s.found_mass < kept ? s.found_mass : kept;
+                }
+                const u64 t = q.draw_target(kept);
+                if (in && t >= before && t - before < w) {
+                    s.found_w = w;
+                    s.found_key = s.few[tid];
+                }
+                __syncthreads();
+                write_result(a, row, s, kept);
+                return;
+            }
             u64 total = 0, above = 0;
             for (unsigned i = tid; i < n; i += kThreads) {
                 const u64 w = r.weight(value_of(s.cand[i]));
                 total += w;
-                if ((double)w >= least) above += w;
+                if (w >= least) above += w;
             }
-            cluster.sync();
             total = block_sum(total, s);
             if (q.top_k > 0 && (unsigned)q.top_k < n) {
                 locate(s, r, n, 0, 0, true, (u64)q.top_k - 1);
@@ -478,15 +554,19 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     {
         u64 above = 0;  // weight of the elements that min_p keeps
         const bool count = q.top_k > 0;
-        for (unsigned i = tid; i < len; i += kThreads) {
-            const float x = value(i);
-            const int b = r.bin(x);
-            if (b < 0) continue;
-            const u64 w = r.weight(x);
-            if ((double)w >= least) above += w;
-            add_wide(&s.row.lo[b], &s.row.hi[b], w);
-            if (count) atomicAdd(&s.row.cnt[b], 1u);
-        }
+        scan([&](const float (&x)[4], int) {
+            int b[4];
+            u64 w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) b[j] = r.bin(x[j]), w[j] = r.weight(x[j]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (b[j] < 0) continue;  // its w is meaningless
+                if (w[j] >= least) above += w[j];
+                add_wide(&s.row.lo[b[j]], &s.row.hi[b[j]], w[j]);
+                if (count) atomicAdd(&s.row.cnt[b[j]], 1u);
+            }
+        });
         above = block_sum(above, s);
         if (tid == 0) leader.rank_mass[rank] = above;
         if (rank != 0)
@@ -558,13 +638,15 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
         if (count > kCand) {
             // the bin's range of keys; then each round leaves 1 / kBins of it, down to single keys
             u64 lo = ~0ull, hi = 0;
-            for (unsigned i = tid; i < len; i += kThreads) {
-                const float x = value(i);
-                if (r.bin(x) != bin) continue;
-                const u64 k = key_of(x, (unsigned)(beg + i));
-                lo = k < lo ? k : lo;
-                hi = k > hi ? k : hi;
-            }
+            scan([&](const float (&x)[4], int i) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (r.bin(x[j]) != bin) continue;
+                    const u64 k = key_of(x[j], (unsigned)(beg + i + j));
+                    lo = k < lo ? k : lo;
+                    hi = k > hi ? k : hi;
+                }
+            });
             block_range(lo, hi, s);
             if (tid == 0) leader.rank_min[rank] = lo, leader.rank_max[rank] = hi;
             cluster.sync();
@@ -577,15 +659,17 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
                 const int sh = shift_for(lo, hi);
                 clear(s.sub);
                 cluster.sync();
-                for (unsigned i = tid; i < len; i += kThreads) {
-                    const float x = value(i);
-                    if (r.bin(x) != bin) continue;
-                    const u64 k = key_of(x, (unsigned)(beg + i));
-                    if (k < lo || k > hi) continue;
-                    const unsigned b = (unsigned)((hi - k) >> sh);
-                    add_wide(&s.sub.lo[b], &s.sub.hi[b], r.weight(x));
-                    atomicAdd(&s.sub.cnt[b], 1u);
-                }
+                scan([&](const float (&x)[4], int i) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if (r.bin(x[j]) != bin) continue;
+                        const u64 k = key_of(x[j], (unsigned)(beg + i + j));
+                        if (k < lo || k > hi) continue;
+                        const unsigned b = (unsigned)((hi - k) >> sh);
+                        add_wide(&s.sub.lo[b], &s.sub.hi[b], r.weight(x[j]));
+                        atomicAdd(&s.sub.cnt[b], 1u);
+                    }
+                });
                 __syncthreads();
                 if (rank != 0)
                     for (int b = tid; b < kBins; b += kThreads)
@@ -624,6 +708,7 @@ cudaError_t run_sample(SampleArgs &a, size_t M, int num_sms, cudaStream_t st) {
     auto kern = sample_kernel<T>;
     static std::atomic<uint64_t> done{0};
     constexpr size_t fixed = (sizeof(Shared) + 15) / 16 * 16, most = 200 * 1024;
+    constexpr size_t pad = 2 * 16 / sizeof(T);  // a segment's phase, and its last vector's end
     cudaError_t e = once_per_device(done, [&] {
         return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
     });
@@ -633,9 +718,9 @@ cudaError_t run_sample(SampleArgs &a, size_t M, int num_sms, cudaStream_t st) {
     int ranks = 1;
     while (ranks < kMaxCluster && (size_t)ranks * 4096 < a.n) ranks *= 2;
     while (ranks > 1 && M * ranks > (size_t)num_sms * 2 && (a.n / (ranks / 2)) * sizeof(T) + fixed < 112 * 1024) ranks /= 2;
-    const size_t per = (a.n + ranks - 1) / ranks, room = (most - fixed) / sizeof(T) - 16 / sizeof(T);
+    const size_t per = (a.n + ranks - 1) / ranks, room = (most - fixed) / sizeof(T) - pad;
     a.cap = (unsigned)std::min(per, room);
-    const size_t bytes = fixed + (a.cap + 16 / sizeof(T)) * sizeof(T);
+    const size_t bytes = fixed + (a.cap + pad) * sizeof(T);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ranks, (unsigned)M);
     cfg.blockDim = dim3(kThreads);
