@@ -121,6 +121,29 @@ PYXIS_DEVINL void add_wide(unsigned *lo, unsigned *hi, u64 w) {
     const unsigned c = (unsigned)(w >> 32) + (old + wl < old ? 1u : 0u);
     if (c) atomicAdd(hi, c);
 }
+// The adds of four elements (b < 0: none) into this CTA's own histogram: the four low words' atomics
+// are all in flight before the first one's old value is needed for its carry.
+PYXIS_DEVINL void add_wide4(Histogram &h, const int (&b)[4], const u64 (&w)[4], bool count) {
+    const unsigned lo = (unsigned)__cvta_generic_to_shared(h.lo), hi = (unsigned)__cvta_generic_to_shared(h.hi),
+                   cnt = (unsigned)__cvta_generic_to_shared(h.cnt);
+    unsigned old[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        asm volatile("{\n .reg .pred p;\n setp.ge.s32 p, %3, 0;\n mov.u32 %0, 0;\n @p atom.shared.add.u32 %0, [%1], %2;\n}\n"
+                     : "=r"(old[j])
+                     : "r"(lo + 4 * b[j]), "r"((unsigned)w[j]), "r"(b[j])
+                     : "memory");
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const unsigned c = b[j] < 0 ? 0 : (unsigned)(w[j] >> 32) + (old[j] + (unsigned)w[j] < old[j] ? 1u : 0u);
+        asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %1, 0;\n @p red.shared.add.u32 [%0], %1;\n}\n" ::"r"(hi + 4 * b[j]), "r"(c)
+                     : "memory");
+        if (count)
+            asm volatile("{\n .reg .pred p;\n setp.ge.s32 p, %1, 0;\n @p red.shared.add.u32 [%0], 1;\n}\n" ::"r"(cnt + 4 * b[j]),
+                         "r"(b[j])
+                         : "memory");
+    }
+}
 PYXIS_DEVINL u64 wide(const Histogram &h, int b) { return ((u64)h.hi[b] << 32) | h.lo[b]; }
 
 struct Row {
@@ -559,13 +582,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
             u64 w[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) b[j] = r.bin(x[j]), w[j] = r.weight(x[j]);
+            add_wide4(s.row, b, w, count);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (b[j] < 0) continue;  // its w is meaningless
-                if (w[j] >= least) above += w[j];
-                add_wide(&s.row.lo[b[j]], &s.row.hi[b[j]], w[j]);
-                if (count) atomicAdd(&s.row.cnt[b[j]], 1u);
-            }
+            for (int j = 0; j < 4; ++j) above += b[j] >= 0 && w[j] >= least ? w[j] : 0;
         });
         above = block_sum(above, s);
         if (tid == 0) leader.rank_mass[rank] = above;
