@@ -44,7 +44,7 @@ constexpr float kBinsPerNat = 32.0f;
 constexpr int kCand = 2048;  // elements that the leader takes
 constexpr int kMaxTopK = 1024;
 constexpr int kRank = 128;   // elements that are ranked against one another
-constexpr int kMaxCluster = 8;
+constexpr int kMaxCluster = 16;     // 8 is portable; 16 where the device takes it
 constexpr int kTable = 256;  // steps of 2 in the exponentials' table
 
 struct SampleArgs {
@@ -729,30 +729,42 @@ cudaError_t run_sample(SampleArgs &a, size_t M, int num_sms, cudaStream_t st) {
     constexpr size_t fixed = (sizeof(Shared) + 15) / 16 * 16, most = 200 * 1024;
     constexpr size_t pad = 2 * 16 / sizeof(T);  // a segment's phase, and its last vector's end
     cudaError_t e = once_per_device(done, [&] {
-        return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
+        const cudaError_t x = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
+        return x != cudaSuccess ? x : cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     });
     if (e != cudaSuccess) return e;
-    // one CTA per 4096 tokens, up to eight; fewer where the rows fill the GPU (two CTAs an SM) without
+    // one CTA per 4096 tokens, up to 16 while the rows leave SMs idle, else up to 8 (one row of 151936
+    // f32: 31 us with 8, 25 us with 16); fewer where the rows fill the GPU (two CTAs an SM) without
     // them and two such segments still fit an SM
     int ranks = 1;
-    while (ranks < kMaxCluster && (size_t)ranks * 4096 < a.n) ranks *= 2;
+    const int widest = M * kMaxCluster <= (size_t)num_sms ? kMaxCluster : 8;
+    while (ranks < widest && (size_t)ranks * 4096 < a.n) ranks *= 2;
     while (ranks > 1 && M * ranks > (size_t)num_sms * 2 && (a.n / (ranks / 2)) * sizeof(T) + fixed < 112 * 1024) ranks /= 2;
-    const size_t per = (a.n + ranks - 1) / ranks, room = (most - fixed) / sizeof(T) - pad;
-    a.cap = (unsigned)std::min(per, room);
-    const size_t bytes = fixed + (a.cap + pad) * sizeof(T);
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(ranks, (unsigned)M);
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = bytes;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = ranks;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kern, a);
+    for (;; ranks = 8) {
+        const size_t per = (a.n + ranks - 1) / ranks, room = (most - fixed) / sizeof(T) - pad;
+        a.cap = (unsigned)std::min(per, room);
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(ranks, (unsigned)M);
+        cfg.blockDim = dim3(kThreads);
+        cfg.dynamicSmemBytes = fixed + (a.cap + pad) * sizeof(T);
+        cfg.stream = st;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = ranks;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        if (ranks > 8) {  // not every device places 16 CTAs side by side
+            int clusters = 0;
+            e = cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg);
+            if (e != cudaSuccess || clusters < 1) {
+                cudaGetLastError();
+                continue;
+            }
+        }
+        return cudaLaunchKernelEx(&cfg, kern, a);
+    }
 }
 
 }  // namespace
