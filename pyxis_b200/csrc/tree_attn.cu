@@ -53,6 +53,54 @@ PYXIS_DEVINL float2 ld2(const __nv_bfloat16 *p) {
 }
 PYXIS_DEVINL float to_f32(float x) { return x; }
 PYXIS_DEVINL float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+// Byte offset in the cache of the key at a position of the sequence; -1 past its last.
+PYXIS_DEVINL long long key_offset(const TreeParams &p, const SeqShape &sh, int seq, int kvh, long long pos) {
+    if (pos >= sh.total) return -1;
+    const long long page_i = pos / p.page_size;
+    const int page = min(max(p.block_table[seq * p.table_stride + page_i], 0), p.num_pages - 1);
+    return page * p.page_stride + (pos - page_i * p.page_size) * p.slot_stride + kvh * p.head_stride;
+}
+
+// A block's rows into a warp's buffer: every lane with an offset copies its own.
+template <uint32_t BYTES, int PITCH>
+PYXIS_DEVINL void load_rows(const char *base, void *dst, uint64_t *bar, long long off, int lane) {
+    const unsigned valid = __ballot_sync(0xffffffffu, off >= 0);
+    if (lane == 0) tc::mbar_arrive_expect_tx(bar, __popc(valid) * BYTES);
+    __syncwarp();
+    if (off >= 0) tc::bulk_load(reinterpret_cast<char *>(dst) + lane * PITCH, base + off, BYTES, bar);
+}
+
+// Joins the warps' outputs (f32 [RT][HD] at the start of each warp's part of shared memory) by their
+// maxima and sums, and writes the tile or its split's partial sums.
+template <typename T, int HD, int RT, int WARPS>
+PYXIS_DEVINL void join_warps(const TreeParams &p, const SeqShape &sh, const unsigned char *parts, int part_bytes,
+                             const float *sml, int rows, int r0, int kvh, int split) {
+    const int n_out = min(rows, RT) * HD;
+    for (int i = threadIdx.x; i < n_out; i += WARPS * 32) {
+        const int r = i / HD, d = i % HD;
+        float m = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) m = fmaxf(m, sml[(w * RT + r) * 2]);
+        const float base = m == -INFINITY ? 0.f : m;
+        float o = 0.f, l = 0.f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            const float f = exp2f(sml[(w * RT + r) * 2] - base);
+            o = fmaf(f, reinterpret_cast<const float *>(parts + w * part_bytes)[r * HD + d], o);
+            l = fmaf(f, sml[(w * RT + r) * 2 + 1], l);
+        }
+        const int t = (r0 + r) / p.group, head = kvh * p.group + (r0 + r) % p.group;
+        const long long row = sh.row0 + t;
+        if (p.splits == 1) {
+            store(reinterpret_cast<T *>(p.out + row * p.out_row + head * p.out_head) + d, l == 0.f ? 0.f : o / l);
+        } else {
+            const long long at = (row * p.n_q + head) * p.splits + split;
+            p.part_o[at * HD + d] = o;
+            if (d == 0) p.part_ml[at * 2] = m, p.part_ml[at * 2 + 1] = l;
+        }
+    }
+}
+
 template <typename T, int HD, int RT>
 struct TreeCfg {
     static constexpr int kPitch = HD * (int)sizeof(T) + 16;          // bytes of a K or V row in shared memory
@@ -119,19 +167,9 @@ __global__ void __launch_bounds__(TreeCfg<T, HD, RT>::kWarps * 32) tree_attentio
     }
     __syncthreads();
 
-    // row of key `lane` of block b in the cache (bytes), for the bulk copies
-    auto row_offset = [&](long long b) -> long long {
-        const long long pos = b * kBlock + lane, page_i = pos / p.page_size;
-        if (pos >= sh.total) return -1;
-        const int page = min(max(p.block_table[seq * p.table_stride + page_i], 0), p.num_pages - 1);
-        return page * p.page_stride + (pos - page_i * p.page_size) * p.slot_stride + kvh * p.head_stride;
-    };
+    auto row_offset = [&](long long b) -> long long { return key_offset(p, sh, seq, kvh, b * kBlock + lane); };
     auto load = [&](const char *base, T *dst, uint64_t *bar, long long off) {
-        constexpr uint32_t bytes = HD * sizeof(T);
-        const unsigned valid = __ballot_sync(0xffffffffu, off >= 0);
-        if (lane == 0) tc::mbar_arrive_expect_tx(bar, __popc(valid) * bytes);
-        __syncwarp();
-        if (off >= 0) tc::bulk_load(reinterpret_cast<char *>(dst) + lane * C::kPitch, base + off, bytes, bar);
+        load_rows<HD * sizeof(T), C::kPitch>(base, dst, bar, off, lane);
     };
 
     float2 acc[RT][kCols / 2];
@@ -278,30 +316,374 @@ __global__ void __launch_bounds__(TreeCfg<T, HD, RT>::kWarps * 32) tree_attentio
             *reinterpret_cast<float2 *>(so + r * HD + lane * kCols + 2 * c) = acc[r][c];
     if (lane < RT) sml[(warp * RT + lane) * 2] = m_run, sml[(warp * RT + lane) * 2 + 1] = l_run;
     __syncthreads();
-    const int n_out = min(rows, RT) * HD;
-    for (int i = threadIdx.x; i < n_out; i += kWarps * 32) {
-        const int r = i / HD, d = i % HD;
-        float m = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) m = fmaxf(m, sml[(w * RT + r) * 2]);
-        const float base = m == -INFINITY ? 0.f : m;
-        float o = 0.f, l = 0.f;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            const float f = exp2f(sml[(w * RT + r) * 2] - base);
-            o = fmaf(f, reinterpret_cast<const float *>(smem + w * C::kWarpBytes)[r * HD + d], o);
-            l = fmaf(f, sml[(w * RT + r) * 2 + 1], l);
-        }
-        const int t = (r0 + r) / p.group, head = kvh * p.group + (r0 + r) % p.group;
-        const long long row = sh.row0 + t;
-        if (p.splits == 1) {
-            store(reinterpret_cast<T *>(p.out + row * p.out_row + head * p.out_head) + d, l == 0.f ? 0.f : o / l);
-        } else {
-            const long long at = (row * p.n_q + head) * p.splits + split;
-            p.part_o[at * HD + d] = o;
-            if (d == 0) p.part_ml[at * 2] = m, p.part_ml[at * 2 + 1] = l;
-        }
+    join_warps<T, HD, RT, kWarps>(p, sh, smem, C::kWarpBytes, sml, rows, r0, kvh, split);
+}
+
+// The same with the products on the tensor cores (mma.sync m16n8k8, tf32), for more rows than the
+// CUDA cores' FMAs keep up with: a warp's 16-key block against MT tiles of 16 rows.  f32 operands are
+// split into two tf32 terms and multiplied as lo.hi + hi.lo + hi.hi, which leaves 2^-22 of a product;
+// bf16 operands are tf32 numbers already, only the probabilities are split.
+// A fragment's k index may name the dims (keys) in any order that both operands share: lane c of a
+// quad takes dims 4c .. 4c + 3 of 16 with one 16-byte read, keys 2c and 2c + 1 of 8 (the columns of S
+// that it holds), and an output tile's columns are every fourth dim, so V is read 16 bytes at a time
+// and P never leaves its registers.
+PYXIS_DEVINL uint32_t tf32(float x) {
+    uint32_t r;
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
+    return r;
+}
+struct Split {
+    uint32_t hi, lo;
+};
+template <bool TWO>
+PYXIS_DEVINL Split split(float x) {
+    if constexpr (!TWO) return Split{__float_as_uint(x), 0u};
+    const uint32_t h = tf32(x);
+    return Split{h, __float_as_uint(x - __uint_as_float(h))};  // the multiplier drops the bits past tf32's
+}
+PYXIS_DEVINL void mma_tf32(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+constexpr int kMmaKeys = 16;  // keys of a warp's block here: small buffers, so that more warps fit an SM
+
+template <typename T, int HD, int MT>
+struct MmaCfg {
+    static constexpr bool kTwo = sizeof(T) == 4;                     // operands of two tf32 terms
+    static constexpr int kRows = 16 * MT, kQPitch = HD + 4;          // floats of a query row in shared memory
+    static constexpr int kPitch = HD * (int)sizeof(T) + 16, kHalf = kMmaKeys * kPitch;
+    static constexpr int kQBytes = (kTwo ? 2 : 1) * kRows * kQPitch * 4 + kRows * 8 + 16;
+    static constexpr int kWarpBytes = 2 * kHalf > kRows * HD * 4 ? 2 * kHalf : kRows * HD * 4;  // K, V; then the output
+    static constexpr int kPerWarp = kWarpBytes + kRows * 8 + 16;
+    static constexpr int kFit = (232448 - kQBytes) / kPerWarp;
+    static constexpr int kMost = MT == 1 ? 12 : 8;  // 168 or 255 registers a thread
+    static constexpr int kWarps = kFit < kMost ? kFit : kMost;
+    static constexpr int kBytes = kQBytes + kWarps * kPerWarp;
+};
+
+template <typename T, int HD, int MT>
+__global__ void __launch_bounds__(MmaCfg<T, HD, MT>::kWarps * 32) tree_attention_mma_kernel(const TreeParams p) {
+    using C = MmaCfg<T, HD, MT>;
+    constexpr int kWarps = C::kWarps, RT = C::kRows;
+    constexpr bool kTwo = C::kTwo;
+    constexpr int kTiles = kMmaKeys / 8;
+    extern __shared__ __align__(128) unsigned char smem[];
+    float *sq = reinterpret_cast<float *>(smem + kWarps * C::kWarpBytes);  // [hi, lo][RT][kQPitch], times scale2
+    unsigned long long *smask = reinterpret_cast<unsigned long long *>(sq + (kTwo ? 2 : 1) * RT * C::kQPitch);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smask + RT);
+    float *sml = reinterpret_cast<float *>(bars + 2 * kWarps);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(sml + kWarps * RT * 2);
+
+    pdl_wait();
+    pdl_trigger();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    const int split_i = blockIdx.x, kvh = blockIdx.y / p.row_tiles, r0 = (blockIdx.y % p.row_tiles) * RT, seq = blockIdx.z;
+    const SeqShape sh = seq_shape(p, seq);
+    const int rows = sh.nodes * p.group - r0;
+    if (rows <= 0) return;
+    const long long blocks = (sh.total + kMmaKeys - 1) / kMmaKeys;
+    const long long b0 = blocks * split_i / p.splits, b1 = blocks * (split_i + 1) / p.splits;
+
+    unsigned char *mine = smem + warp * C::kWarpBytes;
+    T *sk = reinterpret_cast<T *>(mine), *sv = reinterpret_cast<T *>(mine + C::kHalf);
+    uint64_t *kbar = bars + 2 * warp, *vbar = kbar + 1;
+    if (lane == 0) {
+        tc::mbar_init(kbar, 1);
+        tc::mbar_init(vbar, 1);
+        tc::fence_mbar_init();
     }
+    if (threadIdx.x == 0) *abort_flag = 0;
+    for (int i = threadIdx.x; i < RT * HD; i += kWarps * 32) {
+        const int r = i / HD, d = i % HD;
+        float x = 0.f;
+        if (r < rows) {
+            const int t = (r0 + r) / p.group, gg = (r0 + r) % p.group;
+            x = to_f32(*reinterpret_cast<const T *>(p.q + (sh.row0 + t) * p.q_row + (kvh * p.group + gg) * p.q_head + d * sizeof(T)));
+        }
+        // f32: times the scale, in two terms; bf16: as it is (the scale follows in f32)
+        const Split s = split<kTwo>(kTwo ? x * p.scale2 : x);
+        sq[r * C::kQPitch + d] = __uint_as_float(s.hi);
+        if (kTwo) sq[(RT + r) * C::kQPitch + d] = __uint_as_float(s.lo);
+    }
+    if (threadIdx.x < RT) {
+        unsigned long long m = 0;
+        if ((int)threadIdx.x < rows) {
+            const int t = (r0 + threadIdx.x) / p.group;
+            m = p.tree_mask ? p.tree_mask[sh.row0 + t] : (2ull << t) - 1;
+        }
+        smask[threadIdx.x] = m;
+    }
+    __syncthreads();
+
+    auto row_offset = [&](long long b) -> long long { return lane < kMmaKeys ? key_offset(p, sh, seq, kvh, b * kMmaKeys + lane) : -1; };
+    auto load = [&](const char *base, T *dst, uint64_t *bar, long long off) {
+        load_rows<HD * sizeof(T), C::kPitch>(base, dst, bar, off, lane);
+    };
+    float acc[MT][HD / 8][4];  // tile 4 j + e, column n: dim 32 j + 4 n + e
+    float m_run[MT][2], l_run[MT][2];  // rows g and g + 8 of each tile; l: this lane's keys only
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+        for (int i = 0; i < HD / 8; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) acc[mt][i][k] = 0.f;
+        m_run[mt][0] = m_run[mt][1] = -INFINITY;
+        l_run[mt][0] = l_run[mt][1] = 0.f;
+    }
+    bool ok = true;
+    uint32_t phase = 0;
+    long long b = b0 + warp;
+    long long off = b < b1 ? row_offset(b) : -1;
+    if (b < b1) {
+        load(p.k, sk, kbar, off);
+        load(p.v, sv, vbar, off);
+    }
+    for (; b < b1 && ok; b += kWarps, phase ^= 1) {
+        const long long next_off = b + kWarps < b1 ? row_offset(b + kWarps) : -1;
+        ok = __all_sync(0xffffffffu, tc::mbar_wait_bounded(kbar, phase, abort_flag, p.err, kErrLoad, kTimeoutNs));
+        if (!ok) break;
+        // ---- S: columns nt * 8 + 2 c, + 1 of rows g, g + 8
+        float s[MT][kTiles][4];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int nt = 0; nt < kTiles; ++nt)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) s[mt][nt][k] = 0.f;
+#pragma unroll 2
+        for (int d = 4 * c; d < HD; d += 16) {
+            Split kf[kTiles][4];
+#pragma unroll
+            for (int nt = 0; nt < kTiles; ++nt) {
+                const float4 x = ld4(reinterpret_cast<const T *>(reinterpret_cast<const char *>(sk) + (nt * 8 + g) * C::kPitch) + d);
+                kf[nt][0] = split<kTwo>(x.x), kf[nt][1] = split<kTwo>(x.y), kf[nt][2] = split<kTwo>(x.z), kf[nt][3] = split<kTwo>(x.w);
+            }
+            // products of one kind for all tiles before the next kind: no MMA waits for the one before
+            uint4 h0[MT], h1[MT];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                const float *q0 = sq + (mt * 16 + g) * C::kQPitch + d;
+                h0[mt] = *reinterpret_cast<const uint4 *>(q0);
+                h1[mt] = *reinterpret_cast<const uint4 *>(q0 + 8 * C::kQPitch);
+            }
+            if constexpr (kTwo) {
+                uint4 l0[MT], l1[MT];
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    const float *q0 = sq + (RT + mt * 16 + g) * C::kQPitch + d;
+                    l0[mt] = *reinterpret_cast<const uint4 *>(q0);
+                    l1[mt] = *reinterpret_cast<const uint4 *>(q0 + 8 * C::kQPitch);
+                }
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int nt = 0; nt < kTiles; ++nt)
+                        mma_tf32(s[mt][nt], l0[mt].x, l1[mt].x, l0[mt].y, l1[mt].y, kf[nt][0].hi, kf[nt][1].hi);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int nt = 0; nt < kTiles; ++nt)
+                        mma_tf32(s[mt][nt], l0[mt].z, l1[mt].z, l0[mt].w, l1[mt].w, kf[nt][2].hi, kf[nt][3].hi);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int nt = 0; nt < kTiles; ++nt)
+                        mma_tf32(s[mt][nt], h0[mt].x, h1[mt].x, h0[mt].y, h1[mt].y, kf[nt][0].lo, kf[nt][1].lo);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int nt = 0; nt < kTiles; ++nt)
+                        mma_tf32(s[mt][nt], h0[mt].z, h1[mt].z, h0[mt].w, h1[mt].w, kf[nt][2].lo, kf[nt][3].lo);
+            }
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int nt = 0; nt < kTiles; ++nt)
+                    mma_tf32(s[mt][nt], h0[mt].x, h1[mt].x, h0[mt].y, h1[mt].y, kf[nt][0].hi, kf[nt][1].hi);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int nt = 0; nt < kTiles; ++nt)
+                    mma_tf32(s[mt][nt], h0[mt].z, h1[mt].z, h0[mt].w, h1[mt].w, kf[nt][2].hi, kf[nt][3].hi);
+        }
+        __syncwarp();
+        if (b + kWarps < b1) load(p.k, sk, kbar, next_off);
+        const bool tail = (b + 1) * kMmaKeys > sh.ctx;  // holds drafts or ends inside
+        if (!kTwo) {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int nt = 0; nt < kTiles; ++nt)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) s[mt][nt][k] *= p.scale2;
+        }
+        if (tail) {
+            const long long d0 = b * kMmaKeys - sh.ctx;  // draft of column 0
+            const int avail = (int)(sh.total - sh.ctx);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const unsigned long long m = smask[mt * 16 + g + 8 * h];
+#pragma unroll
+                    for (int nt = 0; nt < kTiles; ++nt)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const long long d = d0 + nt * 8 + 2 * c + i;
+                            if (d >= 0 && (d >= avail || !((m >> d) & 1))) s[mt][nt][2 * h + i] = -INFINITY;
+                        }
+                }
+        }
+        // ---- running maximum, probabilities
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float top = fmaxf(s[mt][0][2 * h], s[mt][0][2 * h + 1]);
+#pragma unroll
+                for (int nt = 1; nt < kTiles; ++nt) top = fmaxf(top, fmaxf(s[mt][nt][2 * h], s[mt][nt][2 * h + 1]));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const float m_new = fmaxf(m_run[mt][h], top), base = m_new == -INFINITY ? 0.f : m_new;
+                if (__any_sync(0xffffffffu, m_new > m_run[mt][h])) {
+                    const float alpha = exp2f(m_run[mt][h] - base);
+                    l_run[mt][h] *= alpha;
+#pragma unroll
+                    for (int i = 0; i < HD / 8; ++i) acc[mt][i][2 * h] *= alpha, acc[mt][i][2 * h + 1] *= alpha;
+                }
+                m_run[mt][h] = m_new;
+#pragma unroll
+                for (int nt = 0; nt < kTiles; ++nt)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float x = exp2f(s[mt][nt][2 * h + i] - base);
+                        s[mt][nt][2 * h + i] = x;
+                        l_run[mt][h] += x;
+                    }
+            }
+        ok = __all_sync(0xffffffffu, tc::mbar_wait_bounded(vbar, phase, abort_flag, p.err, kErrLoad, kTimeoutNs));
+        if (!ok) break;
+        // ---- O += P V
+        if (tail) {
+            // every value has to be fit to be multiplied by a weight of zero
+            const int nk = (int)min((long long)kMmaKeys, sh.total - b * kMmaKeys);
+            char *row = reinterpret_cast<char *>(sv) + lane * C::kPitch;
+            bool finite = true;
+            for (int i = 0; lane < kMmaKeys && i < HD * (int)sizeof(T) / 16; ++i) {
+                uint4 *x = reinterpret_cast<uint4 *>(row) + i;
+                if (lane >= nk) {
+                    *x = make_uint4(0, 0, 0, 0);  // never loaded
+                } else {
+                    const float4 lo = ld4(reinterpret_cast<const T *>(x));
+                    finite = finite && isfinite(lo.x) && isfinite(lo.y) && isfinite(lo.z) && isfinite(lo.w);
+                    if constexpr (sizeof(T) == 2) {
+                        const float4 hi = ld4(reinterpret_cast<const T *>(x) + 4);
+                        finite = finite && isfinite(hi.x) && isfinite(hi.y) && isfinite(hi.z) && isfinite(hi.w);
+                    }
+                }
+            }
+            __syncwarp();
+            unsigned odd = __ballot_sync(0xffffffffu, !finite);
+            if (odd) {
+                // a value that is not finite reaches the rows that see it, and no others: those get it
+                // here, then it becomes zero
+                for (unsigned rest = odd; rest; rest &= rest - 1) {
+                    const int k = __ffs(rest) - 1;
+                    const T *vrow = reinterpret_cast<const T *>(reinterpret_cast<const char *>(sv) + k * C::kPitch);
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            // key k's weight: by masks, as an index would move s out of the registers
+                            uint32_t bits = 0;
+#pragma unroll
+                            for (int i = 0; i < 2 * kTiles; ++i)
+                                bits |= __float_as_uint(s[mt][i >> 1][2 * h + (i & 1)]) &
+                                        (((k >> 3) * 2 + (k & 1)) == i ? 0xffffffffu : 0u);
+                            const float w = __uint_as_float(__shfl_sync(0xffffffffu, bits, (lane & ~3) | ((k >> 1) & 3)));
+#pragma unroll
+                            for (int i = 0; i < HD / 8; ++i)
+#pragma unroll
+                                for (int n = 0; n < 2; ++n) {
+                                    const float x = to_f32(vrow[32 * (i >> 2) + 4 * (2 * c + n) + (i & 3)]);
+                                    if (w != 0.f && !isfinite(x)) acc[mt][i][2 * h + n] += x;
+                                }
+                        }
+                }
+                __syncwarp();
+                if (!finite)
+                    for (int i = 0; i < HD; ++i)
+                        if (!isfinite(to_f32(reinterpret_cast<const T *>(row)[i]))) store(reinterpret_cast<T *>(row) + i, 0.f);
+                __syncwarp();
+            }
+        }
+#pragma unroll
+        for (int nt = 0; nt < kTiles; ++nt) {
+            Split a[MT][4];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                a[mt][0] = split<true>(s[mt][nt][0]), a[mt][1] = split<true>(s[mt][nt][2]);
+                a[mt][2] = split<true>(s[mt][nt][1]), a[mt][3] = split<true>(s[mt][nt][3]);
+            }
+            const char *v0 = reinterpret_cast<const char *>(sv) + (nt * 8 + 2 * c) * C::kPitch;
+#pragma unroll
+            for (int j = 0; j < HD / 32; ++j) {
+                const float4 x = ld4(reinterpret_cast<const T *>(v0) + 32 * j + 4 * g);
+                const float4 y = ld4(reinterpret_cast<const T *>(v0 + C::kPitch) + 32 * j + 4 * g);
+                const float xe[4] = {x.x, x.y, x.z, x.w}, ye[4] = {y.x, y.y, y.z, y.w};
+                Split u[4], v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) u[e] = split<kTwo>(xe[e]), v[e] = split<kTwo>(ye[e]);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        mma_tf32(acc[mt][4 * j + e], a[mt][0].lo, a[mt][1].lo, a[mt][2].lo, a[mt][3].lo, u[e].hi, v[e].hi);
+                if constexpr (kTwo) {
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            mma_tf32(acc[mt][4 * j + e], a[mt][0].hi, a[mt][1].hi, a[mt][2].hi, a[mt][3].hi, u[e].lo, v[e].lo);
+                }
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        mma_tf32(acc[mt][4 * j + e], a[mt][0].hi, a[mt][1].hi, a[mt][2].hi, a[mt][3].hi, u[e].hi, v[e].hi);
+            }
+        }
+        __syncwarp();
+        if (b + kWarps < b1) load(p.v, sv, vbar, next_off);
+    }
+    if (!ok) {  // a copy did not land in time: give those in flight a last chance before the buffers go
+        volatile int never = 0;
+        tc::mbar_wait_bounded(kbar, phase, &never, p.err, kErrDrain, 100000000ull);
+        tc::mbar_wait_bounded(vbar, phase, &never, p.err, kErrDrain, 100000000ull);
+    }
+
+    // ---- join the warps: their outputs go where their K and V were
+    __syncwarp();
+    float *so = reinterpret_cast<float *>(mine);
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int r = mt * 16 + g + 8 * h;
+#pragma unroll
+            for (int i = 0; i < HD / 8; ++i)
+#pragma unroll
+                for (int n = 0; n < 2; ++n) so[r * HD + 32 * (i >> 2) + 4 * (2 * c + n) + (i & 3)] = acc[mt][i][2 * h + n];
+            float l = l_run[mt][h];
+            l += __shfl_xor_sync(0xffffffffu, l, 1);
+            l += __shfl_xor_sync(0xffffffffu, l, 2);
+            if (c == 0) sml[(warp * RT + r) * 2] = m_run[mt][h], sml[(warp * RT + r) * 2 + 1] = l;
+        }
+    __syncthreads();
+    join_warps<T, HD, RT, kWarps>(p, sh, smem, C::kWarpBytes, sml, rows, r0, kvh, split_i);
 }
 
 // Joins the splits: a warp per (node, query head).
@@ -333,34 +715,45 @@ __global__ void __launch_bounds__(256) tree_join_kernel(const TreeParams p) {
     for (int c = 0; c < kCols; ++c) store(dst + c, l == 0.f ? 0.f : o[c] / l);
 }
 
-template <typename T, int HD, int RT>
-cudaError_t run_tile(const TreeParams &p, size_t n_seq, cudaStream_t st) {
-    using C = TreeCfg<T, HD, RT>;
-    auto kern = tree_attention_kernel<T, HD, RT>;
-    static std::atomic<uint64_t> done{0};
-    cudaError_t e = once_per_device(
-        done, [&] { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kBytes); });
+template <typename T, int HD>
+cudaError_t run_kernel(void (*kern)(TreeParams), int threads, int smem, std::atomic<uint64_t> &done, const TreeParams &p,
+                       size_t n_seq, cudaStream_t st) {
+    cudaError_t e =
+        once_per_device(done, [&] { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
     if (e != cudaSuccess) return e;
+    PdlScope pdl;
     for (size_t s = 0; s < n_seq; s += 65535) {  // grid.z
         TreeParams q = p;
         q.q_start += s, q.context_len += s, q.block_table += s * p.table_stride;
         const unsigned m = (unsigned)std::min<size_t>(n_seq - s, 65535);
-        e = launch_kernel(kern, dim3(p.splits, p.n_kv * p.row_tiles, m), dim3(C::kWarps * 32), C::kBytes, st, q);
+        e = launch_kernel(kern, dim3(p.splits, p.n_kv * p.row_tiles, m), dim3(threads), smem, st, q);
         if (e == cudaSuccess && p.splits > 1)
             e = launch_kernel(tree_join_kernel<T, HD>, dim3((p.max_tree * p.n_q + 7) / 8, m), dim3(256), 0, st, q);
         if (e != cudaSuccess) return e;
     }
     return cudaSuccess;
 }
+template <typename T, int HD, int RT>
+cudaError_t run_fma(const TreeParams &p, size_t n_seq, cudaStream_t st) {
+    using C = TreeCfg<T, HD, RT>;
+    static std::atomic<uint64_t> done{0};
+    return run_kernel<T, HD>(tree_attention_kernel<T, HD, RT>, C::kWarps * 32, C::kBytes, done, p, n_seq, st);
+}
+template <typename T, int HD, int MT>
+cudaError_t run_mma(const TreeParams &p, size_t n_seq, cudaStream_t st) {
+    using C = MmaCfg<T, HD, MT>;
+    static std::atomic<uint64_t> done{0};
+    return run_kernel<T, HD>(tree_attention_mma_kernel<T, HD, MT>, C::kWarps * 32, C::kBytes, done, p, n_seq, st);
+}
 
 template <typename T, int HD>
 cudaError_t run_tree(const TreeParams &p, int row_tile, size_t n_seq, cudaStream_t st) {
     switch (row_tile) {
-    case 2: return run_tile<T, HD, 2>(p, n_seq, st);
-    case 4: return run_tile<T, HD, 4>(p, n_seq, st);
-    case 8: return run_tile<T, HD, 8>(p, n_seq, st);
-    case 16: return run_tile<T, HD, 16>(p, n_seq, st);
-    default: return run_tile<T, HD, 32>(p, n_seq, st);
+    case 2: return run_fma<T, HD, 2>(p, n_seq, st);
+    case 4: return run_fma<T, HD, 4>(p, n_seq, st);
+    case 8: return run_fma<T, HD, 8>(p, n_seq, st);
+    case 16: return run_mma<T, HD, 1>(p, n_seq, st);
+    default: return run_mma<T, HD, 2>(p, n_seq, st);
     }
 }
 
