@@ -51,13 +51,26 @@ PYXIS_DEVINL float2 ld2(const __nv_bfloat16 *p) {
     const uint32_t u = *reinterpret_cast<const uint32_t *>(p);
     return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u));
 }
+// 16 bytes of T hold no infinity and no NaN.
+template <typename T>
+PYXIS_DEVINL bool all_finite(uint4 x) {
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    bool ok = true;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        ok = ok && (w[i] & 0x7F800000u) != 0x7F800000u;
+        if (sizeof(T) == 2) ok = ok && (w[i] & 0x7F80u) != 0x7F80u;
+    }
+    return ok;
+}
 PYXIS_DEVINL float to_f32(float x) { return x; }
 PYXIS_DEVINL float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
 // Byte offset in the cache of the key at a position of the sequence; -1 past its last.
 PYXIS_DEVINL long long key_offset(const TreeParams &p, const SeqShape &sh, int seq, int kvh, long long pos) {
     if (pos >= sh.total) return -1;
-    const long long page_i = pos / p.page_size;
-    const int page = min(max(p.block_table[seq * p.table_stride + page_i], 0), p.num_pages - 1);
+    // (a 32-bit division where the tables reach no further)
+    const long long page_i = p.capacity >> 31 ? pos / p.page_size : (long long)((unsigned)pos / (unsigned)p.page_size);
+    const int page = min(max(__ldg(p.block_table + seq * p.table_stride + page_i), 0), p.num_pages - 1);
     return page * p.page_stride + (pos - page_i * p.page_size) * p.slot_stride + kvh * p.head_stride;
 }
 
@@ -252,7 +265,25 @@ __global__ void __launch_bounds__(TreeCfg<T, HD, RT>::kWarps * 32) tree_attentio
         if (!ok) break;
         // ---- O += P V: this lane's columns
         const int nk = tail ? (int)min((long long)kBlock, sh.total - b * kBlock) : kBlock;
-        if (!tail) {
+        // Whether every value is fit to be multiplied by a weight of zero.  Few rows go key by key
+        // without looking: the look at 32 rows of values costs more (one token over 152 f32 positions: 12 us
+        // with it, 8 without).
+        bool plain = !tail;
+        if (RT > 4 && tail) {
+            char *row = reinterpret_cast<char *>(sv) + lane * C::kPitch;
+            bool finite = true;
+#pragma unroll 8
+            for (int i = 0; i < HD * (int)sizeof(T) / 16; ++i) {
+                uint4 *x = reinterpret_cast<uint4 *>(row) + i;
+                if (lane >= nk)
+                    *x = make_uint4(0, 0, 0, 0);  // never loaded
+                else
+                    finite = finite && all_finite<T>(*x);
+            }
+            plain = __all_sync(0xffffffffu, finite);
+            __syncwarp();
+        }
+        if (plain) {
 #pragma unroll 2
             for (int j = 0; j < kBlock; j += 4) {
                 float2 v[4][kCols / 2];
@@ -280,8 +311,8 @@ __global__ void __launch_bounds__(TreeCfg<T, HD, RT>::kWarps * 32) tree_attentio
                 }
             }
         } else {
-            // a value that a row does not attend to (p = 0) may be anything: it is left out, not
-            // multiplied by zero; so are the rows past the last key, which were never loaded
+            // a value that is not finite reaches the rows that see it, and no others: key by key, a weight
+            // of zero leaves the value out (the other rows' sums are those of the loop above, bit for bit)
             for (int j = 0; j < nk; ++j) {
                 const T *vrow = reinterpret_cast<const T *>(reinterpret_cast<const char *>(sv) + j * C::kPitch) + lane * kCols;
                 float2 v[kCols / 2];
@@ -327,19 +358,16 @@ __global__ void __launch_bounds__(TreeCfg<T, HD, RT>::kWarps * 32) tree_attentio
 // quad takes dims 4c .. 4c + 3 of 16 with one 16-byte read, keys 2c and 2c + 1 of 8 (the columns of S
 // that it holds), and an output tile's columns are every fourth dim, so V is read 16 bytes at a time
 // and P never leaves its registers.
-PYXIS_DEVINL uint32_t tf32(float x) {
-    uint32_t r;
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
-    return r;
-}
 struct Split {
     uint32_t hi, lo;
 };
 template <bool TWO>
 PYXIS_DEVINL Split split(float x) {
     if constexpr (!TWO) return Split{__float_as_uint(x), 0u};
-    const uint32_t h = tf32(x);
-    return Split{h, __float_as_uint(x - __uint_as_float(h))};  // the multiplier drops the bits past tf32's
+    // tf32 is the upper 19 bits, and the multiplier drops the rest: hi is x cut off (no overflow), lo
+    // the remainder rounded (half a step added before its cut), off by 2^-23 of x
+    const uint32_t h = __float_as_uint(x) & 0xffffe000u;
+    return Split{h, __float_as_uint(x - __uint_as_float(h)) + 0x1000u};
 }
 PYXIS_DEVINL void mma_tf32(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -547,14 +575,17 @@ __global__ void __launch_bounds__(MmaCfg<T, HD, MT>::kWarps * 32) tree_attention
                 for (int nt = 1; nt < kTiles; ++nt) top = fmaxf(top, fmaxf(s[mt][nt][2 * h], s[mt][nt][2 * h + 1]));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const float m_new = fmaxf(m_run[mt][h], top), base = m_new == -INFINITY ? 0.f : m_new;
-                if (__any_sync(0xffffffffu, m_new > m_run[mt][h])) {
-                    const float alpha = exp2f(m_run[mt][h] - base);
+                // the reference is raised only by more than 2^8: the weights stay below that, and their
+                // f32 precision is the same
+                const bool raise = top > m_run[mt][h] + 8.f || (m_run[mt][h] == -INFINITY && top > m_run[mt][h]);
+                if (__any_sync(0xffffffffu, raise)) {
+                    const float alpha = raise ? exp2f(m_run[mt][h] - top) : 1.f;
+                    if (raise) m_run[mt][h] = top;
                     l_run[mt][h] *= alpha;
 #pragma unroll
                     for (int i = 0; i < HD / 8; ++i) acc[mt][i][2 * h] *= alpha, acc[mt][i][2 * h + 1] *= alpha;
                 }
-                m_run[mt][h] = m_new;
+                const float base = m_run[mt][h] == -INFINITY ? 0.f : m_run[mt][h];
 #pragma unroll
                 for (int nt = 0; nt < kTiles; ++nt)
 #pragma unroll
@@ -572,18 +603,13 @@ __global__ void __launch_bounds__(MmaCfg<T, HD, MT>::kWarps * 32) tree_attention
             const int nk = (int)min((long long)kMmaKeys, sh.total - b * kMmaKeys);
             char *row = reinterpret_cast<char *>(sv) + lane * C::kPitch;
             bool finite = true;
-            for (int i = 0; lane < kMmaKeys && i < HD * (int)sizeof(T) / 16; ++i) {
+#pragma unroll 8
+            for (int i = 0; i < (lane < kMmaKeys ? HD * (int)sizeof(T) / 16 : 0); ++i) {
                 uint4 *x = reinterpret_cast<uint4 *>(row) + i;
-                if (lane >= nk) {
+                if (lane >= nk)
                     *x = make_uint4(0, 0, 0, 0);  // never loaded
-                } else {
-                    const float4 lo = ld4(reinterpret_cast<const T *>(x));
-                    finite = finite && isfinite(lo.x) && isfinite(lo.y) && isfinite(lo.z) && isfinite(lo.w);
-                    if constexpr (sizeof(T) == 2) {
-                        const float4 hi = ld4(reinterpret_cast<const T *>(x) + 4);
-                        finite = finite && isfinite(hi.x) && isfinite(hi.y) && isfinite(hi.z) && isfinite(hi.w);
-                    }
-                }
+                else
+                    finite = finite && all_finite<T>(*x);
             }
             __syncwarp();
             unsigned odd = __ballot_sync(0xffffffffu, !finite);
@@ -761,15 +787,20 @@ cudaError_t run_tree(const TreeParams &p, int row_tile, size_t n_seq, cudaStream
 
 TreePlan plan_tree_attention(const pyxis_tree_attention_args &a, const pyxis_kv_pages &kv, int num_sms) {
     TreePlan t;
-    t.tensor = tree_attention_tc_supported(a, kv);
     const long long rows = (long long)a.max_tree * (a.n_q_heads / kv.n_kv_heads);
+    const long long keys = std::max<long long>(1, std::min<long long>(a.max_context + a.max_tree,
+                                                                     (long long)a.table_width * kv.page_size));
+    // Few rows over few keys: the CUDA cores are done before the tensor-core kernel has started its
+    // pipeline.  Measured (16 query heads, 8 kv heads of 128, bf16): 2 rows, 16 sequences of 600
+    // positions 18 us against 27, of 2303 45 against 45, 64 of 2303 162 against 113; 8 rows, 4 sequences
+    // of 600 18 against 21, of 2303 39 against 27.
+    t.tensor = tree_attention_tc_supported(a, kv) &&
+               (rows > 8 || (double)a.n_seq * kv.n_kv_heads * keys * rows * rows > 1.2e6);
     t.row_tile = 2;
     while (t.row_tile < 32 && t.row_tile < rows) t.row_tile *= 2;
     t.row_tiles = (int)((rows + t.row_tile - 1) / t.row_tile);
     // the split that wastes least of the last wave, a split costing about 64 keys of start-up
     const long long units = (long long)a.n_seq * kv.n_kv_heads * t.row_tiles;
-    const long long keys = std::max<long long>(1, std::min<long long>(a.max_context + a.max_tree,
-                                                                     (long long)a.table_width * kv.page_size));
     const long long most = std::min<long long>(256, (keys + 255) / 256);
     double best = 0;
     t.splits = 1;
