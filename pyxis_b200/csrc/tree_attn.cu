@@ -794,8 +794,10 @@ TreePlan plan_tree_attention(const pyxis_tree_attention_args &a, const pyxis_kv_
     // pipeline.  Measured (16 query heads, 8 kv heads of 128, bf16): 2 rows, 16 sequences of 600
     // positions 18 us against 27, of 2303 45 against 45, 64 of 2303 162 against 113; 8 rows, 4 sequences
     // of 600 18 against 21, of 2303 39 against 27.
-    t.tensor = tree_attention_tc_supported(a, kv) &&
-               (rows > 8 || (double)a.n_seq * kv.n_kv_heads * keys * rows * rows > 1.2e6);
+    const bool f32 = kv.dtype == PYXIS_DTYPE_F32;
+    t.tensor = f32 ? tree_attention_tc32_supported(a, kv) && rows > 8
+                   : tree_attention_tc_supported(a, kv) &&
+                         (rows > 8 || (double)a.n_seq * kv.n_kv_heads * keys * rows * rows > 1.2e6);
     t.row_tile = 2;
     while (t.row_tile < 32 && t.row_tile < rows) t.row_tile *= 2;
     t.row_tiles = (int)((rows + t.row_tile - 1) / t.row_tile);
@@ -814,7 +816,8 @@ TreePlan plan_tree_attention(const pyxis_tree_attention_args &a, const pyxis_kv_
 
 size_t tree_attention_workspace(const TreePlan &t, const pyxis_tree_attention_args &a, const pyxis_kv_pages &kv,
                                 int num_sms) {
-    if (t.tensor) return tree_attention_tc_workspace(kv, num_sms);
+    if (t.tensor)
+        return kv.dtype == PYXIS_DTYPE_F32 ? tree_attention_tc32_workspace(kv, num_sms) : tree_attention_tc_workspace(kv, num_sms);
     return t.splits == 1 ? 0 : a.n_rows * a.n_q_heads * t.splits * (size_t)(kv.head_dim + 2) * 4;
 }
 
@@ -850,7 +853,9 @@ cudaError_t launch_tree_attention(const pyxis_tree_attention_args &a, const pyxi
     p.row_tiles = t.row_tiles;
     p.scale2 = a.scale * kLog2e;
     p.err = err;
-    if (t.tensor) return launch_tree_attention_tc(p, a, kv, workspace, num_sms, st);
+    if (t.tensor)
+        return kv.dtype == PYXIS_DTYPE_F32 ? launch_tree_attention_tc32(p, a, kv, workspace, num_sms, st)
+                                           : launch_tree_attention_tc(p, a, kv, workspace, num_sms, st);
     p.part_ml = (float *)workspace;
     p.part_o = p.part_ml ? p.part_ml + a.n_rows * a.n_q_heads * t.splits * 2 : nullptr;
     if (kv.dtype == PYXIS_DTYPE_F32)

@@ -43,11 +43,15 @@ PYXIS_DEVINL SeqShape seq_shape(const TreeParams &p, int seq) {
 PYXIS_DEVINL void store(float *p, float x) { *p = x; }
 PYXIS_DEVINL void store(__nv_bfloat16 *p, float x) { *p = __float2bfloat16_rn(x); }
 
-// The tensor-core form (bf16 pages of a size that tiles 128 keys): whether it takes the call, its
-// workspace, its launch.
+// The tensor-core forms, bf16 and f32 pages of sizes that tile their blocks of keys: whether one takes
+// the call, its workspace, its launch.
 bool tree_attention_tc_supported(const pyxis_tree_attention_args &a, const pyxis_kv_pages &kv);
 size_t tree_attention_tc_workspace(const pyxis_kv_pages &kv, int num_sms);
 cudaError_t launch_tree_attention_tc(const TreeParams &p, const pyxis_tree_attention_args &a, const pyxis_kv_pages &kv,
                                      void *workspace, int num_sms, cudaStream_t st);
+bool tree_attention_tc32_supported(const pyxis_tree_attention_args &a, const pyxis_kv_pages &kv);
+size_t tree_attention_tc32_workspace(const pyxis_kv_pages &kv, int num_sms);
+cudaError_t launch_tree_attention_tc32(const TreeParams &p, const pyxis_tree_attention_args &a, const pyxis_kv_pages &kv,
+                                       void *workspace, int num_sms, cudaStream_t st);
 
 }  // namespace pyxis
