@@ -790,12 +790,16 @@ TreePlan plan_tree_attention(const pyxis_tree_attention_args &a, const pyxis_kv_
     const long long rows = (long long)a.max_tree * (a.n_q_heads / kv.n_kv_heads);
     const long long keys = std::max<long long>(1, std::min<long long>(a.max_context + a.max_tree,
                                                                      (long long)a.table_width * kv.page_size));
-    // Few rows over few keys: the CUDA cores are done before the tensor-core kernel has started its
-    // pipeline.  Measured (16 query heads, 8 kv heads of 128, bf16): 2 rows, 16 sequences of 600
-    // positions 18 us against 27, of 2303 45 against 45, 64 of 2303 162 against 113; 8 rows, 4 sequences
-    // of 600 18 against 21, of 2303 39 against 27.
+    // bf16: few rows over few keys are done on the CUDA cores before the tensor-core kernel has started
+    // its pipeline.  Measured (16 query heads, 8 kv heads of 128): 2 rows, 16 sequences of 600 positions
+    // 18 us against 27, of 2303 45 against 45, 64 of 2303 162 against 113; 8 rows, 4 sequences of 600
+    // 18 against 21, of 2303 39 against 27.
+    // f32: the tcgen05 kernel pays the same for 1 row as for 128 (three products of 128 rows and the
+    // conversion of every key), the mma.sync kernel for each tile of 16.  16 sequences of 2303 positions:
+    // 16 rows 89 us against the tcgen05 kernel's 113, 32 rows 160 against 115, 64 rows 310 against 120;
+    // one sequence of 152: 16 rows 18 against 24, 128 rows 31 against 25.
     const bool f32 = kv.dtype == PYXIS_DTYPE_F32;
-    t.tensor = f32 ? tree_attention_tc32_supported(a, kv) && rows > 8
+    t.tensor = f32 ? tree_attention_tc32_supported(a, kv) && rows > 16
                    : tree_attention_tc_supported(a, kv) &&
                          (rows > 8 || (double)a.n_seq * kv.n_kv_heads * keys * rows * rows > 1.2e6);
     t.row_tile = 2;

@@ -9,16 +9,21 @@
 // tiles is taken in registers with the tiles' scales.
 //
 // 64 keys of K and V are 64 KB that take 2800 cycles to arrive at an SM; their products are 36 MMAs
-// (about 2000 cycles) for up to 128 rows, so HBM bounds it for any number of rows up to 128.
+// (about 2000 cycles) for up to 128 rows, and Q lies in TMEM, so that they read no more of shared memory
+// than K's and V's terms.  The converters bound it: 64 KB read, split and written again per tile by four
+// warps.  The scale of a tile is taken from the tile before (with room of a factor of four), which spares
+// them a pass over it for its largest magnitude: 137 -> 115 us for 16 sequences of 2303 positions and 16
+// nodes (8 kv heads of 128, a floor of 41 us at the memory's rate), 374 -> 316 us for 58 sequences of
+// 1731 positions and 64 nodes (121 us).
 //
 // One CTA per SM takes an equal share of all units' tiles (tree_attn_tc.cuh).  Warps:
 //   0       producer: a tile's pages by TMA (one box per page) into a ring of f32 tiles, in the order
 //           S_0, S_1, O_0, S_2, O_1, ... of the MMAs
 //   1       MMA issuer (and TMEM owner)
-//   4-7     converters: a tile from the ring into registers, its largest magnitude (exchanged between
-//           the warps), then its two fp16 terms into the operand's place in the 128-byte swizzle
-//   8-15    softmax: a row per thread, half of a tile's keys and of O's columns per warp.  The rows of
-//           Q are split by them at a segment's start.
+//   4-7     converters: a tile from the ring into its two fp16 terms, in the 128-byte swizzle, twice
+//           buffered; the tile's largest magnitude is found on the way and sets the next one's scale
+//   8-15    softmax: a row per thread, half of a tile's keys and of O's columns per warp.  They split
+//           their rows of Q into TMEM at a segment's start.
 #include <algorithm>
 #include <atomic>
 
@@ -35,8 +40,7 @@ constexpr int kThreads = (kSmWarp0 + kSmWarps) * 32;
 // stays below what the block is launched with, 4 x 128.
 constexpr int kRegsLaunch = 128, kRegsFew = 88, kRegsConv = 88, kRegsSoft = 160;
 static_assert(kRegsFew + kRegsConv + 2 * kRegsSoft <= 4 * kRegsLaunch - 16, "register split");
-constexpr int kSBufs = 3;
-constexpr uint32_t kTmemCols = 512, kOCol = kSBufs * kTile;  // three score buffers, two of O
+constexpr uint32_t kTmemCols = 512, kOCol = 2 * kTile, kQCol = kOCol + 2 * 128;  // S twice, O twice, Q hi and lo
 constexpr uint64_t kTimeoutNs = 2000000000ull;
 constexpr float kRaise = 11.0f;  // weights up to 2^11 stay in fp16's range
 enum { kErrProd = 0x721, kErrMma = 0x722, kErrConv = 0x723, kErrSoft = 0x724, kErrDrain = 0x725, kErrAlign = 0x726 };
@@ -44,36 +48,35 @@ enum { kErrProd = 0x721, kErrMma = 0x722, kErrConv = 0x723, kErrSoft = 0x724, kE
 template <int HD>
 struct Smem {
     static constexpr int kDB = HD / 64;                 // 64-column panels of a row of fp16
-    static constexpr uint32_t kQPanel = kRows * 128, kQTerm = kDB * kQPanel;   // hi; lo follows
-    static constexpr uint32_t kPanel = kTile * 128, kTerm = kDB * kPanel;      // of a tile of K or V
+    static constexpr uint32_t kPanel = kTile * 128, kTerm = kDB * kPanel;      // of a tile of K or V: hi; lo follows
     static constexpr uint32_t kEntry = kTile * HD * 4;  // a tile of the ring, f32
     static constexpr int kRing = HD == 128 ? 3 : 9;
-    static constexpr uint32_t q = 0;
-    static constexpr uint32_t k = q + 2 * kQTerm;
-    static constexpr uint32_t v = k + 2 * kTerm;
-    static constexpr uint32_t ring = v + 2 * kTerm;
+    static constexpr uint32_t k = 0;                    // two tiles of two terms each
+    static constexpr uint32_t v = k + 4 * kTerm;
+    static constexpr uint32_t ring = v + 4 * kTerm;
     static constexpr uint32_t bar = ring + kRing * kEntry;
-    static constexpr int kBars = 2 * kRing + 1 + 2 + 2 + 1 + 1 + 2 + 3 * kSBufs;
+    static constexpr int kBars = 2 * kRing + 1 + 4 + 4 + 1 + 1 + 2 + 3 * 2;
     static constexpr uint32_t misc = bar + (kBars * 8 + 15) / 16 * 16;
     static constexpr uint32_t wmax = misc + 64;          // [2][kConvWarps] magnitudes
     static constexpr uint32_t scale = wmax + 32;         // [2][4]: 2^-e of K and of V of the latest tiles
-    static constexpr uint32_t qinv = scale + 32;         // [128] 2^-e of Q's rows
-    static constexpr uint32_t red = qinv + kRows * 4;    // [2][2 halves][128 rows]
+    static constexpr uint32_t red = scale + 32;          // [2][2 halves][128 rows]
     static constexpr uint32_t bytes = red + 2 * 2 * kRows * 4;
 };
 static_assert(Smem<128>::bytes <= 232448 && Smem<64>::bytes <= 232448, "227 KB of shared memory per CTA");
-static_assert(kOCol + 2 * 128 <= kTmemCols, "TMEM columns");
+static_assert(kQCol + 128 <= kTmemCols, "TMEM columns");
 
 __host__ __device__ constexpr uint32_t idesc_f16(int M, int N, bool b_mn) {
     return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 
-// Four values times a power of two as fp16 hi and lo.
+// Four values times a power of two as fp16 hi and lo: hi is the value rounded to 11 bits by integer
+// arithmetic (so that it need not be read back from fp16), lo the exact remainder, rounded.
+PYXIS_DEVINL float to11(float x) { return __uint_as_float((__float_as_uint(x) + 0x1000u) & 0xFFFFE000u); }
 PYXIS_DEVINL void split4(float4 x, float sc, uint2 &hi, uint2 &lo) {
-    const float2 a = make_float2(x.x * sc, x.y * sc), b = make_float2(x.z * sc, x.w * sc);
-    const __half2 ha = __float22half2_rn(a), hb = __float22half2_rn(b);
-    const float2 fa = __half22float2(ha), fb = __half22float2(hb);
-    const __half2 la = __floats2half2_rn(a.x - fa.x, a.y - fa.y), lb = __floats2half2_rn(b.x - fb.x, b.y - fb.y);
+    x.x *= sc, x.y *= sc, x.z *= sc, x.w *= sc;
+    const float4 h = make_float4(to11(x.x), to11(x.y), to11(x.z), to11(x.w));
+    const __half2 ha = __floats2half2_rn(h.x, h.y), hb = __floats2half2_rn(h.z, h.w);
+    const __half2 la = __floats2half2_rn(x.x - h.x, x.y - h.y), lb = __floats2half2_rn(x.z - h.z, x.w - h.w);
     hi = make_uint2(*reinterpret_cast<const uint32_t *>(&ha), *reinterpret_cast<const uint32_t *>(&hb));
     lo = make_uint2(*reinterpret_cast<const uint32_t *>(&la), *reinterpret_cast<const uint32_t *>(&lb));
 }
@@ -99,10 +102,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr int kDB = L::kDB, kRing = L::kRing, kOH = HD / 2;  // columns of O per softmax warp
     extern __shared__ __align__(1024) uint8_t smem[];
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::bar);
-    uint64_t *full = bars, *empty = bars + kRing, *cmax = empty + kRing, *cfull = cmax + 1, *cempty = cfull + 2;  // [K, V]
-    uint64_t *qfull = cempty + 2, *drain = qfull + 1, *ofree = drain + 1;
+    uint64_t *full = bars, *empty = bars + kRing, *cmax = empty + kRing, *cfull = cmax + 1, *cempty = cfull + 4;  // [K, V][2]
+    uint64_t *qfull = cempty + 4, *drain = qfull + 1, *ofree = drain + 1;
     // per score buffer: sfull (S_j landed), pfull (P_j written), odone (P_j V_j done)
-    uint64_t *sfull = ofree + 2, *pfull = sfull + kSBufs, *odone = pfull + kSBufs;
+    uint64_t *sfull = ofree + 2, *pfull = sfull + 2, *odone = pfull + 2;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + L::misc);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::misc + 4);
     // [2]: 1 + the last segment of that parity with a draft's value that is not finite
@@ -111,7 +114,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     int &start_seq = *reinterpret_cast<int *>(smem + L::misc + 24);
     volatile uint32_t *wmax = reinterpret_cast<volatile uint32_t *>(smem + L::wmax);
     volatile float *scale = reinterpret_cast<volatile float *>(smem + L::scale);
-    volatile float *qinv = reinterpret_cast<volatile float *>(smem + L::qinv);
     float *red = reinterpret_cast<float *>(smem + L::red);
     long long *warp_sum = reinterpret_cast<long long *>(smem + L::ring);  // before the ring is used
     const TreeParams &p = a.t;
@@ -127,14 +129,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc::mbar_init(&empty[s], kConvWarps);
         }
         tc::mbar_init(cmax, kConvWarps);
-        for (int b = 0; b < 2; ++b) {
+        for (int b = 0; b < 4; ++b) {
             tc::mbar_init(&cfull[b], kConvWarps);
             tc::mbar_init(&cempty[b], 1);
-            tc::mbar_init(&ofree[b], kSmWarps);
         }
         tc::mbar_init(qfull, kSmWarps);
         tc::mbar_init(drain, 1);
-        for (int b = 0; b < kSBufs; ++b) {
+        for (int b = 0; b < 2; ++b) {
+            tc::mbar_init(&ofree[b], kSmWarps);
             tc::mbar_init(&sfull[b], 1);
             tc::mbar_init(&pfull[b], kSmWarps);
             tc::mbar_init(&odone[b], 1);
@@ -213,7 +215,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // ---------------------------------------------------------------- MMA issuer
                 if (elect_one()) {
                     constexpr uint32_t idesc_s = idesc_f16(kRows, kTile, false), idesc_o = idesc_f16(kRows, HD, true);
-                    const uint64_t q_d = tc::desc_sw128(tc::smem_u32(smem + L::q)), k_d = tc::desc_sw128(tc::smem_u32(smem + L::k));
+                    const uint64_t k_d = tc::desc_sw128(tc::smem_u32(smem + L::k));
                     const uint64_t v_d = desc_mn_sw128(tc::smem_u32(smem + L::v), L::kPanel);
                     int kuse = 0, vuse = 0;  // K and V tiles multiplied
                     auto wait = [&](uint64_t *bar, int phase) -> bool {
@@ -221,42 +223,44 @@ __global__ void __launch_bounds__(kThreads, 1)
                     };
                     bool ok = true;
                     auto score = [&]() -> bool {
-                        const int b = kuse % kSBufs;
+                        const int b = kuse & 1;
                         // the buffer's earlier probabilities have been multiplied, and K is there
-                        if (!wait(&odone[b], kuse / kSBufs - 1) || !wait(&cfull[0], kuse)) return false;
+                        if (!wait(&odone[b], kuse / 2 - 1) || !wait(&cfull[b], kuse / 2)) return false;
                         tc::tc_fence_after();
                         const uint32_t tS = tmem_base + (uint32_t)(b * kTile);
+                        const uint64_t kd = k_d + (uint64_t)(b * (2 * L::kTerm >> 4));
 #pragma unroll
                         for (int term = 0; term < 3; ++term) {  // lo.hi, hi.lo, hi.hi
-                            const uint64_t qt = q_d + (uint64_t)(term == 0 ? L::kQTerm >> 4 : 0);
-                            const uint64_t kt = k_d + (uint64_t)(term == 1 ? L::kTerm >> 4 : 0);
+                            const uint32_t qt = tmem_base + kQCol + (uint32_t)(term == 0 ? HD / 2 : 0);
+                            const uint64_t kt = kd + (uint64_t)(term == 1 ? L::kTerm >> 4 : 0);
 #pragma unroll
                             for (int x = 0; x < kDB; ++x)
 #pragma unroll
-                                for (int kk = 0; kk < 4; ++kk)
-                                    tc::mma_f16(tS, qt + (uint64_t)(x * (L::kQPanel >> 4) + kk * 2),
-                                                kt + (uint64_t)(x * (L::kPanel >> 4) + kk * 2), idesc_s, (uint32_t)(term | x | kk));
+                                for (int kk = 0; kk < 4; ++kk)  // 16 dims: 8 columns of Q
+                                    tc::mma_f16_ts(tS, qt + (uint32_t)(x * 32 + kk * 8),
+                                                   kt + (uint64_t)(x * (L::kPanel >> 4) + kk * 2), idesc_s, (uint32_t)(term | x | kk));
                         }
-                        tc::mma_commit(&cempty[0]);
+                        tc::mma_commit(&cempty[b]);
                         tc::mma_commit(&sfull[b]);
                         ++kuse;
                         return true;
                     };
                     auto output = [&]() -> bool {
-                        const int b = vuse % kSBufs, ob = vuse & 1;
-                        if (!wait(&cfull[1], vuse) || !wait(&pfull[b], vuse / kSBufs) || !wait(&ofree[ob], vuse / 2 - 1)) return false;
+                        const int b = vuse & 1;
+                        if (!wait(&cfull[2 + b], vuse / 2) || !wait(&pfull[b], vuse / 2) || !wait(&ofree[b], vuse / 2 - 1)) return false;
                         tc::tc_fence_after();
-                        const uint32_t tP = tmem_base + (uint32_t)(b * kTile), tO = tmem_base + kOCol + (uint32_t)(ob * HD);
+                        const uint32_t tP = tmem_base + (uint32_t)(b * kTile), tO = tmem_base + kOCol + (uint32_t)(b * HD);
+                        const uint64_t vd = v_d + (uint64_t)(b * (2 * L::kTerm >> 4));
 #pragma unroll
                         for (int term = 0; term < 3; ++term) {
                             const uint32_t pt = tP + (term == 0 ? kTile / 2 : 0);  // lo terms follow the hi ones
-                            const uint64_t vt = v_d + (uint64_t)(term == 1 ? L::kTerm >> 4 : 0);
+                            const uint64_t vt = vd + (uint64_t)(term == 1 ? L::kTerm >> 4 : 0);
 #pragma unroll
                             for (int kk = 0; kk < kTile / 16; ++kk)  // 16 keys: 8 columns of P, 16 rows of V
                                 tc::mma_f16_ts(tO, pt + (uint32_t)(kk * 8), vt + (uint64_t)(kk * (2048 >> 4)), idesc_o,
                                                (uint32_t)(term | kk));
                         }
-                        tc::mma_commit(&cempty[1]);
+                        tc::mma_commit(&cempty[2 + b]);
                         tc::mma_commit(&odone[b]);
                         ++vuse;
                         return true;
@@ -283,61 +287,83 @@ __global__ void __launch_bounds__(kThreads, 1)
                 return __all_sync(0xffffffffu, tc::mbar_wait_bounded(bar, (uint32_t)(phase & 1), abort_flag, p.err, kErrConv,
                                                                      kTimeoutNs));
             };
-            int e = 0, use[2] = {0, 0};
+            int e = 0, use[2] = {0, 0}, looks = 0;  // looks: exchanges of the largest magnitude
+            int ex[2] = {13, 13};                   // scale exponents of K and V
             bool ok = true;
             int seg = 0;
             for (; ok && w.next(p, a.n_seq); ++seg) {
                 const int T = w.te - w.tb;
                 const SeqShape &sh = w.w.sh;
                 auto convert = [&](int is_v, int j) -> bool {
-                    const int slot = e % kRing, parity = e & 1;
+                    const int slot = e % kRing;
                     if (!wait(&full[slot], e / kRing)) return false;
                     const long long k0 = (long long)(w.tb + j) * kTile;
                     const int valid = (int)min((long long)kTile, max(sh.total - k0, 0ll));
                     const int drafts = (int)min((long long)valid, max(sh.ctx - k0, 0ll));  // first draft's row
-                    float4 x[kSteps];
-                    uint32_t m = 0;
-#pragma unroll
-                    for (int i = 0; i < kSteps; ++i) {
-                        const int row = cw * (kTile / kConvWarps) + i * kPer + sub;
-                        x[i] = *reinterpret_cast<const float4 *>(smem + L::ring + slot * L::kEntry + row * (HD * 4) + li * 16);
-                        if (row >= valid) x[i] = make_float4(0.f, 0.f, 0.f, 0.f);  // not loaded, or not a key
+                    // this lane's four dims of row first + i * kPer; zero past the last key (never loaded, or
+                    // not a key), and so is a draft's value that is not finite: the rows that see the draft
+                    // get it back at the end
+                    const int first = cw * (kTile / kConvWarps) + sub;
+                    const float4 *src = reinterpret_cast<const float4 *>(smem + L::ring + slot * L::kEntry) + first * (HD / 4) + li;
+                    const bool inner = valid == kTile && (!is_v || drafts == kTile);
+                    auto edge = [&](int i) -> float4 {
+                        const int row = first + i * kPer;
+                        if (row >= valid) return make_float4(0.f, 0.f, 0.f, 0.f);
+                        float4 x = src[i * 32];
                         if (is_v && row >= drafts) {
-                            // a draft's value that is not finite becomes zero here; the rows that see the
-                            // draft get it back at the end
-                            float *v = &x[i].x;
-#pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                if (!isfinite(v[k])) v[k] = 0.f, bad[seg & 1] = seg + 1;
+                            const bool odd = !isfinite(x.x) || !isfinite(x.y) || !isfinite(x.z) || !isfinite(x.w);
+                            if (odd) {
+                                bad[seg & 1] = seg + 1;
+                                x.x = isfinite(x.x) ? x.x : 0.f, x.y = isfinite(x.y) ? x.y : 0.f;
+                                x.z = isfinite(x.z) ? x.z : 0.f, x.w = isfinite(x.w) ? x.w : 0.f;
+                            }
                         }
-                        m = max(m, magnitude(x[i]));
-                    }
-                    __syncwarp();
-                    m = __reduce_max_sync(0xffffffffu, m);
-                    if (lane == 0) {
-                        tc::mbar_arrive(&empty[slot]);
-                        wmax[parity * kConvWarps + cw] = m;
-                        tc::mbar_arrive(cmax);
-                    }
-                    if (!wait(cmax, e) || !wait(&cempty[is_v], use[is_v] - 1)) return false;
+                        return x;
+                    };
+                    const int buf = use[is_v] & 1;
+                    if (!wait(&cempty[is_v * 2 + buf], use[is_v] / 2 - 1)) return false;
+                    uint8_t *dst = smem + (is_v ? L::v : L::k) + buf * 2 * L::kTerm;
+                    // The scale is that of the tile before, which leaves a factor of 4 to fp16's largest number;
+                    // a tile that does not fit it (or is far below it) is done again with its own.
+                    for (int round = 0;; ++round) {
+                        const float sc = attn_pow2(ex[is_v]);
+                        uint32_t m = 0;
+                        auto put = [&](int i, float4 x) {
+                            uint2 hi, low;
+                            split4(x, sc, hi, low);
+                            const uint32_t at = swizzled(first + i * kPer, li, L::kPanel);
+                            *reinterpret_cast<uint2 *>(dst + at) = hi;
+                            *reinterpret_cast<uint2 *>(dst + L::kTerm + at) = low;
+                            m = max(m, magnitude(x));
+                        };
+                        if (inner) {
+#pragma unroll 2
+                            for (int i = 0; i < kSteps; ++i) put(i, src[i * 32]);
+                        } else {
+#pragma unroll 1
+                            for (int i = 0; i < kSteps; ++i) put(i, edge(i));
+                        }
+                        m = __reduce_max_sync(0xffffffffu, m);
+                        if (lane == 0) {
+                            wmax[(looks & 1) * kConvWarps + cw] = m;
+                            tc::mbar_arrive(cmax);
+                        }
+                        if (!wait(cmax, looks)) return false;
 #pragma unroll
-                    for (int i = 0; i < kConvWarps; ++i) m = max(m, wmax[parity * kConvWarps + i]);
-                    const int ex = attn_scale_exp(__uint_as_float(m));
-                    const float sc = attn_pow2(ex);
-                    uint8_t *dst = smem + (is_v ? L::v : L::k);
-#pragma unroll
-                    for (int i = 0; i < kSteps; ++i) {
-                        const int row = cw * (kTile / kConvWarps) + i * kPer + sub;
-                        uint2 hi, low;
-                        split4(x[i], sc, hi, low);
-                        const uint32_t at = swizzled(row, li, L::kPanel);
-                        *reinterpret_cast<uint2 *>(dst + at) = hi;
-                        *reinterpret_cast<uint2 *>(dst + L::kTerm + at) = low;
+                        for (int i = 0; i < kConvWarps; ++i) m = max(m, wmax[(looks & 1) * kConvWarps + i]);
+                        ++looks;
+                        const float top = __uint_as_float(m) * sc;
+                        const int used = ex[is_v];
+                        if (m) ex[is_v] = attn_scale_exp(__uint_as_float(m)) - 1;  // [2^13, 2^14): for the next tile
+                        if (round > 0 || m == 0 || (top < 65504.f && top >= 1.f)) {
+                            if (cw == 0 && lane == 0) scale[is_v * 4 + (use[is_v] & 3)] = attn_pow2(-used);
+                            break;
+                        }
                     }
-                    if (cw == 0 && lane == 0) scale[is_v * 4 + (use[is_v] & 3)] = attn_pow2(-ex);
+                    if (lane == 0) tc::mbar_arrive(&empty[slot]);
                     tc::fence_proxy_async_smem();
                     __syncwarp();
-                    if (lane == 0) tc::mbar_arrive(&cfull[is_v]);
+                    if (lane == 0) tc::mbar_arrive(&cfull[is_v * 2 + buf]);
                     ++use[is_v];
                     ++e;
                     return true;
@@ -366,52 +392,62 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const SeqShape &sh = w.w.sh;
                 const int rows = min(sh.nodes * p.group - r0, kRows);
                 const bool active = quad * 32 < rows;  // the warp has rows
-                // ---- Q: 16 rows per warp; the last segment's MMAs are done (odone)
-                {
-                    constexpr int kLanes = HD / 4, kPer = 32 / kLanes, kSteps = 16 / kPer;
-                    const int li = lane % kLanes, sub = lane / kLanes;
-                    float4 x[kSteps];
+                // ---- Q into TMEM, this row's half of the dims; the last segment's MMAs are done (odone)
+                float qscale = 1.f;  // 2^-e of the row
+                if (active) {
+                    constexpr int kQ4 = kOH / 4;
+                    float4 x[kQ4];
+                    const int t = (r0 + row) / p.group;
+                    const float *src = reinterpret_cast<const float *>(
+                                           p.q + (sh.row0 + t) * p.q_row + (kvh * p.group + r0 + row - t * p.group) * p.q_head) +
+                                       half * kOH;
+                    uint32_t m = 0;
 #pragma unroll
-                    for (int i = 0; i < kSteps; ++i) {
-                        const int rr = sw * 16 + i * kPer + sub, t = (r0 + rr) / p.group;
+                    for (int i = 0; i < kQ4; ++i) {
                         x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                        if (rr >= rows) continue;
-                        const float *src = reinterpret_cast<const float *>(
-                            p.q + (sh.row0 + t) * p.q_row + (kvh * p.group + r0 + rr - t * p.group) * p.q_head) + li * 4;
-                        x[i] = a.vec_q ? *reinterpret_cast<const float4 *>(src) : make_float4(src[0], src[1], src[2], src[3]);
+                        if (row < rows)
+                            x[i] = a.vec_q ? reinterpret_cast<const float4 *>(src)[i]
+                                           : make_float4(src[4 * i], src[4 * i + 1], src[4 * i + 2], src[4 * i + 3]);
                     }
 #pragma unroll
-                    for (int i = 0; i < kSteps; ++i) {
-                        const int rr = sw * 16 + i * kPer + sub;
-                        uint32_t m = magnitude(x[i]);
+                    for (int i = 0; i < kQ4; ++i) m = max(m, magnitude(x[i]));
+                    float *rd = red + (swaps++ & 1) * 2 * kRows;
+                    rd[half * kRows + row] = __uint_as_float(m);
+                    named_bar(1 + quad, 64);
+                    m = max(m, __float_as_uint(rd[(1 - half) * kRows + row]));
+                    const int ex = attn_scale_exp(__uint_as_float(m));
+                    const float sc = sign * attn_pow2(ex);
+                    qscale = attn_pow2(-ex);
 #pragma unroll
-                        for (int o = kLanes / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-                        const int ex = attn_scale_exp(__uint_as_float(m));
-                        uint2 hi, low;
-                        split4(x[i], sign * attn_pow2(ex), hi, low);
-                        const uint32_t at = swizzled(rr, li, L::kQPanel);
-                        *reinterpret_cast<uint2 *>(smem + L::q + at) = hi;
-                        *reinterpret_cast<uint2 *>(smem + L::q + L::kQTerm + at) = low;
-                        if (li == 0) qinv[rr] = attn_pow2(-ex);
+                    for (int ch = 0; ch < kQ4 / 8; ++ch) {  // 32 dims: 16 columns of each term
+                        uint32_t hi[16], low[16];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            uint2 h2, l2;
+                            split4(x[ch * 8 + i], sc, h2, l2);
+                            hi[2 * i] = h2.x, hi[2 * i + 1] = h2.y, low[2 * i] = l2.x, low[2 * i + 1] = l2.y;
+                        }
+                        tmem_st16(tq + kQCol + (uint32_t)(half * (kOH / 2) + ch * 16), hi);
+                        tmem_st16(tq + kQCol + (uint32_t)(HD / 2 + half * (kOH / 2) + ch * 16), low);
                     }
-                    tc::fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) tc::mbar_arrive(qfull);
+                    tc::tmem_wait_st();
+                    tc::tc_fence_before();
                 }
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(qfull);
                 unsigned long long mask = 0;
                 if (row < rows) {
                     const int t = (r0 + row) / p.group;
                     mask = p.tree_mask ? p.tree_mask[sh.row0 + t] : (2ull << t) - 1;
                 }
-                ok = ok && wait(qfull, seg);
-                const float c2row = fabsf(p.scale2) * qinv[row];
+                const float c2row = fabsf(p.scale2) * qscale;
                 float m_run = -INFINITY, l = 0.f;
                 float acc[kOH];
 #pragma unroll
                 for (int i = 0; i < kOH; ++i) acc[i] = 0.f;
                 // (O + acc) of tile m into acc, then times alpha
                 auto fold = [&](int m, float alpha) -> bool {
-                    if (!wait(&odone[m % kSBufs], m / kSBufs)) return false;
+                    if (!wait(&odone[m & 1], m / 2)) return false;
                     if (active) {
                         tc::tc_fence_after();
                         const float vs = scale[4 + (m & 3)];
@@ -432,11 +468,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // after a failed wait the loops run on without work, so that the barriers of a row's two
                 // warps keep their counts
                 for (int j = 0; j < T; ++j, ++n) {
-                    const int b = n % kSBufs;
+                    const int b = n & 1;
                     const long long k0 = (long long)(w.tb + j) * kTile;
                     const uint32_t tS = tq + (uint32_t)(b * kTile);
                     const bool tail = k0 + kTile > sh.ctx;
-                    ok = ok && wait(&sfull[b], n / kSBufs);
+                    ok = ok && wait(&sfull[b], n / 2);
                     float alpha = 1.f;
                     if (active) {
                         float s[32];
