@@ -34,12 +34,12 @@ namespace pyxis {
 namespace {
 
 constexpr int kRows = kTcRows, kTile = 64;
-constexpr int kProdWarp = 0, kMmaWarp = 1, kConvWarp0 = 4, kConvWarps = 4, kSmWarp0 = 8, kSmWarps = 8;
+constexpr int kProdWarp = 0, kMmaWarp = 1, kConvWarp0 = 2, kConvWarps = 6, kSmWarp0 = 8, kSmWarps = 8;
 constexpr int kThreads = (kSmWarp0 + kSmWarps) * 32;
 // Registers per thread of the four warpgroups (producer and MMA, converters, softmax twice): their sum
 // stays below what the block is launched with, 4 x 128.
-constexpr int kRegsLaunch = 128, kRegsFew = 88, kRegsConv = 88, kRegsSoft = 160;
-static_assert(kRegsFew + kRegsConv + 2 * kRegsSoft <= 4 * kRegsLaunch - 16, "register split");
+constexpr int kRegsLaunch = 128, kRegsFew = 88, kRegsSoft = 160;
+static_assert(2 * kRegsFew + 2 * kRegsSoft <= 4 * kRegsLaunch - 16, "register split");
 constexpr uint32_t kTmemCols = 512, kOCol = 2 * kTile, kQCol = kOCol + 2 * 128;  // S twice, O twice, Q hi and lo
 constexpr uint64_t kTimeoutNs = 2000000000ull;
 constexpr float kRaise = 11.0f;  // weights up to 2^11 stay in fp16's range
@@ -58,7 +58,7 @@ struct Smem {
     static constexpr int kBars = 2 * kRing + 1 + 4 + 4 + 1 + 1 + 2 + 3 * 2;
     static constexpr uint32_t misc = bar + (kBars * 8 + 15) / 16 * 16;
     static constexpr uint32_t wmax = misc + 64;          // [2][kConvWarps] magnitudes
-    static constexpr uint32_t scale = wmax + 32;         // [2][4]: 2^-e of K and of V of the latest tiles
+    static constexpr uint32_t scale = wmax + 64;         // [2][4]: 2^-e of K and of V of the latest tiles
     static constexpr uint32_t red = scale + 32;          // [2][2 halves][128 rows]
     static constexpr uint32_t bytes = red + 2 * 2 * kRows * 4;
 };
@@ -162,8 +162,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int g = r.ctas, c = blockIdx.x;
     if (count > 0) {
         // (all warps of a warpgroup, and of the CTA, come here or none: count is the CTA's)
+        if (warp < kSmWarp0) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsFew));
         if (warp < kConvWarp0) {
-            asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsFew));
             if (warp == kProdWarp) {
                 // ---------------------------------------------------------------- producer
                 int e = 0;
@@ -278,10 +278,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
         } else if (warp < kSmWarp0) {
-            asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsConv));
             // ---------------------------------------------------------------- converters
             const int cw = warp - kConvWarp0;
-            constexpr int kLanes = HD / 4, kPer = 32 / kLanes, kSteps = kTile / kConvWarps / kPer;  // lanes of a row
+            constexpr int kLanes = HD / 4, kPer = 32 / kLanes, kSteps = kTile / kPer;  // lanes of a row, rows and steps of a warp
             const int li = lane % kLanes, sub = lane / kLanes;
             auto wait = [&](uint64_t *bar, int phase) -> bool {
                 return __all_sync(0xffffffffu, tc::mbar_wait_bounded(bar, (uint32_t)(phase & 1), abort_flag, p.err, kErrConv,
@@ -300,14 +299,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const long long k0 = (long long)(w.tb + j) * kTile;
                     const int valid = (int)min((long long)kTile, max(sh.total - k0, 0ll));
                     const int drafts = (int)min((long long)valid, max(sh.ctx - k0, 0ll));  // first draft's row
-                    // this lane's four dims of row first + i * kPer; zero past the last key (never loaded, or
+                    // this lane's four dims of row i * kPer + sub; zero past the last key (never loaded, or
                     // not a key), and so is a draft's value that is not finite: the rows that see the draft
                     // get it back at the end
-                    const int first = cw * (kTile / kConvWarps) + sub;
-                    const float4 *src = reinterpret_cast<const float4 *>(smem + L::ring + slot * L::kEntry) + first * (HD / 4) + li;
+                                        const float4 *src = reinterpret_cast<const float4 *>(smem + L::ring + slot * L::kEntry) + lane;
                     const bool inner = valid == kTile && (!is_v || drafts == kTile);
                     auto edge = [&](int i) -> float4 {
-                        const int row = first + i * kPer;
+                        const int row = i * kPer + sub;
                         if (row >= valid) return make_float4(0.f, 0.f, 0.f, 0.f);
                         float4 x = src[i * 32];
                         if (is_v && row >= drafts) {
@@ -331,17 +329,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                         auto put = [&](int i, float4 x) {
                             uint2 hi, low;
                             split4(x, sc, hi, low);
-                            const uint32_t at = swizzled(first + i * kPer, li, L::kPanel);
+                            const uint32_t at = swizzled(i * kPer + sub, li, L::kPanel);
                             *reinterpret_cast<uint2 *>(dst + at) = hi;
                             *reinterpret_cast<uint2 *>(dst + L::kTerm + at) = low;
                             m = max(m, magnitude(x));
                         };
                         if (inner) {
 #pragma unroll 2
-                            for (int i = 0; i < kSteps; ++i) put(i, src[i * 32]);
+                            for (int i = cw; i < kSteps; i += kConvWarps) put(i, src[i * 32]);
                         } else {
 #pragma unroll 1
-                            for (int i = 0; i < kSteps; ++i) put(i, edge(i));
+                            for (int i = cw; i < kSteps; i += kConvWarps) put(i, edge(i));
                         }
                         m = __reduce_max_sync(0xffffffffu, m);
                         if (lane == 0) {
@@ -617,7 +615,7 @@ cudaError_t run_tc32(const CUtensorMap &k, const CUtensorMap &v, const TcParams 
         const cudaError_t x = cudaFuncGetAttributes(&at, kern);
         if (x != cudaSuccess) return x;
         // the softmax warps' share is taken from the launch's registers: with fewer they would wait for good
-        if (at.numRegs * 4 < kRegsFew + kRegsConv + 2 * kRegsSoft) return cudaErrorInvalidConfiguration;
+        if (at.numRegs * 4 < 2 * kRegsFew + 2 * kRegsSoft) return cudaErrorInvalidConfiguration;
         return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Smem<HD>::bytes);
     });
     if (e != cudaSuccess) return e;
