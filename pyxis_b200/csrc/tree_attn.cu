@@ -796,7 +796,7 @@ TreePlan plan_tree_attention(const pyxis_tree_attention_args &a, const pyxis_kv_
     // 18 against 21, of 2303 39 against 27.
     // f32: the tcgen05 kernel pays the same for 1 row as for 128 (three products of 128 rows and the
     // conversion of every key), the mma.sync kernel for each tile of 16.  16 sequences of 2303 positions:
-    // 16 rows 89 us against the tcgen05 kernel's 113, 32 rows 160 against 115, 64 rows 310 against 120;
+    // 16 rows 89 us against the tcgen05 kernel's 100, 32 rows 160 against 100, 64 rows 310 against 105;
     // one sequence of 152: 16 rows 18 against 24, 128 rows 31 against 25.
     const bool f32 = kv.dtype == PYXIS_DTYPE_F32;
     t.tensor = f32 ? tree_attention_tc32_supported(a, kv) && rows > 16

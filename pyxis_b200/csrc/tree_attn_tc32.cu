@@ -10,17 +10,18 @@
 //
 // 64 keys of K and V are 64 KB that take 2800 cycles to arrive at an SM; their products are 36 MMAs
 // (about 2000 cycles) for up to 128 rows, and Q lies in TMEM, so that they read no more of shared memory
-// than K's and V's terms.  The converters bound it: 64 KB read, split and written again per tile by four
+// than K's and V's terms.  The converters bound it: 64 KB read, split and written again per tile by six
 // warps.  The scale of a tile is taken from the tile before (with room of a factor of four), which spares
-// them a pass over it for its largest magnitude: 137 -> 115 us for 16 sequences of 2303 positions and 16
-// nodes (8 kv heads of 128, a floor of 41 us at the memory's rate), 374 -> 316 us for 58 sequences of
-// 1731 positions and 64 nodes (121 us).
+// them a pass over it for its largest magnitude (137 -> 115 us for 16 sequences of 2303 positions and 16
+// nodes, 8 kv heads of 128), six warps instead of four 115 -> 106, loops that are not unrolled, for the
+// instruction cache's sake, 106 -> 100: a floor of 41 us at the memory's rate.  58 sequences of 1731
+// positions and 64 nodes 290 us (121).
 //
 // One CTA per SM takes an equal share of all units' tiles (tree_attn_tc.cuh).  Warps:
 //   0       producer: a tile's pages by TMA (one box per page) into a ring of f32 tiles, in the order
 //           S_0, S_1, O_0, S_2, O_1, ... of the MMAs
 //   1       MMA issuer (and TMEM owner)
-//   4-7     converters: a tile from the ring into its two fp16 terms, in the 128-byte swizzle, twice
+//   2-7     converters: a tile from the ring into its two fp16 terms, in the 128-byte swizzle, twice
 //           buffered; the tile's largest magnitude is found on the way and sets the next one's scale
 //   8-15    softmax: a row per thread, half of a tile's keys and of O's columns per warp.  They split
 //           their rows of Q into TMEM at a segment's start.
@@ -229,7 +230,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         tc::tc_fence_after();
                         const uint32_t tS = tmem_base + (uint32_t)(b * kTile);
                         const uint64_t kd = k_d + (uint64_t)(b * (2 * L::kTerm >> 4));
-#pragma unroll
+#pragma unroll 1
                         for (int term = 0; term < 3; ++term) {  // lo.hi, hi.lo, hi.hi
                             const uint32_t qt = tmem_base + kQCol + (uint32_t)(term == 0 ? HD / 2 : 0);
                             const uint64_t kt = kd + (uint64_t)(term == 1 ? L::kTerm >> 4 : 0);
@@ -251,7 +252,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         tc::tc_fence_after();
                         const uint32_t tP = tmem_base + (uint32_t)(b * kTile), tO = tmem_base + kOCol + (uint32_t)(b * HD);
                         const uint64_t vd = v_d + (uint64_t)(b * (2 * L::kTerm >> 4));
-#pragma unroll
+#pragma unroll 1
                         for (int term = 0; term < 3; ++term) {
                             const uint32_t pt = tP + (term == 0 ? kTile / 2 : 0);  // lo terms follow the hi ones
                             const uint64_t vt = vd + (uint64_t)(term == 1 ? L::kTerm >> 4 : 0);
@@ -302,7 +303,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     // this lane's four dims of row i * kPer + sub; zero past the last key (never loaded, or
                     // not a key), and so is a draft's value that is not finite: the rows that see the draft
                     // get it back at the end
-                                        const float4 *src = reinterpret_cast<const float4 *>(smem + L::ring + slot * L::kEntry) + lane;
+                    const float4 *src = reinterpret_cast<const float4 *>(smem + L::ring + slot * L::kEntry) + lane;
                     const bool inner = valid == kTile && (!is_v || drafts == kTile);
                     auto edge = [&](int i) -> float4 {
                         const int row = i * kPer + sub;
@@ -325,21 +326,26 @@ __global__ void __launch_bounds__(kThreads, 1)
                     // a tile that does not fit it (or is far below it) is done again with its own.
                     for (int round = 0;; ++round) {
                         const float sc = attn_pow2(ex[is_v]);
-                        uint32_t m = 0;
+                        float mf = 0.f;  // (fmaxf passes over NaN)
                         auto put = [&](int i, float4 x) {
                             uint2 hi, low;
                             split4(x, sc, hi, low);
                             const uint32_t at = swizzled(i * kPer + sub, li, L::kPanel);
                             *reinterpret_cast<uint2 *>(dst + at) = hi;
                             *reinterpret_cast<uint2 *>(dst + L::kTerm + at) = low;
-                            m = max(m, magnitude(x));
+                            mf = fmaxf(fmaxf(fmaxf(mf, fabsf(x.x)), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
                         };
                         if (inner) {
-#pragma unroll 2
+#pragma unroll 1
                             for (int i = cw; i < kSteps; i += kConvWarps) put(i, src[i * 32]);
                         } else {
 #pragma unroll 1
                             for (int i = cw; i < kSteps; i += kConvWarps) put(i, edge(i));
+                        }
+                        uint32_t m = __float_as_uint(mf);
+                        if (m == 0x7F800000u) {  // an infinity, which sets no scale: the largest finite one
+                            m = 0;
+                            for (int i = cw; i < kSteps; i += kConvWarps) m = max(m, magnitude(edge(i)));
                         }
                         m = __reduce_max_sync(0xffffffffu, m);
                         if (lane == 0) {
