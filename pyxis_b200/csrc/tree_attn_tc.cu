@@ -46,7 +46,8 @@ template <int HD>
 struct Smem {
     static constexpr int kDB = HD / 64;                  // 64-column panels of a row
     static constexpr uint32_t kPanel = kTile * 128;      // 128 rows x 128 B
-    static constexpr uint32_t kEntry = kDB * kPanel;     // a tile of K or of V
+    static constexpr uint32_t kEntry = kDB * kPanel;     // a tile of K or of V (or Q, panel after panel):
+    static constexpr uint32_t kGroup = kDB * 1024;       // groups of 8 rows, each panel after panel
     static constexpr int kRing = HD == 128 ? 5 : 12;
     static constexpr uint32_t q = 0;  // two buffers: the next segment's rows come while this one runs
     static constexpr uint32_t ring = q + 2 * kEntry;
@@ -196,11 +197,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (lane == 0) tc::mbar_arrive_expect_tx(&full[slot], (uint32_t)(n * a.box_rows * HD * 2));
                     __syncwarp();
                     if (lane < n) {
-                        uint8_t *dst = smem + L::ring + slot * L::kEntry + lane * a.box_rows * 128;
+                        uint8_t *dst = smem + L::ring + slot * L::kEntry + lane * a.box_rows * (HD * 2);
                         const int row = a.page_tiles == 1 ? 0 : (w.tb + j) % a.page_tiles * kTile;
-#pragma unroll
-                        for (int x = 0; x < kDB; ++x)
-                            tma_load_4d(dst + x * L::kPanel, is_k ? &tm_k : &tm_v, x * 64, kvh, row, page, &full[slot]);
+                        const void *map = is_k ? &tm_k : &tm_v;
+                        if (kDB == 1 || a.head_units) {
+                            tma_load_5d(dst, map, 0, 0, kDB == 1 ? kvh : kvh * a.head_units, row / 8, page, &full[slot]);
+                        } else {
+                            for (int i = 0; i < a.box_rows / 8 * kDB; ++i)
+                                tma_load_5d(dst + i * 1024, map, i % kDB * 64, 0, kvh, row / 8 + i / kDB, page, &full[slot]);
+                        }
                     }
                     newest = e;
                     return true;
@@ -231,8 +236,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (elect_one()) {
                 constexpr uint32_t idesc_s = idesc_bf16(kRows, kTile, false), idesc_o = idesc_bf16(kRows, HD, true);
                 const uint64_t q_d = tc::desc_sw128(tc::smem_u32(smem + L::q));
-                const uint64_t k_d = tc::desc_sw128(tc::smem_u32(smem + L::ring));
-                const uint64_t v_d = desc_mn_sw128(tc::smem_u32(smem + L::ring), L::kPanel);
+                const uint64_t k_d = desc_rows_sw128(tc::smem_u32(smem + L::ring), 1024, L::kGroup), v_d = k_d;
                 const uint32_t tO = tmem_base + kOCol;
                 int slot = 0, fills = 0;   // ring
                 int sb = 0, suse = 0;      // score buffer of the next S, and how often it was used
@@ -252,7 +256,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk)
                             tc::mma_f16(tS, qd + (uint64_t)(x * (L::kPanel >> 4) + kk * 2),
-                                        kd + (uint64_t)(x * (L::kPanel >> 4) + kk * 2), idesc_s, (uint32_t)(x | kk));
+                                        kd + (uint64_t)(x * (1024 >> 4) + kk * 2), idesc_s, (uint32_t)(x | kk));
                     tc::mma_commit(&empty[slot]);
                     tc::mma_commit(&sfull[sb]);
                     if (++slot == kRing) slot = 0, ++fills;
@@ -266,7 +270,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const uint64_t vd = v_d + (uint64_t)(slot * (L::kEntry >> 4));
 #pragma unroll
                     for (int kk = 0; kk < kTile / 16; ++kk)  // 16 keys: 8 columns of P, 16 rows of V
-                        tc::mma_f16_ts(tO, tS + (uint32_t)(kk * 8), vd + (uint64_t)(kk * (2048 >> 4)), idesc_o,
+                        tc::mma_f16_ts(tO, tS + (uint32_t)(kk * 8), vd + (uint64_t)(kk * (2 * L::kGroup >> 4)), idesc_o,
                                        (uint32_t)(add || kk > 0));
                     tc::mma_commit(&empty[slot]);
                     tc::mma_commit(&odone[ob]);
@@ -336,7 +340,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         const int drafts = (int)min((long long)valid, max(sh.ctx - k0, 0ll));  // first draft's row
                         for (int i = tid; ok && i < (kTile - drafts) * (HD / 8); i += kSmWarps * 32) {
                             const int r = drafts + i / (HD / 8), ch = i % (HD / 8);
-                            uint4 *at = reinterpret_cast<uint4 *>(v + (ch >> 3) * L::kPanel + r * 128 + ((ch & 7) << 4));
+                            uint4 *at = reinterpret_cast<uint4 *>(v + (r >> 3) * L::kGroup + (ch >> 3) * 1024 + ((r & 7) << 7) + ((ch & 7) << 4));
                             if (r >= valid) {
                                 *at = make_uint4(0, 0, 0, 0);
                                 continue;
@@ -500,18 +504,29 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == kMmaWarp) tc::tmem_dealloc(tmem_base, kTmemCols);
 }
 
-// [page][slot][head][64-column panel] of K or V
-bool make_map(CUtensorMap *m, const void *base, const pyxis_kv_pages &kv, int box_rows) {
+// K or V as [page][8-slot group][panel][slot of 8][64 columns], with panels counted over all heads, so that
+// a page is one box in the order in which it lies in shared memory; heads that are not a whole number of
+// panels apart are an axis of their own, and boxes are a group's panel.
+bool make_map(CUtensorMap *m, const void *base, const pyxis_kv_pages &kv, int box_rows, int head_units) {
     auto fn = tensor_map_encoder();
     if (!fn) return false;
+    const bool panels = head_units > 0 || kv.head_dim == 64;
+    const int db = kv.head_dim / 64;
     const auto stride = [&](int n, int64_t s) { return (cuuint64_t)(n > 1 ? s : kv.head_dim) * 2; };  // of an axis of one: any
-    cuuint64_t dims[4] = {(cuuint64_t)kv.head_dim, (cuuint64_t)kv.n_kv_heads, (cuuint64_t)kv.page_size,
+    cuuint64_t dims[5] = {(cuuint64_t)(panels ? 64 : kv.head_dim), 8, (cuuint64_t)kv.n_kv_heads, (cuuint64_t)kv.page_size / 8,
                           (cuuint64_t)kv.num_pages};
-    cuuint64_t strides[3] = {stride(kv.n_kv_heads, kv.head_stride), stride(kv.page_size, kv.slot_stride),
-                             stride(kv.num_pages, kv.page_stride)};
-    cuuint32_t box[4] = {64, 1, (cuuint32_t)box_rows, 1};
-    cuuint32_t es[4] = {1, 1, 1, 1};
-    return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(base), dims, strides, box, es,
+    cuuint64_t strides[4] = {(cuuint64_t)kv.slot_stride * 2, stride(kv.n_kv_heads, kv.head_stride),
+                             stride(kv.page_size / 8, kv.slot_stride * 8), stride(kv.num_pages, kv.page_stride)};
+    cuuint32_t box[5] = {64, 8, 1, (cuuint32_t)box_rows / 8, 1};
+    if (head_units > 0) {
+        dims[2] = (cuuint64_t)(kv.n_kv_heads - 1) * head_units + db;
+        strides[1] = 128;
+        box[2] = (cuuint32_t)db;
+    } else if (!panels) {
+        box[3] = 1;
+    }
+    cuuint32_t es[5] = {1, 1, 1, 1, 1};
+    return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void *>(base), dims, strides, box, es,
               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -535,7 +550,7 @@ cudaError_t run_tc(const CUtensorMap &k, const CUtensorMap &v, const TcParams &a
 // Boxes of whole 8-row swizzle groups: a page of 8 to 128 slots that tiles 128 keys, or a multiple of
 // 128 slots.  Strides within the tensor map's 2^40 bytes.
 bool tree_attention_tc_supported(const pyxis_tree_attention_args &a, const pyxis_kv_pages &kv) {
-    const int64_t most = (int64_t)1 << 38;
+    const int64_t most = (int64_t)1 << 35;  // (a group of 8 slots is an axis)
     return kv.dtype == PYXIS_DTYPE_BF16 && kv.page_size % 8 == 0 &&
            (kTile % kv.page_size == 0 || kv.page_size % kTile == 0) && kv.page_stride < most &&
            kv.slot_stride < most && kv.head_stride < most;
@@ -560,8 +575,12 @@ cudaError_t launch_tree_attention_tc(const TreeParams &p, const pyxis_tree_atten
     a.vec_q = a.q_sign == 0 && vec(args.q, args.q_row, args.q_head);
     a.vec_out = vec(args.out, args.out_row, args.out_head);
     set_tc_workspace(a, workspace, kv.head_dim, num_sms);
+    // panels counted over all heads, as far as a coordinate reaches
+    const int64_t units = kv.n_kv_heads == 1 ? kv.head_dim / 64 : kv.head_stride % 64 == 0 ? kv.head_stride / 64 : 0;
+    a.head_units = kv.head_dim == 128 && units > 0 && units * kv.n_kv_heads < (1ll << 31) ? (int)units : 0;
     CUtensorMap k, v;
-    if (!make_map(&k, kv.k, kv, a.box_rows) || !make_map(&v, kv.v, kv, a.box_rows)) return cudaErrorInvalidValue;
+    if (!make_map(&k, kv.k, kv, a.box_rows, a.head_units) || !make_map(&v, kv.v, kv, a.box_rows, a.head_units))
+        return cudaErrorInvalidValue;
     return kv.head_dim == 128 ? run_tc<128>(k, v, a, num_sms, st) : run_tc<64>(k, v, a, num_sms, st);
 }
 

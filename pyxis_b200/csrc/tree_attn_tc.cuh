@@ -19,6 +19,7 @@ struct TcParams {
     int box_rows;       // rows of a TMA box: a page, or a tile of a larger page
     int tile_pages;     // boxes per tile
     int page_tiles;     // tiles per page (1 for pages of up to 128 slots)
+    int head_units;     // bf16: 64-column panels from a kv head to the next; 0 if that is no whole number
     int vec_q, vec_out; // 16-byte accesses to q's and out's rows
     uint32_t q_sign;    // flips q's signs for a negative scale (bf16 pairs)
     float *part_o, *part_ml;  // [CTA][2][HD][128], [CTA][2][128][2]
@@ -31,6 +32,13 @@ struct Shared {
     int last, row0, kvh, r0, rows;
 };
 
+PYXIS_DEVINL void tma_load_5d(void *dst, const void *tmap, int x, int y, int z, int w, int v, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(
+            tc::smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(v), "r"(tc::smem_u32(bar))
+        : "memory");
+}
 PYXIS_DEVINL void tma_load_4d(void *dst, const void *tmap, int x, int y, int z, int w, uint64_t *bar) {
     asm volatile(
         "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
@@ -39,12 +47,13 @@ PYXIS_DEVINL void tma_load_4d(void *dst, const void *tmap, int x, int y, int z, 
         : "memory");
 }
 
-// MN-major operand, 128-byte swizzle: 64-element panels `panel` bytes apart, 8-row groups 1024 bytes apart.
-PYXIS_DEVINL uint64_t desc_mn_sw128(uint32_t smem_addr, uint32_t panel) {
+// Operand in the 128-byte swizzle: 64-element panels `panel` bytes apart (which a K-major one does not
+// look at), 8-row groups `group` bytes apart.
+PYXIS_DEVINL uint64_t desc_rows_sw128(uint32_t smem_addr, uint32_t panel, uint32_t group) {
     uint64_t d = 0;
     d |= (uint64_t)((smem_addr & 0x3FFFFu) >> 4);
     d |= (uint64_t)(panel >> 4) << 16;
-    d |= (uint64_t)(1024u >> 4) << 32;
+    d |= (uint64_t)(group >> 4) << 32;
     d |= (uint64_t)1 << 46;
     d |= (uint64_t)2 << 61;
     return d;

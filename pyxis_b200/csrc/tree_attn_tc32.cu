@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (elect_one()) {
                     constexpr uint32_t idesc_s = idesc_f16(kRows, kTile, false), idesc_o = idesc_f16(kRows, HD, true);
                     const uint64_t k_d = tc::desc_sw128(tc::smem_u32(smem + L::k));
-                    const uint64_t v_d = desc_mn_sw128(tc::smem_u32(smem + L::v), L::kPanel);
+                    const uint64_t v_d = desc_rows_sw128(tc::smem_u32(smem + L::v), L::kPanel, 1024);
                     int kuse = 0, vuse = 0;  // K and V tiles multiplied
                     auto wait = [&](uint64_t *bar, int phase) -> bool {
                         return tc::mbar_wait_bounded(bar, (uint32_t)(phase & 1), abort_flag, p.err, kErrMma, kTimeoutNs);

@@ -322,6 +322,132 @@ def test_tree_workspace_is_checked_and_enough():
     assert torch.equal(t.run(workspace=torch.empty(4 << 20, dtype=torch.uint8, device="cuda")), want)
 
 
+def relaid(x, pad=0, slots=0, order="nd"):
+    """The same pages [num, size, heads, hd] in other strides, NaN between."""
+    num, size, heads, hd = x.shape
+    if order == "heads":  # heads outermost
+        wide = torch.full((heads, num, size + slots, hd + pad), math.nan, dtype=x.dtype, device="cuda").permute(1, 2, 0, 3)
+    else:
+        wide = torch.full((num, size + slots, heads, hd + pad), math.nan, dtype=x.dtype, device="cuda")
+    y = wide[:, :size, :, :hd]
+    y.copy_(x)
+    return y
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("trees", [[20, 5], [2, 1]])
+def test_cache_strides(dt, hd, trees):
+    t = Tree(30, [700, 131], trees, 8, 4, hd, dt)
+    want = t.run()
+    t.check(want)
+    a = t.args()
+    for pad, slots, order in ((8, 0, "nd"), (16, 3, "nd"), (64, 0, "nd"), (0, 0, "heads"), (24, 1, "heads")):
+        k, v = relaid(t.k, pad, slots, order), relaid(t.v, pad, slots, order)
+        assert torch.equal(px.tree_attention_dev(a[0], k, v, *a[3:], max_tree=max(trees)), want)
+    # one kv head; keys and values in one buffer
+    t = Tree(31, [300], [trees[0]], 4, 1, hd, dt)
+    a, both = t.args(), torch.stack([t.k, t.v], 2)
+    assert torch.equal(px.tree_attention_dev(a[0], relaid(t.k, 8), relaid(t.v, 8), *a[3:], max_tree=trees[0]), t.run())
+    out = px.tree_attention_dev(a[0], both[:, :, 0], both[:, :, 1], *a[3:], max_tree=trees[0])
+    t.check(out)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("trees", [[40, 3, 0, 17], [2, 1, 1, 2]])
+@pytest.mark.parametrize("page", [1, 8, 24, 64, 128, 256, 384])
+def test_page_sizes(dt, hd, trees, page):
+    t = Tree(page, [700, 127, 385, 0], trees, 6, 3, hd, dt, page)
+    t.check(t.run())
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("nodes", [1, 12])
+def test_many_ragged_sequences(dt, nodes):
+    rng = np.random.default_rng(nodes)
+    n = 1100
+    ctx, trees = rng.integers(0, 70, n), rng.integers(0, nodes + 1, n)
+    ctx[::97] = rng.integers(0, 600, len(ctx[::97]))
+    t = Tree(nodes, ctx.tolist(), trees.tolist(), 4, 2, 64, dt)
+    t.check(t.run())
+    t.check(t.run(max_context=600))
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("trees", [[40, 9], [8, 3], [2, 1]])
+def test_odd_strides_of_rows_and_negative_scales(dt, trees):
+    t = Tree(33, [333, 90], trees, 8, 4, 64, dt)
+    a, n = t.args(), sum(trees)
+    want = t.run()
+    q = torch.full((n, 9, 67), math.nan, dtype=dt, device="cuda")[:, 1:, 3:]
+    q.copy_(t.q)
+    buf = torch.full((n, 9, 65), 7.0, dtype=dt, device="cuda")
+    got = px.tree_attention_dev(q, *a[1:], max_tree=max(trees), out=buf[:, :8, 1:])
+    assert torch.equal(got, want)
+    assert (buf[:, 8] == 7).all() and (buf[:, :, 0] == 7).all()
+    for scale in (-0.11, 0.0, 1e-3):
+        t.check(t.run(scale=scale), scale=scale)
+        assert torch.equal(px.tree_attention_dev(q, *a[1:], max_tree=max(trees), scale=scale, out=buf[:, :8, 1:]), t.run(scale=scale))
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("group,nodes", [(1, 64), (2, 10), (16, 3)])
+def test_nodes_past_max_tree_and_masks_past_the_tree(dt, group, nodes):
+    hq = 2 * group
+    t = Tree(34, [150, 40], [nodes, 2], hq, 2, 128, dt)
+    t.check(t.run())
+    if nodes < 64:  # bits of nodes that are not there count for nothing
+        want = t.run()
+        t.mask |= np.uint64((1 << 63) | (1 << nodes))
+        assert torch.equal(t.run(), want)
+    most = max(2, nodes // 2)
+    out = torch.full_like(t.q, 5.0)
+    t.run(max_tree=most, out=out)
+    assert (out[most:nodes] == 5).all() and (out[:most] != 5).any()
+    part = Tree(34, [150, 40], [nodes, 2], hq, 2, 128, dt)
+    part.mask[:] &= np.uint64((1 << most) - 1)  # the nodes left out are no keys either
+    part.check(torch.cat([out[:most], part.run()[most:]]))
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_every_tensor_on_a_side_stream_and_uint64_masks(dt):
+    t = Tree(35, [900, 4, 60], [30, 1, 64], 4, 1, 128, dt)
+    a = t.args()
+    want = t.run()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        b = [x.clone() for x in a[:6]] + [a[6].view(torch.uint64).clone()]
+        out = px.tree_attention_dev(*b, max_tree=64)
+    s.synchronize()
+    assert torch.equal(out, want)
+    ws = torch.empty(64 << 20, dtype=torch.uint8, device="cuda")  # two calls at once: a workspace each
+    out2 = torch.empty_like(out)
+    with torch.cuda.stream(s):
+        px.tree_attention_dev(*b, max_tree=64, out=out2, workspace=ws)
+    out3 = t.run()
+    torch.cuda.synchronize()
+    assert torch.equal(out2, want) and torch.equal(out3, want)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("size", [1e-30, 1e-3, 1e18])
+def test_tree_attention_of_very_small_and_large_values(dt, size):
+    # scores of an ordinary size from keys far from 1, values far from 1, and one tile much larger than the rest
+    t = Tree(36, [500, 70], [20, 40], 4, 2, 128, dt)
+    t.k *= size
+    t.v *= size
+    t.v[int(t.table[0, 20])] *= 64.0
+    t.q /= size
+    for i in range(2):
+        n = t.ctx[i] + t.trees[i]
+        pos = np.arange(n)
+        pages, slots = t.table[i][pos // t.page].astype(np.int64), pos % t.page
+        t.keys[i], t.vals[i] = t.k[pages, slots].double().cpu(), t.v[pages, slots].double().cpu()
+    t.check(t.run())
+
+
 # ------------------------------------------------------------------------------------------ pages
 @pytest.mark.parametrize("dt", [F32, BF16])
 @pytest.mark.parametrize("layers,size,heads,hd,order", [(1, 16, 1, 64, "nd"), (3, 16, 8, 128, "nd"), (2, 5, 3, 64, "hd"), (4, 64, 2, 128, "lay")])
