@@ -13,11 +13,11 @@
 // sequences load all SMs alike.  A unit inside one CTA is written out at once; one that several
 // CTAs share leaves unnormalised partial sums (at most two per CTA) that a second kernel joins.
 //
-// Warps: 0 and 2 producers (of K and Q, and of V), 1 MMA issuer (and TMEM owner), 4-11 softmax: a row
+// Warps: 0, 2 and 3 producers (of K, of V and of Q), 1 MMA issuer (and TMEM owner), 4-11 softmax: a row
 // per thread, half of a tile's keys per warp.
-//   producers  a tile's pages by TMA (one box per page and 64 columns, 128-byte swizzle) through a
-//              ring of tiles in the order S_0, S_1, O_0, S_2, O_1, ... of the MMAs; the next segment's
-//              Q rows by cp.async while the current one runs
+//   producers  a tile's pages by TMA (one box per page, 128-byte swizzle) through a ring of tiles in the
+//              order S_0, S_1, O_0, S_2, O_1, ... of the MMAs; the next segment's Q rows by cp.async while
+//              the current one runs (the first segment's, which everything waits for, by the softmax warps)
 //   MMA        S_j into one of three TMEM buffers; O += P_j V_j with P_j from TMEM and V_j as an
 //              MN-major operand, as it lies in the cache
 //   softmax    reads S_j, masks the tiles that hold drafts or end inside, writes P_j over S_j.  The
@@ -34,7 +34,7 @@ namespace pyxis {
 namespace {
 
 constexpr int kRows = kTcRows, kTile = 128;
-constexpr int kProdWarp = 0, kMmaWarp = 1, kProdWarpV = 2, kSmWarp0 = 4, kSmWarps = 8;
+constexpr int kProdWarp = 0, kMmaWarp = 1, kProdWarpV = 2, kProdWarpQ = 3, kSmWarp0 = 4, kSmWarps = 8;
 constexpr int kThreads = (kSmWarp0 + kSmWarps) * 32;
 constexpr int kSBufs = 3;
 constexpr uint32_t kTmemCols = 512, kOCol = kSBufs * kTile;
@@ -124,55 +124,42 @@ __global__ void __launch_bounds__(kThreads, 1)
     const long long total = r.total, lo = r.lo, count = r.count;
     const int g = r.ctas, c = blockIdx.x;
     if (count > 0) {
+        // A segment's Q into buffer b, 16 bytes per copy, in the 128-byte swizzle, by `of` warps, of which this
+        // is number `part`; rows past the unit's are left as they are (their lanes' results are never
+        // written).  Done once the copies of all the warps' lanes are waited for and fenced.
+        auto load_q = [&](const Walk<kTile> &s, int b, int part, int of) {
+            uint8_t *dst = smem + L::q + b * L::kEntry;
+            constexpr int kCh = HD / 8;  // 16-byte chunks of a row; a lane keeps its chunk
+            const int r0 = s.row0(), rows = min(s.w.sh.nodes * p.group - r0, kRows), ch = lane % kCh;
+            const char *head0 = p.q + s.w.sh.row0 * p.q_row + s.kvh() * p.group * p.q_head + ch * 16;
+#pragma unroll 1
+            for (int r = part * (32 / kCh) + lane / kCh; r < rows; r += of * (32 / kCh)) {
+                const int t = (r0 + r) / p.group, h = r0 + r - t * p.group;
+                const char *src = head0 + t * p.q_row + h * p.q_head;
+                uint8_t *at = dst + (ch >> 3) * L::kPanel + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
+                if (a.vec_q) {
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(tc::smem_u32(at)), "l"(src) : "memory");
+                } else {
+                    const uint16_t *e = reinterpret_cast<const uint16_t *>(src);
+                    uint32_t x[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) x[k] = ((uint32_t)e[2 * k] | (uint32_t)e[2 * k + 1] << 16) ^ a.q_sign;
+                    *reinterpret_cast<uint4 *>(at) = make_uint4(x[0], x[1], x[2], x[3]);
+                }
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            tc::fence_proxy_async_smem();
+            __syncwarp();
+        };
         if (warp == kProdWarp || warp == kProdWarpV) {
-            // ---------------------------------------------------------------- producers: K and Q, V
+            // ---------------------------------------------------------------- producers of K and of V
             const bool is_k = warp == kProdWarp;
             int e0 = 0, newest = -1;  // ring places of earlier segments; the latest place filled
             bool ok = true;
-            Walk<kTile> ahead = w;  // one segment ahead: whose Q is loaded next
-            int qseg = 0;
-            bool q_pending = false;
             auto wait = [&](uint64_t *bar, int phase) -> bool {
                 return __all_sync(0xffffffffu, tc::mbar_wait_bounded(bar, (uint32_t)(phase & 1), abort_flag, p.err, kErrProd,
                                                                      kTimeoutNs));
             };
-            // Q of the next segment, 16 bytes per copy, in the 128-byte swizzle; rows past the unit's
-            // are left as they are (their lanes' results are never written)
-            auto load_q = [&]() -> bool {
-                if (!ahead.next(p, a.n_seq)) return true;
-                const int b = qseg & 1;
-                if (!wait(&qempty[b], qseg / 2 - 1)) return false;
-                uint8_t *dst = smem + L::q + b * L::kEntry;
-                constexpr int kCh = HD / 8;  // 16-byte chunks of a row; a lane keeps its chunk
-                const int r0 = ahead.row0(), rows = min(ahead.w.sh.nodes * p.group - r0, kRows), ch = lane % kCh;
-                const char *head0 = p.q + ahead.w.sh.row0 * p.q_row + ahead.kvh() * p.group * p.q_head + ch * 16;
-                for (int r = lane / kCh; r < rows; r += 32 / kCh) {
-                    const int t = (r0 + r) / p.group, h = r0 + r - t * p.group;
-                    const char *src = head0 + t * p.q_row + h * p.q_head;
-                    uint8_t *at = dst + (ch >> 3) * L::kPanel + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
-                    if (a.vec_q) {
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(tc::smem_u32(at)), "l"(src) : "memory");
-                    } else {
-                        const uint16_t *e = reinterpret_cast<const uint16_t *>(src);
-                        uint32_t x[4];
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) x[k] = ((uint32_t)e[2 * k] | (uint32_t)e[2 * k + 1] << 16) ^ a.q_sign;
-                        *reinterpret_cast<uint4 *>(at) = make_uint4(x[0], x[1], x[2], x[3]);
-                    }
-                }
-                q_pending = true;
-                return true;
-            };
-            auto finish_q = [&]() {
-                if (!q_pending) return;
-                asm volatile("cp.async.wait_all;" ::: "memory");
-                tc::fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) tc::mbar_arrive(&qfull[qseg & 1]);
-                ++qseg;
-                q_pending = false;
-            };
-            if (is_k) ok = load_q();
             while (ok && w.next(p, a.n_seq)) {
                 const int T = w.te - w.tb, kvh = w.kvh();
                 const int32_t *table = p.block_table + w.seq * p.table_stride;
@@ -215,14 +202,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const int next = page_of(j + 1);
                     ok = issue(j, cur);
                     cur = next;
-                    if (is_k) {
-                        if (j > 0 || T == 1) finish_q();  // a tile's time after load_q
-                        if (ok && j == 2) ok = load_q();
-                    }
-                }
-                if (is_k) {
-                    finish_q();
-                    if (ok && T <= 2) ok = load_q();
                 }
                 e0 += 2 * T;
             }
@@ -295,8 +274,23 @@ __global__ void __launch_bounds__(kThreads, 1)
                 volatile int no_abort = 0;
                 tc::mbar_wait_bounded(drain, 0, &no_abort, p.err, kErrDrain, kTimeoutNs);
             }
+        } else if (warp == kProdWarpQ) {
+            // ---------------------------------------------------------------- producer of the next segment's Q
+            bool ok = w.next(p, a.n_seq);  // the softmax warps load the first one's
+            for (int seg = 1; ok && w.next(p, a.n_seq); ++seg) {
+                ok = __all_sync(0xffffffffu, tc::mbar_wait_bounded(&qempty[seg & 1], (uint32_t)((seg / 2 - 1) & 1), abort_flag,
+                                                                   p.err, kErrProd, kTimeoutNs));
+                if (ok) load_q(w, seg & 1, 0, 1);
+                if (ok && lane == 0) tc::mbar_arrive(&qfull[seg & 1]);
+            }
         } else if (warp >= kSmWarp0) {
             // ---------------------------------------------------------------- softmax
+            {
+                Walk<kTile> first = w;
+                if (first.next(p, a.n_seq)) load_q(first, 0, warp - kSmWarp0, kSmWarps);
+                named_bar(5, kSmWarps * 32);
+                if (threadIdx.x == kSmWarp0 * 32) tc::mbar_arrive(&qfull[0]);
+            }
             const int quad = warp & 3;                 // TMEM lanes 32 quad .. 32 quad + 31
             const int half = (warp - kSmWarp0) >> 2;   // keys [64 half, +64) of each tile, columns [HD/2 half, +HD/2) of O
             const int row = quad * 32 + lane, tid = threadIdx.x - kSmWarp0 * 32;

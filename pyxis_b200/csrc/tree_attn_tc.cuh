@@ -129,7 +129,13 @@ PYXIS_DEVINL int shares(long long total, int grid) {
     const long long most = (total + kTcMinTiles - 1) / kTcMinTiles;
     return (int)(most < grid ? most : grid);
 }
-PYXIS_DEVINL long long first_tile(long long total, int c, int g) { return total * c / g; }
+PYXIS_DEVINL long long quotient(long long a, int b) {  // a 32-bit division where it will do
+    return a >> 32 ? a / b : (long long)((unsigned)a / (unsigned)b);
+}
+PYXIS_DEVINL long long first_tile(long long total, int c, int g) {  // total c / g, g at most an SM's number
+    const long long q = quotient(total, g);
+    return q * c + (unsigned)((int)(total - q * g) * c) / (unsigned)g;
+}
 
 // The segments (a unit's tiles, or part of them) of a CTA's range, one after another.
 template <int TILE>
@@ -144,7 +150,7 @@ struct Walk {
     PYXIS_DEVINL void begin(const TreeParams &p, int seq0, long long offset, long long count) {
         seq = seq0;
         w = seq_work<TILE>(p, seq);
-        unit = (int)(offset / w.tiles);
+        unit = (int)quotient(offset, w.tiles);
         tile = (int)(offset - (long long)unit * w.tiles);
         left = count;
         first = true;
