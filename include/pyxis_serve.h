@@ -89,7 +89,8 @@ int pyxis_cuda_qk_norm_rope_dev(pyxis_cuda_ctx *ctx, const pyxis_qk_norm_rope_ar
  * tree_mask[row] set, whose keys and values are at position context_len[s] + i.  A NULL tree_mask
  * is a chain: node j attends to nodes 0 .. j.
  *   q, out  [rows][n_q_heads][head_dim], strides q_row / q_head and out_row / out_head in elements
- *   n_seq sequences, at most max_tree nodes each (1 .. 64; further nodes get no output)
+ *   n_seq sequences, at most max_tree nodes each (1 .. 64; further nodes get no output);
+ *   max_tree * n_q_heads <= 65535
  *   block_table [n_seq][table_stride] pages, table_width of them valid
  *   max_context  a bound of context_len that only plans the split of the keys over the GPU
  * out = softmax(scale * q . k) v; a row that attends to nothing is zero, rows outside

@@ -92,7 +92,7 @@ int check_tree(const pyxis_tree_attention_args *a, const pyxis_kv_pages *kv) {
     if (a->n_seq > 1 && a->table_stride < a->table_width)
         return fail(PYXIS_EINVAL, "block table rows of %zu with stride %zu", a->table_width, a->table_stride);
     if (a->table_width > (size_t)INT32_MAX) return fail(PYXIS_EINVAL, "block table too wide");
-    if ((long long)a->max_tree * a->n_q_heads > 65535ll * 2) return fail(PYXIS_EINVAL, "too many query heads");
+    if ((long long)a->max_tree * a->n_q_heads > 65535) return fail(PYXIS_EINVAL, "too many query heads");
     return PYXIS_OK;
 }
 

@@ -788,7 +788,7 @@ cudaError_t run_tree(const TreeParams &p, int row_tile, size_t n_seq, cudaStream
 TreePlan plan_tree_attention(const pyxis_tree_attention_args &a, const pyxis_kv_pages &kv, int num_sms) {
     TreePlan t;
     const long long rows = (long long)a.max_tree * (a.n_q_heads / kv.n_kv_heads);
-    const long long keys = std::max<long long>(1, std::min<long long>(a.max_context + a.max_tree,
+    const long long keys = std::max<long long>(1, std::min<long long>(std::min<long long>(a.max_context, 1ll << 40) + a.max_tree,
                                                                      (long long)a.table_width * kv.page_size));
     // bf16: few rows over few keys are done on the CUDA cores before the tensor-core kernel has started
     // its pipeline.  Measured (16 query heads, 8 kv heads of 128): 2 rows, 16 sequences of 600 positions
@@ -796,8 +796,8 @@ TreePlan plan_tree_attention(const pyxis_tree_attention_args &a, const pyxis_kv_
     // 18 against 21, of 2303 39 against 27.
     // f32: the tcgen05 kernel pays the same for 1 row as for 128 (three products of 128 rows and the
     // conversion of every key), the mma.sync kernel for each tile of 16.  16 sequences of 2303 positions:
-    // 16 rows 89 us against the tcgen05 kernel's 100, 32 rows 160 against 100, 64 rows 310 against 105;
-    // one sequence of 152: 16 rows 18 against 24, 128 rows 31 against 25.
+    // 16 rows 89 us against the tcgen05 kernel's 103, 32 rows 160 against 103, 64 rows 310 against 107;
+    // one sequence of 152: 16 rows 18 against 24, 128 rows 31 against 28.
     const bool f32 = kv.dtype == PYXIS_DTYPE_F32;
     t.tensor = f32 ? tree_attention_tc32_supported(a, kv) && rows > 16
                    : tree_attention_tc_supported(a, kv) &&

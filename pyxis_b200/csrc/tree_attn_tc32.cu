@@ -2,11 +2,11 @@
 // (include/pyxis_serve.h; tree_attn_tc.cu is the bf16 form).
 //
 // Every f32 operand is split into two fp16 terms after a scaling by a power of two (hi = fp16(x 2^e),
-// lo = fp16(x 2^e - hi), 22 significant bits; e so that the group's largest magnitude is in
-// [2^14, 2^15): a query row, a tile of K, a tile of V, as attn_tc.h has it for the prefill), and a
-// product is taken as lo.hi + hi.lo + hi.hi with f32 accumulation.  The tensor core's accumulation
-// rounds toward zero, so each chain is one tile's products, the small ones first, and the sum over
-// tiles is taken in registers with the tiles' scales.
+// lo = fp16(x 2^e - hi), 22 significant bits of the values within 2^-12 of the largest of their group: a
+// query row, a tile of K, a tile of V; a key in a tile with drafts), and a product is taken as
+// lo.hi + hi.lo + hi.hi with f32 accumulation.  The tensor core's accumulation rounds toward zero, so
+// each chain is one tile's products, the small ones first, and the sum over tiles is taken in registers
+// with the tiles' scales.
 //
 // 64 keys of K and V are 64 KB that take 2800 cycles to arrive at an SM; their products are 36 MMAs
 // (about 2000 cycles) for up to 128 rows, and Q lies in TMEM, so that they read no more of shared memory
@@ -14,8 +14,10 @@
 // warps.  The scale of a tile is taken from the tile before (with room of a factor of four), which spares
 // them a pass over it for its largest magnitude (137 -> 115 us for 16 sequences of 2303 positions and 16
 // nodes, 8 kv heads of 128), six warps instead of four 115 -> 106, loops that are not unrolled, for the
-// instruction cache's sake, 106 -> 100: a floor of 41 us at the memory's rate.  58 sequences of 1731
-// positions and 64 nodes 290 us (121).
+// instruction cache's sake, 106 -> 100: a floor of 41 us at the memory's rate.  Tiles with drafts, which
+// some rows see and others do not, must not let one draft cost another one bits: a scale for each of
+// their keys, and values out of the scale's range added in f32 (100 -> 103 us).  58 sequences of 1731
+// positions and 64 nodes 298 us (121).
 //
 // One CTA per SM takes an equal share of all units' tiles (tree_attn_tc.cuh).  Warps:
 //   0       producer: a tile's pages by TMA (one box per page) into a ring of f32 tiles, in the order
@@ -60,7 +62,10 @@ struct Smem {
     static constexpr uint32_t misc = bar + (kBars * 8 + 15) / 16 * 16;
     static constexpr uint32_t wmax = misc + 64;          // [2][kConvWarps] magnitudes
     static constexpr uint32_t scale = wmax + 64;         // [2][4]: 2^-e of K and of V of the latest tiles
-    static constexpr uint32_t red = scale + 32;          // [2][2 halves][128 rows]
+    static constexpr uint32_t aside = scale + 32;        // [4] a segment's drafts that are not in their tiles
+    static constexpr uint32_t vexp = aside + 32;         // [2][64] exponents of the values of a tile's drafts
+    static constexpr uint32_t kexp = vexp + 2 * kTile;   // [4][64] 127 - e of a tile's keys, where each has its own
+    static constexpr uint32_t red = kexp + 4 * kTile;    // [2][2 halves][128 rows]
     static constexpr uint32_t bytes = red + 2 * 2 * kRows * 4;
 };
 static_assert(Smem<128>::bytes <= 232448 && Smem<64>::bytes <= 232448, "227 KB of shared memory per CTA");
@@ -81,6 +86,8 @@ PYXIS_DEVINL void split4(float4 x, float sc, uint2 &hi, uint2 &lo) {
     hi = make_uint2(*reinterpret_cast<const uint32_t *>(&ha), *reinterpret_cast<const uint32_t *>(&hb));
     lo = make_uint2(*reinterpret_cast<const uint32_t *>(&la), *reinterpret_cast<const uint32_t *>(&lb));
 }
+// The exponent e that takes a finite magnitude (its bits) to [2^14, 2^15); 2^e and 2^-e are normal.
+PYXIS_DEVINL int scale_exp(uint32_t m) { return m ? min(141 - (int)(m >> 23), 100) : 0; }
 // The largest finite magnitude of four values, as its bits.
 PYXIS_DEVINL uint32_t magnitude(float4 x) {
     const auto bits = [](float v) {
@@ -109,8 +116,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint64_t *sfull = ofree + 2, *pfull = sfull + 2, *odone = pfull + 2;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + L::misc);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::misc + 4);
-    // [2]: 1 + the last segment of that parity with a draft's value that is not finite
-    volatile int *bad = reinterpret_cast<volatile int *>(smem + L::misc + 8);
+    // (the converters are at most two segments ahead of the softmax warps)
+    unsigned long long *aside = reinterpret_cast<unsigned long long *>(smem + L::aside);
+    uint8_t *kexp = smem + L::kexp;
+    volatile uint8_t *vexp = smem + L::vexp;
     long long &start_off = *reinterpret_cast<long long *>(smem + L::misc + 16);
     int &start_seq = *reinterpret_cast<int *>(smem + L::misc + 24);
     volatile uint32_t *wmax = reinterpret_cast<volatile uint32_t *>(smem + L::wmax);
@@ -143,7 +152,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc::mbar_init(&odone[b], 1);
         }
         *abort_flag = 0;
-        bad[0] = bad[1] = 0;
         tc::fence_mbar_init();
         tc::prefetch_tmap(&tm_k);
         tc::prefetch_tmap(&tm_v);
@@ -294,76 +302,123 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (; ok && w.next(p, a.n_seq); ++seg) {
                 const int T = w.te - w.tb;
                 const SeqShape &sh = w.w.sh;
+                if (cw == 0 && lane == 0) aside[seg & 3] = 0;  // (before the exchange that precedes any set bit)
                 auto convert = [&](int is_v, int j) -> bool {
                     const int slot = e % kRing;
                     if (!wait(&full[slot], e / kRing)) return false;
                     const long long k0 = (long long)(w.tb + j) * kTile;
                     const int valid = (int)min((long long)kTile, max(sh.total - k0, 0ll));
-                    const int drafts = (int)min((long long)valid, max(sh.ctx - k0, 0ll));  // first draft's row
+                    const int drafts = (int)min((long long)kTile, max(sh.ctx - k0, 0ll));  // first draft's row
                     // this lane's four dims of row i * kPer + sub; zero past the last key (never loaded, or
-                    // not a key), and so is a draft's value that is not finite: the rows that see the draft
-                    // get it back at the end
+                    // not a key)
                     const float4 *src = reinterpret_cast<const float4 *>(smem + L::ring + slot * L::kEntry) + lane;
-                    const bool inner = valid == kTile && (!is_v || drafts == kTile);
-                    auto edge = [&](int i) -> float4 {
-                        const int row = i * kPer + sub;
-                        if (row >= valid) return make_float4(0.f, 0.f, 0.f, 0.f);
-                        float4 x = src[i * 32];
-                        if (is_v && row >= drafts) {
-                            const bool odd = !isfinite(x.x) || !isfinite(x.y) || !isfinite(x.z) || !isfinite(x.w);
-                            if (odd) {
-                                bad[seg & 1] = seg + 1;
-                                x.x = isfinite(x.x) ? x.x : 0.f, x.y = isfinite(x.y) ? x.y : 0.f;
-                                x.z = isfinite(x.z) ? x.z : 0.f, x.w = isfinite(x.w) ? x.w : 0.f;
-                            }
-                        }
-                        return x;
-                    };
+                    auto edge = [&](int i) { return i * kPer + sub < valid ? src[i * 32] : make_float4(0.f, 0.f, 0.f, 0.f); };
                     const int buf = use[is_v] & 1;
                     if (!wait(&cempty[is_v * 2 + buf], use[is_v] / 2 - 1)) return false;
                     uint8_t *dst = smem + (is_v ? L::v : L::k) + buf * 2 * L::kTerm;
-                    // The scale is that of the tile before, which leaves a factor of 4 to fp16's largest number;
-                    // a tile that does not fit it (or is far below it) is done again with its own.
-                    for (int round = 0;; ++round) {
-                        const float sc = attn_pow2(ex[is_v]);
-                        float mf = 0.f;  // (fmaxf passes over NaN)
-                        auto put = [&](int i, float4 x) {
-                            uint2 hi, low;
-                            split4(x, sc, hi, low);
-                            const uint32_t at = swizzled(i * kPer + sub, li, L::kPanel);
-                            *reinterpret_cast<uint2 *>(dst + at) = hi;
-                            *reinterpret_cast<uint2 *>(dst + L::kTerm + at) = low;
-                            mf = fmaxf(fmaxf(fmaxf(mf, fabsf(x.x)), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
-                        };
-                        if (inner) {
-#pragma unroll 1
-                            for (int i = cw; i < kSteps; i += kConvWarps) put(i, src[i * 32]);
+                    auto put = [&](int i, float4 x, float sc) {
+                        uint2 hi, low;
+                        split4(x, sc, hi, low);
+                        const uint32_t at = swizzled(i * kPer + sub, li, L::kPanel);
+                        *reinterpret_cast<uint2 *>(dst + at) = hi;
+                        *reinterpret_cast<uint2 *>(dst + L::kTerm + at) = low;
+                    };
+                    // largest finite magnitude of the row (of all its lanes)
+                    auto row_max = [&](float4 x) {
+                        uint32_t m = magnitude(x);
+                        if constexpr (kLanes == 32) {
+                            m = __reduce_max_sync(0xffffffffu, m);
                         } else {
-#pragma unroll 1
-                            for (int i = cw; i < kSteps; i += kConvWarps) put(i, edge(i));
-                        }
-                        uint32_t m = __float_as_uint(mf);
-                        if (m == 0x7F800000u) {  // an infinity, which sets no scale: the largest finite one
-                            m = 0;
-                            for (int i = cw; i < kSteps; i += kConvWarps) m = max(m, magnitude(edge(i)));
-                        }
-                        m = __reduce_max_sync(0xffffffffu, m);
-                        if (lane == 0) {
-                            wmax[(looks & 1) * kConvWarps + cw] = m;
-                            tc::mbar_arrive(cmax);
-                        }
-                        if (!wait(cmax, looks)) return false;
 #pragma unroll
-                        for (int i = 0; i < kConvWarps; ++i) m = max(m, wmax[(looks & 1) * kConvWarps + i]);
+                            for (int o = kLanes / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+                        }
+                        return m;
+                    };
+                    int used = ex[is_v];
+                    if (drafts == kTile) {
+                        // The context, which all rows see.  The scale is that of the tile before, which leaves a
+                        // factor of 4 to fp16's largest number; a tile that does not fit it, or is far below
+                        // it, is done again with its own.
+                        for (int round = 0;; ++round) {
+                            const float sc = attn_pow2(ex[is_v]);
+                            float mf = 0.f;  // (fmaxf passes over NaN)
+#pragma unroll 1
+                            for (int i = cw; i < kSteps; i += kConvWarps) {
+                                const float4 x = src[i * 32];
+                                put(i, x, sc);
+                                mf = fmaxf(fmaxf(fmaxf(mf, fabsf(x.x)), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
+                            }
+                            uint32_t m = __float_as_uint(mf);
+                            if (m == 0x7F800000u) {  // an infinity, which sets no scale: the largest finite one
+                                m = 0;
+                                for (int i = cw; i < kSteps; i += kConvWarps) m = max(m, magnitude(src[i * 32]));
+                            }
+                            m = __reduce_max_sync(0xffffffffu, m);
+                            if (lane == 0) {
+                                wmax[(looks & 1) * kConvWarps + cw] = m;
+                                tc::mbar_arrive(cmax);
+                            }
+                            if (!wait(cmax, looks)) return false;
+#pragma unroll
+                            for (int i = 0; i < kConvWarps; ++i) m = max(m, wmax[(looks & 1) * kConvWarps + i]);
+                            ++looks;
+                            used = ex[is_v];
+                            if (m) ex[is_v] = scale_exp(m) - 1;  // [2^13, 2^14): for the next tile
+                            const float top = __uint_as_float(m) * sc;
+                            if (round > 0 || m == 0 || (top < 65504.f && top >= 1024.f)) break;
+                        }
+                    } else if (!is_v) {
+                        // Drafts, which some rows see and others do not: a scale for each key, so that none
+                        // costs another one bits.
+#pragma unroll 1
+                        for (int i = cw; i < kSteps; i += kConvWarps) {
+                            const float4 x = edge(i);
+                            const int e = scale_exp(row_max(x));
+                            put(i, x, attn_pow2(e));
+                            if (li == 0) kexp[(use[0] & 3) * kTile + i * kPer + sub] = (uint8_t)(127 - e);
+                        }
+                        used = 0;
+                    } else {
+                        // Drafts' values: one scale, that of the tile's context or else of its first finite draft,
+                        // with room for values 16 times as large.  A draft that does not fit, is less than
+                        // 1/1024 of it or not finite is set aside (zero here): the rows that see it, and no
+                        // others, get it in f32 at the end.
+                        volatile uint8_t *ve = vexp + (looks & 1) * kTile;
+#pragma unroll 1
+                        for (int i = cw; i < kSteps; i += kConvWarps) {
+                            const float4 x = edge(i);
+                            const int row = i * kPer + sub;
+                            const bool odd = !isfinite(x.x) || !isfinite(x.y) || !isfinite(x.z) || !isfinite(x.w);
+                            const unsigned odds = __ballot_sync(0xffffffffu, odd && row >= drafts) >> (sub * kLanes);
+                            const uint32_t m = row_max(x);
+                            if (li == 0) ve[row] = (odds & (0xFFFFFFFFu >> (32 - kLanes))) ? 255 : (uint8_t)(m >> 23);
+                        }
+                        __syncwarp();
+                        if (lane == 0) tc::mbar_arrive(cmax);
+                        if (!wait(cmax, looks)) return false;
                         ++looks;
-                        const float top = __uint_as_float(m) * sc;
-                        const int used = ex[is_v];
-                        if (m) ex[is_v] = attn_scale_exp(__uint_as_float(m)) - 1;  // [2^13, 2^14): for the next tile
-                        if (round > 0 || m == 0 || (top < 65504.f && top >= 1.f)) {
-                            if (cw == 0 && lane == 0) scale[is_v * 4 + (use[is_v] & 3)] = attn_pow2(-used);
-                            break;
+                        int ref = 0;
+                        unsigned fit[2];
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const int x = ve[h * 32 + lane];
+                            if (h * 32 + lane < drafts) ref = max(ref, x);
+                            fit[h] = __ballot_sync(0xffffffffu, x > 0 && x < 255);
+                        }
+                        ref = __reduce_max_sync(0xffffffffu, ref);
+                        if (ref == 0 && (fit[0] | fit[1])) ref = ve[fit[0] ? __ffs(fit[0]) - 1 : 31 + __ffs(fit[1])];
+                        used = scale_exp((uint32_t)ref << 23) - 4;  // [2^10, 2^11)
+                        const float sc = attn_pow2(used);
+#pragma unroll 1
+                        for (int i = cw; i < kSteps; i += kConvWarps) {
+                            const int row = i * kPer + sub, x = ve[row], at = x - 127 + used;  // values up to 2^(at + 1)
+                            const bool out = row >= drafts && x > 0 && (x == 255 || at > 14 || at < 1);
+                            put(i, out ? make_float4(0.f, 0.f, 0.f, 0.f) : edge(i), sc);
+                            if (out && li == 0) atomicOr(&aside[seg & 3], 1ull << (int)(k0 + row - sh.ctx));
                         }
                     }
+                    if (cw == 0 && lane == 0) scale[is_v * 4 + (use[is_v] & 3)] = attn_pow2(-used);
+                    __syncwarp();
                     if (lane == 0) tc::mbar_arrive(&empty[slot]);
                     tc::fence_proxy_async_smem();
                     __syncwarp();
@@ -419,7 +474,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     rd[half * kRows + row] = __uint_as_float(m);
                     named_bar(1 + quad, 64);
                     m = max(m, __float_as_uint(rd[(1 - half) * kRows + row]));
-                    const int ex = attn_scale_exp(__uint_as_float(m));
+                    const int ex = scale_exp(m);
                     const float sc = sign * attn_pow2(ex);
                     qscale = attn_pow2(-ex);
 #pragma unroll
@@ -487,6 +542,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                             c2 = fmaxf(c2row * scale[n & 3], 1e-37f);
                             tc::tmem_ld32(tS + (uint32_t)(half * 32), s);
                             if (tail) {
+                                const uint32_t *ke = reinterpret_cast<const uint32_t *>(kexp + (n & 3) * kTile + half * 32);
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) s[i] *= __uint_as_float((ke[i >> 2] >> (8 * (i & 3)) & 0xFFu) << 23);
                                 // bit i: the row sees key k0 + 32 half + i -- the context, and its mask's drafts
                                 const long long d0 = sh.ctx - k0 - half * 32;  // the first draft's column
                                 const int avail = (int)(sh.total - sh.ctx);
@@ -549,21 +607,23 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (active && ok && row < rows) {
                     const bool whole = w.whole();
                     const int t = (r0 + row) / p.group, h = kvh * p.group + (r0 + row) % p.group;
-                    if (bad[seg & 1] == seg + 1)  // the drafts' values that are not finite, for the rows that see them
-                        for (int d = 0; d < sh.nodes; ++d) {
-                            const long long pos = sh.ctx + d;
-                            if (!((mask >> d) & 1) || pos >= sh.total || pos < (long long)w.tb * kTile || pos >= (long long)w.te * kTile)
-                                continue;
-                            const int page = min(max(p.block_table[w.seq * p.table_stride + pos / p.page_size], 0), p.num_pages - 1);
-                            const float *v = reinterpret_cast<const float *>(p.v + page * p.page_stride +
-                                                                             (pos % p.page_size) * p.slot_stride + kvh * p.head_stride) +
-                                             half * kOH;
+                    // the drafts that were set aside, for the rows that see them
+                    for (unsigned long long rest = aside[seg & 3] & mask; rest; rest &= rest - 1) {
+                        const long long pos = sh.ctx + __ffsll((long long)rest) - 1;
+                        const int page = min(max(p.block_table[w.seq * p.table_stride + pos / p.page_size], 0), p.num_pages - 1);
+                        const long long key = page * p.page_stride + (pos % p.page_size) * p.slot_stride + kvh * p.head_stride;
+                        const float *k = reinterpret_cast<const float *>(p.k + key), *v = reinterpret_cast<const float *>(p.v + key);
+                        const float *q = reinterpret_cast<const float *>(p.q + (sh.row0 + t) * p.q_row + h * p.q_head);
+                        float x = 0.f;
+#pragma unroll 4
+                        for (int i = 0; i < HD; ++i) x = fmaf(q[i], k[i], x);
+                        const float weight = ex2(x * p.scale2 - (m_run == -INFINITY ? 0.f : m_run));
 #pragma unroll
-                            for (int i = 0; i < kOH; ++i) {
-                                const float x = v[i];
-                                if (!isfinite(x)) acc[i] += x;
-                            }
+                        for (int i = 0; i < kOH; ++i) {
+                            const float y = v[half * kOH + i];
+                            acc[i] += isfinite(y) ? weight * y : y;
                         }
+                    }
                     const long long at = ((long long)(c * 2 + (w.from_before ? 0 : 1)) * kRows + row);
                     if (whole) {
                         const float inv = l == 0.f ? 0.f : 1.f / l;

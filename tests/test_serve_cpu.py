@@ -72,6 +72,11 @@ def test_tree_arguments(kw, text):
     refused(_native.lib().pyxis_cuda_tree_attention_dev(None, C.byref(tree_args(**kw)), C.byref(pages()), None, 0, None), text)
 
 
+def test_more_rows_than_a_grid_holds_are_refused():
+    args = tree_args(max_tree=64, n_q_heads=1024, q_row=1 << 17, out_row=1 << 17)
+    refused(_native.lib().pyxis_cuda_tree_attention_dev(None, C.byref(args), C.byref(pages()), None, 0, None), "too many query heads")
+
+
 def test_page_operator_arguments():
     L, kv = _native.lib(), C.byref(pages())
     refused(L.pyxis_cuda_kv_copy_pages_dev(None, kv, None, A, 1, None), "null src")

@@ -209,7 +209,7 @@ class Tree:
                     e = e + 2.0 ** -8
                 tol = 2 * (e + (c + t) * U) * A * 1.05 + h * want.abs() * 1.05 + 1e-30
                 err = (out[lo : lo + t, head] - want).abs()
-                worst = max(worst, float((err / tol).max()))
+                worst = max(worst, float((err / tol).nan_to_num(nan=math.inf).max()))
         assert worst <= 1.0, worst
 
 
@@ -444,6 +444,60 @@ def test_tree_attention_of_very_small_and_large_values(dt, size):
         n = t.ctx[i] + t.trees[i]
         pos = np.arange(n)
         pages, slots = t.table[i][pos // t.page].astype(np.int64), pos % t.page
+        t.keys[i], t.vals[i] = t.k[pages, slots].double().cpu(), t.v[pages, slots].double().cpu()
+    t.check(t.run())
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("ctx,nodes", [(0, 6), (200, 6), (0, 20), (200, 20), (60, 64), (0, 64)])
+@pytest.mark.parametrize("size", [1e-30, 1e20, 3.3e38])
+def test_hidden_drafts_of_any_size(dt, hd, ctx, nodes, size):
+    t, clean = (Tree(40, [ctx, 77], [nodes, 3], 4, 2, hd, dt) for _ in range(2))
+    for x in (t, clean):  # every node sees its own and node 1, and nodes 2 and 5 are seen by few
+        x.mask[:nodes] = [np.uint64(1 << j | 2 | (4 if j % 5 == 0 else 0)) for j in range(nodes)]
+    for d, sign in ((2, 1.0), (5, -1.0)):
+        pos = ctx + d
+        pg, sl = int(t.table[0, pos // t.page]), pos % t.page
+        t.k[pg, sl] = sign * size
+        t.v[pg, sl] = -sign * size
+    hidden = (t.mask & np.uint64(4 | 32)) == 0
+    hidden[nodes:] = True
+    rows = torch.from_numpy(np.nonzero(hidden)[0]).cuda()
+    assert 0 < len(rows) < len(hidden)
+    want, out = clean.run(), t.run()
+    clean.check(want)
+    mixed = want.clone()
+    mixed[rows] = out[rows]
+    clean.check(mixed)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("ctx,nodes", [(0, 6), (200, 6), (0, 20), (200, 20), (60, 64), (0, 64)])
+def test_drafts_with_values_of_any_size(dt, hd, ctx, nodes):
+    t = Tree(41, [ctx, 77], [nodes, 3], 4, 2, hd, dt)
+    t.mask[5] = 1 << 5  # sees its own alone
+    for d, size in ((0, 1e3), (2, 1e20), (5, 1e-20), (3, 0.0)):
+        pos = ctx + d
+        pg, sl = int(t.table[0, pos // t.page]), pos % t.page
+        t.v[pg, sl] *= size
+        t.vals[0][pos] = t.v[pg, sl].double().cpu()
+    t.check(t.run())
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_keys_and_values_that_change_size_along_the_cache(dt):
+    # tiles of 64 keys far apart in size, up and down; the columns of V apart, too
+    t = Tree(42, [900, 320], [24, 5], 4, 2, 128, dt)
+    cols = torch.logspace(-2, 2, 128, device="cuda").to(dt)
+    for i in range(2):
+        n = t.ctx[i] + t.trees[i]
+        pos = np.arange(n)
+        pages, slots = t.table[i][pos // t.page].astype(np.int64), pos % t.page
+        f = torch.tensor([(1.0, 300.0, 1e-3, 1e4)[(x // 64) % 4] for x in pos], device="cuda").to(dt)
+        t.k[pages, slots] *= (f ** 0.25).to(dt)[:, None, None]
+        t.v[pages, slots] *= f[:, None, None] * cols
         t.keys[i], t.vals[i] = t.k[pages, slots].double().cpu(), t.v[pages, slots].double().cpu()
     t.check(t.run())
 
