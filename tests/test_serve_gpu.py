@@ -799,3 +799,73 @@ def test_a_verified_tree_continues_as_if_decoded_token_by_token(dt):
         assert torch.allclose(one[0].float(), out[j].float(), atol=tol, rtol=tol)
     one, tok, _ = step([c], [40], nxt, [40], [1], [1])
     assert torch.allclose(one.float(), after.float(), atol=tol, rtol=tol) and tok.tolist() == idx_after.tolist()
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("nodes", [5, 24])
+def test_a_captured_verify_step_replays_as_the_calls_do(dt, nodes):
+    """A padded batch of three (the last has no nodes) steps forward five times, by calls and by two
+    captured graphs in turn that share the context's workspace; lengths and accepted nodes change."""
+    g, page, hq, hkv, hd, vocab, n = torch.Generator().manual_seed(50), 16, 8, 4, 128, 3001, 3
+    rng = np.random.default_rng(nodes)
+    f, _ = px.rope_frequencies(hd, 1e6)
+    f, head = dev(f), rand(g, vocab, hq * hd, scale=0.05)
+    k0, v0 = rand(g, 2, 120, page, hkv, hd, dt=dt), rand(g, 2, 120, page, hkv, hd, dt=dt)
+    width = 38
+    table = dev(rng.permutation(120)[: n * width].reshape(n, width).astype(np.int32))
+    mask = dev(np.concatenate([tree_masks(rng, nodes) for _ in range(n)]).view(np.int64))
+    start = torch.tensor([0, nodes, 2 * nodes, 2 * nodes], dtype=torch.int32).cuda()
+    rows = n * nodes  # the last third is padding
+    qkv = rand(g, 5, rows, (hq + 2 * hkv) * hd, dt=dt)
+    uni, accepted = torch.rand(5, rows, generator=g).cuda(), torch.from_numpy(rng.integers(0, 1 << nodes, (5, n))).cuda()
+    accepted[:, 2] = 0
+    node = torch.arange(nodes, device="cuda").repeat(n)
+    seq = torch.arange(n, device="cuda").repeat_interleave(nodes)
+
+    class State:
+        def __init__(self):
+            self.k, self.v = k0.clone(), v0.clone()
+            self.ctx = torch.tensor([37, 500, 0], dtype=torch.int32).cuda()
+            self.qkv, self.uni, self.acc = torch.empty_like(qkv[0]), torch.empty_like(uni[0]), torch.empty_like(accepted[0])
+            self.q = torch.empty((rows, hq, hd), dtype=dt, device="cuda")
+            self.out, self.new = torch.zeros_like(self.q), torch.zeros_like(self.ctx)
+            self.idx, self.prob = torch.zeros(rows, dtype=torch.int32).cuda(), torch.zeros(rows).cuda()
+
+        def feed(self, i):
+            self.qkv.copy_(qkv[i]), self.uni.copy_(uni[i]), self.acc.copy_(accepted[i])
+
+        def step(self):
+            pos = (self.ctx.long()[seq] + node)
+            slots = (table[seq, pos // page].long() * page + pos % page).int()
+            slots[2 * nodes :] = -1
+            for layer in range(2):
+                px.qk_norm_rope_dev(self.qkv, pos.int(), f, hq, hkv, hd, k_pages=self.k[layer], v_pages=self.v[layer], slots=slots,
+                                    q=self.q)
+                px.tree_attention_dev(self.q, self.k[layer], self.v[layer], table, self.ctx, start, mask, max_tree=nodes, out=self.out)
+            px.sample_dev(self.out.float().reshape(rows, -1) @ head.T, self.uni, 0.8, 50, 0.95, idx=self.idx, prob=self.prob)
+            px.kv_compact_dev(self.k, self.v, table, self.ctx, self.acc, new_len=self.new)
+            self.ctx.copy_(self.new)
+
+    a, b = State(), State()
+    graphs = []
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):  # (warm-up on a state of its own)
+        w = State()
+        w.feed(0)
+        w.step()
+    side.synchronize()
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            b.step()
+        graphs.append(graph)
+    for i in range(5):
+        a.feed(i)
+        a.step()
+        b.feed(i)
+        graphs[i % 2].replay()
+        torch.cuda.synchronize()
+        for x in ("ctx", "out", "idx", "prob", "k", "v", "q"):
+            assert torch.equal(getattr(a, x), getattr(b, x)), (i, x)
+        assert (a.out[2 * nodes :] == 0).all() and int(a.ctx[2]) == 0
+    assert a.out[: 2 * nodes].isfinite().all()
