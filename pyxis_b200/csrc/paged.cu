@@ -1,6 +1,11 @@
 // paged.cu -- page copies (forks) and the compaction of accepted drafts in a paged KV cache
 // (the cache of src/kv_cache.rs:34-41 cut into pages; include/pyxis_serve.h).  Both only move
 // bytes: 16 bytes per thread and access, several accesses in flight.
+//
+// Measured (28 layers, pages of 16 positions, 8 kv heads of 128): 96 bf16 pages copied in 57 us, 6.2 TB/s
+// of reads and writes (a floor of 54.5 us at the rate of a plain copy); 2 f32 pages 4.1 us, of which a
+// launch is most.  Compaction of 64 trees of 16 nodes, bf16, 14 us for 47 MB, one tree of 64 nodes, f32,
+// 8 us: not the bytes (7 and 2 us) but the chain mask - table - rows bounds it.
 #include <algorithm>
 
 #include "common.cuh"

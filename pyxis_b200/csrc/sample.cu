@@ -22,6 +22,11 @@
 // Weights are exp() in f64 rounded to 2^-44 (less for rows of over 2^18 tokens, so that a row's sum
 // stays below 2^63): integer sums are exact in any order, so neither the atomics' order nor the
 // cluster's size changes a token, and the sums are far finer than the spacing of uniform numbers.
+//
+// Latency bounds it: a row is read once (0.6 MB: 0.1 us of the memory's time), but maximum, histogram,
+// gather and narrowing follow one another, with a cluster barrier between.  Measured, 151936 tokens: one
+// f32 row with top-p 24.5 us, 64 bf16 rows with top-k, top-p and min-p 18.4 us, with top-p alone 77 us
+// (the weights' exponentials and the histograms' shared-memory atomics).
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 

@@ -16,6 +16,13 @@
 // is HD / 32 columns of the output and the probabilities are broadcast.  Rows arrive by one bulk
 // copy each (an mbarrier per buffer): the next block's keys are under way during P V, its values
 // during Q K.
+//
+// Measured (16 query and 8 kv heads of 128, f32, pages of 16): 64 sequences of 2303 positions, one node
+// each, 198 us, 6.1 TB/s (a floor of 167 us at the rate of a plain copy): HBM bounds it up to 4 rows, its
+// arithmetic from 8; one sequence of 152 positions 8.2 us, latency.  From 9 rows the products of f32 pages
+// go to mma.sync in two tf32 terms (below; 16 rows over 16 x 2303 positions 90 us, a floor of 41: 12 warps
+// per SM, which is what their buffers leave room for, and chains of dependent MMAs), more rows and bf16
+// pages to tcgen05 (tree_attn_tc32.cu, tree_attn_tc.cu).
 #include <cuda_bf16.h>
 
 #include <algorithm>
