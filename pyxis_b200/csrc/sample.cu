@@ -96,6 +96,8 @@ struct Shared {
     u64 few[kRank], few_w[kRank];
     unsigned nfew;
     u64 found_mass, found_w, found_key;
+    double temperature, top_p, min_p, u;  // the row's parameters, read while the row arrives
+    int top_k;
 };
 
 PYXIS_DEVINL float widen(float x) { return x; }
@@ -261,13 +263,26 @@ PYXIS_DEVINL void pick_bin(const Histogram &h, const Range &in, int sh, bool by_
     __syncthreads();
 }
 
-// Ranks n <= kRank keys of s.few against one another (weights in s.few_w): thread i < n gets the
-// weight and the number of those before its own.
+// Ranks n <= kRank keys of s.few against one another (weights in s.few_w), kRankLanes threads to a key:
+// the first of them, few_owner(n), adds the weight and the number of those before it.
+constexpr int kRankLanes = kThreads / kRank;
+static_assert(kRankLanes == 4, "");
+PYXIS_DEVINL unsigned few_index() { return threadIdx.x / kRankLanes; }
+PYXIS_DEVINL bool few_owner(unsigned n) { return threadIdx.x % kRankLanes == 0 && few_index() < n; }
 PYXIS_DEVINL void rank_few(const Shared &s, unsigned n, u64 &before, unsigned &rank) {
-    if (threadIdx.x >= n) return;
-    const u64 k = s.few[threadIdx.x];
-    for (unsigned i = 0; i < n; ++i)
-        if (s.few[i] > k) before += s.few_w[i], ++rank;
+    u64 m = 0;
+    unsigned c = 0;
+    if (few_index() < n) {
+        const u64 k = s.few[few_index()];
+        for (unsigned i = threadIdx.x % kRankLanes; i < n; i += kRankLanes)
+            if (s.few[i] > k) m += s.few_w[i], ++c;
+    }
+#pragma unroll
+    for (int o = 1; o < kRankLanes; o <<= 1) {
+        m += __shfl_xor_sync(0xffffffffu, m, o);
+        c += __shfl_xor_sync(0xffffffffu, c, o);
+    }
+    before += m, rank += c;
 }
 
 // Leader: among the candidates, whose first follows ex_mass and ex_count, the element where the
@@ -311,12 +326,12 @@ PYXIS_DEVINL void locate(Shared &s, const Row &r, unsigned n, u64 ex_mass, unsig
     u64 before = s.narrow.ex_mass;
     unsigned rank = s.narrow.ex_count;
     rank_few(s, s.nfew, before, rank);
-    if (threadIdx.x < s.nfew) {
-        const u64 w = s.few_w[threadIdx.x];
+    if (few_owner(s.nfew)) {
+        const u64 w = s.few_w[few_index()];
         if (by_count ? rank == t : t >= before && t - before < w) {
             s.found_mass = before + w;
             s.found_w = w;
-            s.found_key = s.few[threadIdx.x];
+            s.found_key = s.few[few_index()];
         }
     }
     __syncthreads();
@@ -354,6 +369,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     const size_t row = blockIdx.y;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
+    if (tid == 0) {
+        s.temperature = a.temperature ? (double)a.temperature[row] : a.temperature_all;
+        s.top_k = a.top_k ? a.top_k[row] : a.top_k_all;
+        s.top_p = a.top_p ? (double)a.top_p[row] : a.top_p_all;
+        s.min_p = a.min_p ? (double)a.min_p[row] : a.min_p_all;
+        s.u = (double)a.u[row];
+    }
     // ---- this CTA's segment of the row, and the threads' maxima
     const size_t per = (a.n + ranks - 1) / ranks;
     const size_t beg = rank * per < a.n ? rank * per : a.n, end = beg + per < a.n ? beg + per : a.n;
@@ -431,7 +453,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
         }
         return;
     }
-    const double temperature = a.temperature ? (double)a.temperature[row] : a.temperature_all;
+    const double temperature = s.temperature;
     if (!(temperature > 0.0)) {  // greedy: the first maximum
         u64 best = 0, least = ~0ull;
         scan([&](const float (&x)[4], int i) {
@@ -458,10 +480,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     r.last_bin = a.last_bin;
     r.table = s.table;
     Params q;
-    q.top_k = a.top_k ? a.top_k[row] : a.top_k_all;
-    q.top_p = a.top_p ? (double)a.top_p[row] : a.top_p_all;
-    q.min_p = a.min_p ? (double)a.min_p[row] : a.min_p_all;
-    q.u = (double)a.u[row];
+    q.top_k = s.top_k;
+    q.top_p = s.top_p;
+    q.min_p = s.min_p;
+    q.u = s.u;
     // weights that min_p keeps: w >= min_p 2^shift
     const u64 least = q.min_p > 0.0 ? (u64)ceil(fmin(q.min_p, 1.0) * (double)(1ull << r.shift)) : 0;
 
@@ -522,10 +544,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
             if (n <= kRank) {  // one ranking answers all three
                 u64 w = 0, before = 0;
                 unsigned at = 0;
-                if (tid < (int)n) s.few[tid] = s.cand[tid], s.few_w[tid] = w = r.weight(value_of(s.cand[tid]));
+                if (tid < (int)n) s.few[tid] = s.cand[tid], s.few_w[tid] = r.weight(value_of(s.cand[tid]));
                 __syncthreads();
                 rank_few(s, n, before, at);
-                const bool in = tid < (int)n && (q.top_k <= 0 || at < (unsigned)q.top_k);  // top-k keeps it
+                const bool in = few_owner(n) && (q.top_k <= 0 || at < (unsigned)q.top_k);  // top-k keeps it
+                if (in) w = s.few_w[few_index()];
                 const u64 total = block_sum(in ? w : 0, s);
                 u64 kept = total;
                 if (q.min_p > 0.0) {
@@ -541,7 +564,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
                 const u64 t = q.draw_target(kept);
                 if (in && t >= before && t - before < w) {
                     s.found_w = w;
-                    s.found_key = s.few[tid];
+                    s.found_key = s.few[few_index()];
                 }
                 __syncthreads();
                 write_result(a, row, s, kept);
