@@ -321,9 +321,12 @@ class PagePool:
         return got
 
     def _drop(self, pages) -> None:
+        if len(set(pages)) < len(pages):  # (all checks first: a refusal leaves the pool as it was)
+            _fail("a page stands twice in a table")
         for p in pages:
-            if self._uses[p] <= 0:
-                _fail(f"page {p} is free already")
+            if not 0 <= p < self.num_pages or self._uses[p] <= 0:
+                _fail(f"page {p} is free already" if 0 <= p < self.num_pages else f"no page {p}")
+        for p in pages:
             self._uses[p] -= 1
             if self._uses[p] == 0:
                 self._free.append(p)

@@ -191,6 +191,18 @@ def test_pool_refuses_without_taking_pages():
     assert pool.available == 4
 
 
+def test_pool_refuses_bad_tables_without_giving_pages_back():
+    pool = px.PagePool(4, 16)
+    t = pool.allocate(48)
+    free = (set(range(4)) - set(t)).pop()
+    for bad in (t + [free], t + [t[0]], [t[0], -1], [t[0], 4]):
+        with pytest.raises(px.PyxisError):
+            pool.free(list(bad))
+        assert pool.available == 1
+    pool.free(t)
+    assert pool.available == 4
+
+
 def test_pool_refuses_to_cut_into_a_shared_page():
     pool = px.PagePool(4, 16)
     t = pool.allocate(32)
