@@ -502,6 +502,30 @@ def test_keys_and_values_that_change_size_along_the_cache(dt):
     t.check(t.run())
 
 
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_trees_over_a_cache_past_32_bit_offsets(dt):
+    hkv, hd, page = 1, 128, 64
+    num = ((1 << 32) if dt == BF16 else (1 << 31)) // (page * hd) + 40
+    k = torch.full((num, page, hkv, hd), math.nan, dtype=dt, device="cuda")
+    v = torch.full_like(k, math.nan)
+    for nodes, ctx in ((6, 700), (40, 1000), (64, 0)):  # 12, 80 and 128 rows
+        t = Tree(44, [ctx], [nodes], 2, 1, hd, dt, page)
+        table = (num - 1 - np.arange(t.table.shape[1])).astype(np.int32)[None]
+        for i, p in enumerate(t.table[0]):
+            k[int(table[0, i])], v[int(table[0, i])] = t.k[int(p)], t.v[int(p)]
+        a = t.args()
+        t.check(px.tree_attention_dev(t.q, k, v, dev(table), *a[4:], max_tree=nodes))
+    # pages copied and compacted there, too
+    far = dev(np.array([num - 3], np.int32))
+    px.kv_copy_pages_dev(k[None], v[None], far, dev(np.array([num - 30], np.int32)))
+    assert torch.equal(k[num - 30].nan_to_num(), k[num - 3].nan_to_num())
+    before = k[num - 30].clone()
+    px.kv_compact_dev(k[None], v[None], dev(np.array([[num - 30]], np.int32)), dev(np.array([10], np.int32)),
+                      dev(np.array([0b1010], np.int64)))
+    assert torch.equal(k[num - 30, 10].nan_to_num(), before[11].nan_to_num())
+    assert torch.equal(k[num - 30, 11].nan_to_num(), before[13].nan_to_num())
+
+
 # ------------------------------------------------------------------------------------------ pages
 @pytest.mark.parametrize("dt", [F32, BF16])
 @pytest.mark.parametrize("layers,size,heads,hd,order", [(1, 16, 1, 64, "nd"), (3, 16, 8, 128, "nd"), (2, 5, 3, 64, "hd"), (4, 64, 2, 128, "lay")])
