@@ -19,6 +19,7 @@ struct TreePlan {
     int row_tile;   // query rows (nodes x heads of one kv head) of a CTA
     int row_tiles;  // CTAs over the rows of one (sequence, kv head)
     int splits;     // CTAs over the keys
+    int per_sm;     // CTAs that share an SM
 };
 TreePlan plan_tree_attention(const pyxis_tree_attention_args &a, const pyxis_kv_pages &kv, int num_sms);
 size_t tree_attention_workspace(const TreePlan &p, const pyxis_tree_attention_args &a, const pyxis_kv_pages &kv,

@@ -18,7 +18,7 @@
 // during Q K.
 //
 // Measured (16 query and 8 kv heads of 128, f32, pages of 16): 64 sequences of 2303 positions, one node
-// each, 198 us, 6.1 TB/s (a floor of 167 us at the rate of a plain copy): HBM bounds it up to 4 rows, its
+// each, 194 us, 5.6 TB/s (a floor of 167 us at the rate of a plain copy): HBM bounds it up to 4 rows, its
 // arithmetic from 8; one sequence of 152 positions 8.2 us, latency.  From 9 rows the products of f32 pages
 // go to mma.sync in two tf32 terms (below; 16 rows over 16 x 2303 positions 90 us, a floor of 41: 12 warps
 // per SM, which is what their buffers leave room for, and chains of dependent MMAs), more rows and bf16
@@ -121,7 +121,8 @@ PYXIS_DEVINL void join_warps(const TreeParams &p, const SeqShape &sh, const unsi
     }
 }
 
-template <typename T, int HD, int RT>
+// PER: CTAs that share an SM.
+template <typename T, int HD, int RT, int PER>
 struct TreeCfg {
     static constexpr int kPitch = HD * (int)sizeof(T) + 16;          // bytes of a K or V row in shared memory
     static constexpr int kHalf = kBlock * kPitch;                    // a warp's K buffer (V follows)
@@ -129,16 +130,17 @@ struct TreeCfg {
     static constexpr int kWarpBytes = 2 * kHalf + RT * kPPitch * 4;
     static constexpr int kQBytes = RT * HD * 4 + RT * 8 + 16;        // q, masks, abort flag
     static constexpr int kPerWarp = kWarpBytes + RT * 8 + 16;        // and its m and l, mbarriers
-    static constexpr int kFit = (232448 - kQBytes) / kPerWarp;
-    static constexpr int kWarps = kFit < 8 ? kFit : 8;
+    static constexpr int kMost = PER == 1 ? 232448 : 115712;         // of 228 KB with 1 KB more per CTA
+    static constexpr int kFit = (kMost - kQBytes) / kPerWarp;
+    static constexpr int kWarps = kFit < 12 ? kFit : 12;
     static constexpr int kBytes = kQBytes + kWarps * kPerWarp;
     static_assert(RT * HD * 4 <= 2 * kHalf, "a warp's output fits its buffers");
-    static_assert(kBytes <= 232448, "227 KB of shared memory per CTA");
+    static_assert(kBytes <= kMost, "shared memory of an SM");
 };
 
-template <typename T, int HD, int RT>
-__global__ void __launch_bounds__(TreeCfg<T, HD, RT>::kWarps * 32) tree_attention_kernel(const TreeParams p) {
-    using C = TreeCfg<T, HD, RT>;
+template <typename T, int HD, int RT, int PER>
+__global__ void __launch_bounds__(TreeCfg<T, HD, RT, PER>::kWarps * 32) tree_attention_kernel(const TreeParams p) {
+    using C = TreeCfg<T, HD, RT, PER>;
     constexpr int kWarps = C::kWarps, kCols = HD / 32;
     extern __shared__ __align__(128) unsigned char smem[];
     float *sq = reinterpret_cast<float *>(smem + kWarps * C::kWarpBytes);  // [RT][HD], times scale2
@@ -766,11 +768,11 @@ cudaError_t run_kernel(void (*kern)(TreeParams), int threads, int smem, std::ato
     }
     return cudaSuccess;
 }
-template <typename T, int HD, int RT>
+template <typename T, int HD, int RT, int PER>
 cudaError_t run_fma(const TreeParams &p, size_t n_seq, cudaStream_t st) {
-    using C = TreeCfg<T, HD, RT>;
+    using C = TreeCfg<T, HD, RT, PER>;
     static std::atomic<uint64_t> done{0};
-    return run_kernel<T, HD>(tree_attention_kernel<T, HD, RT>, C::kWarps * 32, C::kBytes, done, p, n_seq, st);
+    return run_kernel<T, HD>(tree_attention_kernel<T, HD, RT, PER>, C::kWarps * 32, C::kBytes, done, p, n_seq, st);
 }
 template <typename T, int HD, int MT>
 cudaError_t run_mma(const TreeParams &p, size_t n_seq, cudaStream_t st) {
@@ -780,11 +782,11 @@ cudaError_t run_mma(const TreeParams &p, size_t n_seq, cudaStream_t st) {
 }
 
 template <typename T, int HD>
-cudaError_t run_tree(const TreeParams &p, int row_tile, size_t n_seq, cudaStream_t st) {
-    switch (row_tile) {
-    case 2: return run_fma<T, HD, 2>(p, n_seq, st);
-    case 4: return run_fma<T, HD, 4>(p, n_seq, st);
-    case 8: return run_fma<T, HD, 8>(p, n_seq, st);
+cudaError_t run_tree(const TreeParams &p, const TreePlan &t, size_t n_seq, cudaStream_t st) {
+    switch (t.row_tile) {
+    case 2: return t.per_sm == 1 ? run_fma<T, HD, 2, 1>(p, n_seq, st) : run_fma<T, HD, 2, 2>(p, n_seq, st);
+    case 4: return t.per_sm == 1 ? run_fma<T, HD, 4, 1>(p, n_seq, st) : run_fma<T, HD, 4, 2>(p, n_seq, st);
+    case 8: return t.per_sm == 1 ? run_fma<T, HD, 8, 1>(p, n_seq, st) : run_fma<T, HD, 8, 2>(p, n_seq, st);
     case 16: return run_mma<T, HD, 1>(p, n_seq, st);
     default: return run_mma<T, HD, 2>(p, n_seq, st);
     }
@@ -798,9 +800,10 @@ TreePlan plan_tree_attention(const pyxis_tree_attention_args &a, const pyxis_kv_
     const long long keys = std::max<long long>(1, std::min<long long>(std::min<long long>(a.max_context, 1ll << 40) + a.max_tree,
                                                                      (long long)a.table_width * kv.page_size));
     // bf16: few rows over few keys are done on the CUDA cores before the tensor-core kernel has started
-    // its pipeline.  Measured (16 query heads, 8 kv heads of 128): 2 rows, 16 sequences of 600 positions
-    // 18 us against 27, of 2303 45 against 45, 64 of 2303 162 against 113; 8 rows, 4 sequences of 600
-    // 18 against 21, of 2303 39 against 27.
+    // its pipeline.  Measured (16 query heads, 8 kv heads of 128): 2 rows, one sequence of 152 positions 8 us
+    // against 15, 16 of 600 16 against 24, of 2303 41 against 40, 64 of 600 45 against 49, of 1200 73 against
+    // 67; 4 rows, 16 of 600 19 against 25, of 1200 32 against 29; 8 rows, 4 of 600 21 against 18, 16 of 600 30
+    // against 23, of 300 18 against 21.
     // f32: the tcgen05 kernel pays the same for 1 row as for 128 (three products of 128 rows and the
     // conversion of every key), the mma.sync kernel for each tile of 16.  16 sequences of 2303 positions:
     // 16 rows 89 us against the tcgen05 kernel's 103, 32 rows 160 against 103, 64 rows 310 against 107;
@@ -808,18 +811,24 @@ TreePlan plan_tree_attention(const pyxis_tree_attention_args &a, const pyxis_kv_
     const bool f32 = kv.dtype == PYXIS_DTYPE_F32;
     t.tensor = f32 ? tree_attention_tc32_supported(a, kv) && rows > 16
                    : tree_attention_tc_supported(a, kv) &&
-                         (rows > 8 || (double)a.n_seq * kv.n_kv_heads * keys * rows * rows > 1.2e6);
+                         (rows > 4 || (double)a.n_seq * kv.n_kv_heads * keys * rows > 640e3);
     t.row_tile = 2;
     while (t.row_tile < 32 && t.row_tile < rows) t.row_tile *= 2;
     t.row_tiles = (int)((rows + t.row_tile - 1) / t.row_tile);
-    // the split that wastes least of the last wave, a split costing about 64 keys of start-up
+    // Much work: two CTAs of half the warps to an SM, so that one's start and end overlap the other's loads.
+    // Measured (8 kv heads, f32, one node): 64 sequences of 2303 positions 195 us against 197, with heads of
+    // 64 104 against 125, 20 sequences of 800 43 against 47, 4 of 40000 201 against 209; the other way round
+    // one sequence of 152 12 against 9, of 9000 30 against 27, 16 of 2303 and 2 nodes 68 against 66.
     const long long units = (long long)a.n_seq * kv.n_kv_heads * t.row_tiles;
+    t.per_sm = t.row_tile <= 8 && (units >= num_sms || (double)units * keys >= 4096.0 * num_sms) ? 2 : 1;
+    // the split that wastes least of the last wave, a split costing about 64 keys of start-up
+    const long long slots = (long long)num_sms * t.per_sm;
     const long long most = std::min<long long>(256, (keys + 255) / 256);
     double best = 0;
     t.splits = 1;
     for (long long s = 1; s <= most; ++s) {
-        const double waves = (double)((units * s + num_sms - 1) / num_sms);
-        const double cost = waves * ((double)keys / s + 64.0) + (s > 1 ? 128.0 : 0.0);
+        const double waves = (double)((units * s + slots - 1) / slots);
+        const double cost = waves * ((double)keys / s + 64.0 * t.per_sm) + (s > 1 ? 128.0 : 0.0);
         if (s == 1 || cost < best * 0.98) best = cost, t.splits = (int)s;
     }
     return t;
@@ -870,10 +879,10 @@ cudaError_t launch_tree_attention(const pyxis_tree_attention_args &a, const pyxi
     p.part_ml = (float *)workspace;
     p.part_o = p.part_ml ? p.part_ml + a.n_rows * a.n_q_heads * t.splits * 2 : nullptr;
     if (kv.dtype == PYXIS_DTYPE_F32)
-        return kv.head_dim == 128 ? run_tree<float, 128>(p, t.row_tile, a.n_seq, st)
-                                  : run_tree<float, 64>(p, t.row_tile, a.n_seq, st);
-    return kv.head_dim == 128 ? run_tree<__nv_bfloat16, 128>(p, t.row_tile, a.n_seq, st)
-                              : run_tree<__nv_bfloat16, 64>(p, t.row_tile, a.n_seq, st);
+        return kv.head_dim == 128 ? run_tree<float, 128>(p, t, a.n_seq, st)
+                                  : run_tree<float, 64>(p, t, a.n_seq, st);
+    return kv.head_dim == 128 ? run_tree<__nv_bfloat16, 128>(p, t, a.n_seq, st)
+                              : run_tree<__nv_bfloat16, 64>(p, t, a.n_seq, st);
 }
 
 }  // namespace pyxis
