@@ -387,7 +387,7 @@ PYXIS_DEVINL void mma_tf32(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
 
 constexpr int kMmaKeys = 16;  // keys of a warp's block here: small buffers, so that more warps fit an SM
 
-template <typename T, int HD, int MT>
+template <typename T, int HD, int MT, int PER>
 struct MmaCfg {
     static constexpr bool kTwo = sizeof(T) == 4;                     // operands of two tf32 terms
     static constexpr int kRows = 16 * MT, kQPitch = HD + 4;          // floats of a query row in shared memory
@@ -395,15 +395,15 @@ struct MmaCfg {
     static constexpr int kQBytes = (kTwo ? 2 : 1) * kRows * kQPitch * 4 + kRows * 8 + 16;
     static constexpr int kWarpBytes = 2 * kHalf > kRows * HD * 4 ? 2 * kHalf : kRows * HD * 4;  // K, V; then the output
     static constexpr int kPerWarp = kWarpBytes + kRows * 8 + 16;
-    static constexpr int kFit = (232448 - kQBytes) / kPerWarp;
-    static constexpr int kMost = MT == 1 ? 12 : 8;  // 168 or 255 registers a thread
+    static constexpr int kFit = ((PER == 1 ? 232448 : 115712) - kQBytes) / kPerWarp;
+    static constexpr int kMost = (MT == 1 ? 12 : 8) / PER;  // 168 or 255 registers a thread
     static constexpr int kWarps = kFit < kMost ? kFit : kMost;
     static constexpr int kBytes = kQBytes + kWarps * kPerWarp;
 };
 
-template <typename T, int HD, int MT>
-__global__ void __launch_bounds__(MmaCfg<T, HD, MT>::kWarps * 32) tree_attention_mma_kernel(const TreeParams p) {
-    using C = MmaCfg<T, HD, MT>;
+template <typename T, int HD, int MT, int PER>
+__global__ void __launch_bounds__(MmaCfg<T, HD, MT, PER>::kWarps * 32, PER) tree_attention_mma_kernel(const TreeParams p) {
+    using C = MmaCfg<T, HD, MT, PER>;
     constexpr int kWarps = C::kWarps, RT = C::kRows;
     constexpr bool kTwo = C::kTwo;
     constexpr int kTiles = kMmaKeys / 8;
@@ -774,11 +774,11 @@ cudaError_t run_fma(const TreeParams &p, size_t n_seq, cudaStream_t st) {
     static std::atomic<uint64_t> done{0};
     return run_kernel<T, HD>(tree_attention_kernel<T, HD, RT, PER>, C::kWarps * 32, C::kBytes, done, p, n_seq, st);
 }
-template <typename T, int HD, int MT>
+template <typename T, int HD, int MT, int PER>
 cudaError_t run_mma(const TreeParams &p, size_t n_seq, cudaStream_t st) {
-    using C = MmaCfg<T, HD, MT>;
+    using C = MmaCfg<T, HD, MT, PER>;
     static std::atomic<uint64_t> done{0};
-    return run_kernel<T, HD>(tree_attention_mma_kernel<T, HD, MT>, C::kWarps * 32, C::kBytes, done, p, n_seq, st);
+    return run_kernel<T, HD>(tree_attention_mma_kernel<T, HD, MT, PER>, C::kWarps * 32, C::kBytes, done, p, n_seq, st);
 }
 
 template <typename T, int HD>
@@ -787,8 +787,8 @@ cudaError_t run_tree(const TreeParams &p, const TreePlan &t, size_t n_seq, cudaS
     case 2: return t.per_sm == 1 ? run_fma<T, HD, 2, 1>(p, n_seq, st) : run_fma<T, HD, 2, 2>(p, n_seq, st);
     case 4: return t.per_sm == 1 ? run_fma<T, HD, 4, 1>(p, n_seq, st) : run_fma<T, HD, 4, 2>(p, n_seq, st);
     case 8: return t.per_sm == 1 ? run_fma<T, HD, 8, 1>(p, n_seq, st) : run_fma<T, HD, 8, 2>(p, n_seq, st);
-    case 16: return run_mma<T, HD, 1>(p, n_seq, st);
-    default: return run_mma<T, HD, 2>(p, n_seq, st);
+    case 16: return t.per_sm == 1 ? run_mma<T, HD, 1, 1>(p, n_seq, st) : run_mma<T, HD, 1, 2>(p, n_seq, st);
+    default: return t.per_sm == 1 ? run_mma<T, HD, 2, 1>(p, n_seq, st) : run_mma<T, HD, 2, 2>(p, n_seq, st);
     }
 }
 
@@ -819,8 +819,10 @@ TreePlan plan_tree_attention(const pyxis_tree_attention_args &a, const pyxis_kv_
     // Measured (8 kv heads, f32, one node): 64 sequences of 2303 positions 195 us against 197, with heads of
     // 64 104 against 125, 20 sequences of 800 43 against 47, 4 of 40000 201 against 209; the other way round
     // one sequence of 152 12 against 9, of 9000 30 against 27, 16 of 2303 and 2 nodes 68 against 66.
+    // With mma.sync (8 nodes) 64 sequences of 1200 182 against 211, 20 of 800 72 against 82, but 4 of 40000
+    // 325 against 282.
     const long long units = (long long)a.n_seq * kv.n_kv_heads * t.row_tiles;
-    t.per_sm = t.row_tile <= 8 && (units >= num_sms || (double)units * keys >= 4096.0 * num_sms) ? 2 : 1;
+    t.per_sm = units >= num_sms || (t.row_tile <= 8 && (double)units * keys >= 4096.0 * num_sms) ? 2 : 1;
     // the split that wastes least of the last wave, a split costing about 64 keys of start-up
     const long long slots = (long long)num_sms * t.per_sm;
     const long long most = std::min<long long>(256, (keys + 255) / 256);
