@@ -62,7 +62,7 @@ class _Torch:
 
     def __init__(self):
         import torch
-        self.empty, self.Tensor = torch.empty, torch.Tensor
+        self.Tensor = torch.Tensor
         self.f32, self.f64, self.i32, self.i64 = torch.float32, torch.float64, torch.int32, torch.int64
         self.masks = (torch.int64, torch.uint64)
         self.types = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16}
@@ -165,7 +165,7 @@ def qk_norm_rope_dev(qkv, positions, inv_freq, n_q_heads: int, n_kv_heads: int, 
     if kv.n_kv_heads != n_kv_heads or kv.head_dim != head_dim or k_pages.dtype is not dtype:
         _fail("the cache's heads or type differ from qkv's")
     if q is None:
-        q = T.empty((n, n_q_heads, head_dim), dtype=dtype, device=qkv.device)
+        q = qkv.new_empty(n, n_q_heads, head_dim)
         ld_q = n_q_heads * head_dim
     else:
         if q.shape != (n, n_q_heads, head_dim) or q.dtype is not dtype or q.get_device() != dev or q.stride(2) != 1 or (
@@ -200,7 +200,7 @@ def tree_attention_dev(q, k_pages, v_pages, block_table, context_len, q_start, t
         _fail("q must be [rows, n_q, head_dim] of the cache's type")
     rows, n_q, hd = shape
     if out is None:
-        out = T.empty((rows, n_q, hd), dtype=dtype, device=q.device)
+        out = q.new_empty(rows, n_q, hd)
     elif out.shape != shape or out.dtype is not dtype or out.get_device() != dev or out.stride(2) != 1:
         _fail("out must have q's shape, type and device")
     o = out.stride()
@@ -243,7 +243,7 @@ def kv_compact_dev(k_pages, v_pages, block_table, context_len, accepted, new_len
     kv = _pages(k_pages, v_pages, dev, True)
     n_seq, width = _table(block_table, "block_table", dev)
     if new_len is None:
-        new_len = T.empty(n_seq, dtype=T.i32, device=k_pages.device)
+        new_len = context_len.new_empty(n_seq)
     rc = T.compact(ctx, C.byref(kv), block_table.data_ptr(), block_table.stride(0), width,
                    _array(context_len, "context_len", T.i32, n_seq, dev), _array(accepted, "accepted", T.i64, n_seq, dev), n_seq,
                    _array(new_len, "new_len", T.i32, n_seq, dev), _stream(stream, dev))
@@ -273,9 +273,9 @@ def sample_dev(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
     params = _SampleParams(t, k, p, m, temperature if t is None else 1.0, top_k if k is None else 0, top_p if p is None else 1.0,
                            min_p if m is None else 0.0)
     if idx is None:
-        idx = T.empty(M, dtype=T.i32, device=logits.device)
+        idx = logits.new_empty(M, dtype=T.i32)
     if prob is None:
-        prob = T.empty(M, dtype=T.f32, device=logits.device)
+        prob = logits.new_empty(M, dtype=T.f32)
     rc = T.sample(ctx, logits.data_ptr(), kind, M, n, logits.stride(0), _array(uniforms, "uniforms", T.f32, M, dev), C.byref(params),
                   _array(idx, "idx", T.i32, M, dev), _array(prob, "prob", T.f32, M, dev), _stream(stream, dev))
     if rc:
