@@ -807,9 +807,13 @@ TreePlan plan_tree_attention(const pyxis_tree_attention_args &a, const pyxis_kv_
     // f32: the tcgen05 kernel pays the same for 1 row as for 128 (three products of 128 rows and the
     // conversion of every key), the mma.sync kernel for each tile of 16.  16 sequences of 2303 positions:
     // 16 rows 89 us against the tcgen05 kernel's 103, 32 rows 160 against 103, 64 rows 310 against 107;
-    // one sequence of 152: 16 rows 18 against 24, 128 rows 31 against 28.
+    // one sequence of 152: 16 rows 18 against 24, 128 rows 31 against 28.  Trees over next to no context are
+    // done before its pipeline has started: 4 sequences of 86 keys and 48 rows 23 against 25, 16 of 17 keys
+    // and 128 rows of one kv head 21 against 35; 4 of 224 keys 29 against 27, and 512 CTAs' worth, 16 of 65
+    // keys and 128 rows, 55 against 36.
     const bool f32 = kv.dtype == PYXIS_DTYPE_F32;
-    t.tensor = f32 ? tree_attention_tc32_supported(a, kv) && rows > 16
+    const bool brief = keys <= 128 && (long long)a.n_seq * kv.n_kv_heads * ((rows + 31) / 32) <= num_sms;
+    t.tensor = f32 ? tree_attention_tc32_supported(a, kv) && rows > 16 && !brief
                    : tree_attention_tc_supported(a, kv) &&
                          (rows > 4 || (double)a.n_seq * kv.n_kv_heads * keys * rows > 640e3);
     t.row_tile = 2;

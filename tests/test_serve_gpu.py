@@ -450,7 +450,7 @@ def test_tree_attention_of_very_small_and_large_values(dt, size):
 
 @pytest.mark.parametrize("dt", [F32, BF16])
 @pytest.mark.parametrize("hd", [64, 128])
-@pytest.mark.parametrize("ctx,nodes", [(0, 6), (200, 6), (0, 20), (200, 20), (60, 64), (0, 64)])
+@pytest.mark.parametrize("ctx,nodes", [(0, 6), (200, 6), (0, 20), (200, 20), (60, 64), (0, 64), (192, 20), (192, 64), (180, 64)])
 @pytest.mark.parametrize("size", [1e-30, 1e20, 3.3e38])
 def test_hidden_drafts_of_any_size(dt, hd, ctx, nodes, size):
     t, clean = (Tree(40, [ctx, 77], [nodes, 3], 4, 2, hd, dt) for _ in range(2))
@@ -474,7 +474,7 @@ def test_hidden_drafts_of_any_size(dt, hd, ctx, nodes, size):
 
 @pytest.mark.parametrize("dt", [F32, BF16])
 @pytest.mark.parametrize("hd", [64, 128])
-@pytest.mark.parametrize("ctx,nodes", [(0, 6), (200, 6), (0, 20), (200, 20), (60, 64), (0, 64)])
+@pytest.mark.parametrize("ctx,nodes", [(0, 6), (200, 6), (0, 20), (200, 20), (60, 64), (0, 64), (192, 20), (192, 64), (180, 64)])
 def test_drafts_with_values_of_any_size(dt, hd, ctx, nodes):
     t = Tree(41, [ctx, 77], [nodes, 3], 4, 2, hd, dt)
     t.mask[5] = 1 << 5  # sees its own alone
