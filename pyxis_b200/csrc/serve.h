@@ -15,7 +15,7 @@ cudaError_t launch_qk_norm_rope(const pyxis_qk_norm_rope_args &a, const pyxis_kv
 
 // How a call's keys are split over the GPU, from sizes the host knows.
 struct TreePlan {
-    bool tensor;    // on the tensor cores, which split the keys on the device
+    bool tensor;    // on the tensor cores, which split rows and keys on the device
     int row_tile;   // query rows (nodes x heads of one kv head) of a CTA
     int row_tiles;  // CTAs over the rows of one (sequence, kv head)
     int splits;     // CTAs over the keys

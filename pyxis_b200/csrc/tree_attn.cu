@@ -795,7 +795,7 @@ cudaError_t run_tree(const TreeParams &p, const TreePlan &t, size_t n_seq, cudaS
 }  // namespace
 
 TreePlan plan_tree_attention(const pyxis_tree_attention_args &a, const pyxis_kv_pages &kv, int num_sms) {
-    TreePlan t;
+    TreePlan t{false, 0, 1, 1, 1};
     const long long rows = (long long)a.max_tree * (a.n_q_heads / kv.n_kv_heads);
     const long long keys = std::max<long long>(1, std::min<long long>(std::min<long long>(a.max_context, 1ll << 40) + a.max_tree,
                                                                      (long long)a.table_width * kv.page_size));
@@ -816,6 +816,7 @@ TreePlan plan_tree_attention(const pyxis_tree_attention_args &a, const pyxis_kv_
     t.tensor = f32 ? tree_attention_tc32_supported(a, kv) && rows > 16 && !brief
                    : tree_attention_tc_supported(a, kv) &&
                          (rows > 4 || (double)a.n_seq * kv.n_kv_heads * keys * rows > 640e3);
+    if (t.tensor) return t;
     t.row_tile = 2;
     while (t.row_tile < 32 && t.row_tile < rows) t.row_tile *= 2;
     t.row_tiles = (int)((rows + t.row_tile - 1) / t.row_tile);
@@ -829,7 +830,9 @@ TreePlan plan_tree_attention(const pyxis_tree_attention_args &a, const pyxis_kv_
     t.per_sm = units >= num_sms || (t.row_tile <= 8 && (double)units * keys >= 4096.0 * num_sms) ? 2 : 1;
     // the split that wastes least of the last wave, a split costing about 64 keys of start-up
     const long long slots = (long long)num_sms * t.per_sm;
-    const long long most = std::min<long long>(256, (keys + 255) / 256);
+    // (partial sums are kept by query row: not more of them than 256 MB, however long the buffer of rows is)
+    const double split_bytes = std::max(1.0, (double)a.n_rows * a.n_q_heads * (kv.head_dim + 2) * 4);
+    const long long most = std::min({256ll, (keys + 255) / 256, std::max(1ll, (long long)(268435456.0 / split_bytes))});
     double best = 0;
     t.splits = 1;
     for (long long s = 1; s <= most; ++s) {

@@ -526,6 +526,23 @@ def test_trees_over_a_cache_past_32_bit_offsets(dt):
     assert torch.equal(k[num - 30, 11].nan_to_num(), before[13].nan_to_num())
 
 
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_few_nodes_in_a_long_buffer_of_rows(dt):
+    t = Tree(45, [9000], [2], 8, 4, 64, dt)
+    a = t.args()
+    q = torch.zeros((200000, 8, 64), dtype=dt, device="cuda")
+    q[150000:150002] = t.q
+    mask = torch.zeros(200000, dtype=torch.int64, device="cuda")
+    mask[150000:150002] = a[6]
+    free = torch.cuda.mem_get_info()[0]
+    out = torch.full_like(q, 2.0)
+    px.tree_attention_dev(q, *a[1:5], a[5] + 150000, mask, max_tree=2, out=out)
+    torch.cuda.synchronize()
+    assert free - torch.cuda.mem_get_info()[0] < 2 << 30
+    t.check(out[150000:150002])
+    assert (out[:150000] == 2).all() and (out[150002:] == 2).all()
+
+
 # ------------------------------------------------------------------------------------------ pages
 @pytest.mark.parametrize("dt", [F32, BF16])
 @pytest.mark.parametrize("layers,size,heads,hd,order", [(1, 16, 1, 64, "nd"), (3, 16, 8, 128, "nd"), (2, 5, 3, 64, "hd"), (4, 64, 2, 128, "lay")])
