@@ -732,18 +732,39 @@ __global__ void __launch_bounds__(256) tree_join_kernel(const TreeParams p) {
     const int t = item / p.n_q, head = item % p.n_q;
     if (t >= sh.nodes) return;
     const long long row = sh.row0 + t, at = (row * p.n_q + head) * p.splits;
-    float m = -INFINITY;
-    for (int s = lane; s < p.splits; s += 32) m = fmaxf(m, p.part_ml[(at + s) * 2]);
+    // a batch of the splits' sums in flight at a time: one latency each, not one per split (one tree of 8
+    // nodes over 26000 f32 positions, 102 splits: 43 us with four, 35 with sixteen)
+    constexpr int kBatch = 16;
+    float o[kCols] = {}, l = 0.f, m = -INFINITY;
+    for (int s0 = 0; s0 < p.splits; s0 += kBatch) {
+        float2 ml[kBatch], x[kBatch][kCols / 2];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float base = m == -INFINITY ? 0.f : m;
-    float o[kCols] = {}, l = 0.f;
-#pragma unroll 4
-    for (int s = 0; s < p.splits; ++s) {
-        const float f = exp2f(p.part_ml[(at + s) * 2] - base);
-        l = fmaf(f, p.part_ml[(at + s) * 2 + 1], l);
+        for (int k = 0; k < kBatch; ++k) {
+            const bool there = s0 + k < p.splits;
+            ml[k] = there ? reinterpret_cast<const float2 *>(p.part_ml)[at + s0 + k] : make_float2(-INFINITY, 0.f);
 #pragma unroll
-        for (int c = 0; c < kCols; ++c) o[c] = fmaf(f, p.part_o[(at + s) * HD + lane * kCols + c], o[c]);
+            for (int c = 0; c < kCols / 2; ++c)
+                x[k][c] = there ? reinterpret_cast<const float2 *>(p.part_o + (at + s0 + k) * HD + lane * kCols)[c]
+                                : make_float2(0.f, 0.f);
+        }
+        float top = m;
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) top = fmaxf(top, ml[k].x);
+        const float base = top == -INFINITY ? 0.f : top, old = exp2f(m - base);
+        m = top;
+        l *= old;
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) o[c] *= old;
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+            const float f = exp2f(ml[k].x - base);
+            l = fmaf(f, ml[k].y, l);
+#pragma unroll
+            for (int c = 0; c < kCols / 2; ++c) {
+                o[2 * c] = fmaf(f, x[k][c].x, o[2 * c]);
+                o[2 * c + 1] = fmaf(f, x[k][c].y, o[2 * c + 1]);
+            }
+        }
     }
     T *dst = reinterpret_cast<T *>(p.out + row * p.out_row + head * p.out_head) + lane * kCols;
 #pragma unroll
@@ -822,22 +843,24 @@ TreePlan plan_tree_attention(const pyxis_tree_attention_args &a, const pyxis_kv_
     t.row_tiles = (int)((rows + t.row_tile - 1) / t.row_tile);
     // Much work: two CTAs of half the warps to an SM, so that one's start and end overlap the other's loads.
     // Measured (8 kv heads, f32, one node): 64 sequences of 2303 positions 195 us against 197, with heads of
-    // 64 104 against 125, 20 sequences of 800 43 against 47, 4 of 40000 201 against 209; the other way round
+    // 64 104 against 125, 20 sequences of 800 39 against 47, 4 of 40000 199 against 209; the other way round
     // one sequence of 152 12 against 9, of 9000 30 against 27, 16 of 2303 and 2 nodes 68 against 66.
-    // With mma.sync (8 nodes) 64 sequences of 1200 182 against 211, 20 of 800 72 against 82, but 4 of 40000
+    // With mma.sync (8 nodes) 64 sequences of 1200 182 against 211, 20 of 800 67 against 82, but 4 of 40000
     // 325 against 282.
     const long long units = (long long)a.n_seq * kv.n_kv_heads * t.row_tiles;
     t.per_sm = units >= num_sms || (t.row_tile <= 8 && (double)units * keys >= 4096.0 * num_sms) ? 2 : 1;
-    // the split that wastes least of the last wave, a split costing about 64 keys of start-up
+    // the split that wastes least of the last wave, a split costing about 32 KB of f32 keys of start-up (20
+    // sequences of 800 43 -> 39 us with that instead of 64 KB for two CTAs per SM), 64 or 128 bf16 ones
     const long long slots = (long long)num_sms * t.per_sm;
     // (partial sums are kept by query row: not more of them than 256 MB, however long the buffer of rows is)
     const double split_bytes = std::max(1.0, (double)a.n_rows * a.n_q_heads * (kv.head_dim + 2) * 4);
     const long long most = std::min({256ll, (keys + 255) / 256, std::max(1ll, (long long)(268435456.0 / split_bytes))});
+    const double start = f32 ? 64.0 * 128 / kv.head_dim : 64.0 * t.per_sm;
     double best = 0;
     t.splits = 1;
     for (long long s = 1; s <= most; ++s) {
         const double waves = (double)((units * s + slots - 1) / slots);
-        const double cost = waves * ((double)keys / s + 64.0 * t.per_sm) + (s > 1 ? 128.0 : 0.0);
+        const double cost = waves * ((double)keys / s + start) + (s > 1 ? 128.0 : 0.0);
         if (s == 1 || cost < best * 0.98) best = cost, t.splits = (int)s;
     }
     return t;
