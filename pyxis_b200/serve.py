@@ -192,7 +192,9 @@ def tree_attention_dev(q, k_pages, v_pages, block_table, context_len, q_start, t
     or uint64 [rows]; None: drafts 0 .. j) at positions ``context_len[s]`` + i of the pages in
     ``block_table`` [sequences, width].  ``max_context`` bounds the contexts, for the split of the work
     (default: what the table holds); ``scale`` defaults to 1 / sqrt(head_dim).  Rows outside every
-    sequence are left as they are (in a new ``out``: uninitialised)."""
+    sequence are left as they are (in a new ``out``: uninitialised).  Partial sums lie in the device
+    context's memory, so calls without a ``workspace`` must not overlap on the GPU; a call that may
+    overlap others brings its own (256-byte aligned; one too small is refused with the size needed)."""
     T, dev, ctx = _begin(q)
     kv = _pages(k_pages, v_pages, dev, False)
     shape, s, dtype = q.shape, q.stride(), q.dtype
