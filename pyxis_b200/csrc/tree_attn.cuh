@@ -43,6 +43,39 @@ PYXIS_DEVINL SeqShape seq_shape(const TreeParams &p, int seq) {
 PYXIS_DEVINL void store(float *p, float x) { *p = x; }
 PYXIS_DEVINL void store(__nv_bfloat16 *p, float x) { *p = __float2bfloat16_rn(x); }
 
+// The sum of the values that are not finite in one column of a kv head (its address in page 0), over those of
+// the positions a .. b - 1 of a sequence with these pages that a row with this mask sees: infinite or NaN, or 0
+// if there are none.  Products in several terms need it (a weight's second term may be zero or negative, and an
+// infinite value has none); nothing else calls it, so it stays out of the kernels' registers.
+template <typename T>
+__device__ __noinline__ float odd_values(const char *column, const int32_t *pages, int num_pages, int page_size,
+                                         long long page_stride, long long slot_stride, long long ctx, unsigned long long mask,
+                                         long long a, long long b) {
+    float sum = 0.f;
+    for (; a < b; ++a) {
+        if (a >= ctx && !((mask >> (a - ctx)) & 1)) continue;
+        const long long i = a / page_size;
+        const int page = min(max(pages[i], 0), num_pages - 1);
+        const float x = (float)*reinterpret_cast<const T *>(column + page * page_stride + (a - i * page_size) * slot_stride);
+        if (!isfinite(x)) sum += x;
+    }
+    return sum;
+}
+template <typename T>
+PYXIS_DEVINL float odd_values(const TreeParams &p, const SeqShape &sh, int seq, int kvh, int d, unsigned long long mask, long long a,
+                              long long b) {
+    return odd_values<T>(p.v + kvh * p.head_stride + d * (int)sizeof(T), p.block_table + seq * p.table_stride, p.num_pages,
+                         p.page_size, p.page_stride, p.slot_stride, sh.ctx, mask, a, min(b, sh.total));
+}
+// 0, or NaN if one of the values is not finite.
+template <int N>
+PYXIS_DEVINL float odd_mark(const float (&x)[N]) {
+    float z[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < N; ++i) z[i & 1] = fmaf(x[i], 0.f, z[i & 1]);
+    return z[0] + z[1];
+}
+
 // The tensor-core forms, bf16 and f32 pages of sizes that tile their blocks of keys: whether one takes
 // the call, its workspace, its launch.
 bool tree_attention_tc_supported(const pyxis_tree_attention_args &a, const pyxis_kv_pages &kv);

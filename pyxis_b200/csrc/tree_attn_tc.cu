@@ -4,7 +4,7 @@
 //
 // The rows of one (sequence, kv head) -- its nodes times the query heads that share the kv head --
 // are the 128 TMEM lanes of a unit, so the cache is read once for all of them and the arithmetic of
-// up to 128 rows (two 128 x 128 x HD products per 128 keys, about 1000 tensor cycles) stays below the
+// up to 128 rows (three 128 x 128 x HD products per 128 keys, about 1600 tensor cycles) stays below the
 // time those keys take to arrive (64 KB per SM: about 2800 cycles): HBM bounds it.  Rows that are
 // not there cost nothing but tensor cycles that are idle anyway.
 //
@@ -18,13 +18,15 @@
 //   producers  a tile's pages by TMA (one box per page, 128-byte swizzle) through a ring of tiles in the
 //              order S_0, S_1, O_0, S_2, O_1, ... of the MMAs; the next segment's Q rows by cp.async while
 //              the current one runs (the first segment's, which everything waits for, by the softmax warps)
-//   MMA        S_j into one of three TMEM buffers; O += P_j V_j with P_j from TMEM and V_j as an
-//              MN-major operand, as it lies in the cache
+//   MMA        S_j into one of three TMEM buffers; O += lo(P_j) V_j + hi(P_j) V_j with P_j from TMEM and
+//              V_j as an MN-major operand, as it lies in the cache
 //   softmax    reads S_j, masks the tiles that hold drafts or end inside, writes P_j over S_j.  The
 //              running maximum is raised only when a tile exceeds it by more than 2^8 (then the row
 //              of O in TMEM is rescaled); O / l does not depend on it.
-// P is rounded to bf16 (2^-9 of each weight), and l sums the rounded weights, so that rounding
-// changes the weights' proportions, never their sum.
+// P is two bf16 terms, hi = bf16(p) and lo = bf16(p - hi), which leaves 2^-16 of each weight at most: O is
+// f32 until its one rounding, as in the forms on the CUDA cores.  The tensor cores have the time for the
+// second product (1600 of the 2800 cycles that a tile takes to arrive), and TMEM the room: both terms lie
+// over the scores.
 //
 // Measured (16 query and 8 kv heads of 128): one sequence of 131000 positions and 64 nodes 107 us, 5.0 TB/s
 // (a floor of 83 us), 16 sequences of 2303 positions and 16 nodes 40 us (20): the tiles pass at HBM's rate;
@@ -253,9 +255,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const uint32_t tS = tmem_base + (uint32_t)(ob * kTile);
                     const uint64_t vd = v_d + (uint64_t)(slot * (L::kEntry >> 4));
 #pragma unroll
-                    for (int kk = 0; kk < kTile / 16; ++kk)  // 16 keys: 8 columns of P, 16 rows of V
-                        tc::mma_f16_ts(tO, tS + (uint32_t)(kk * 8), vd + (uint64_t)(kk * (2 * L::kGroup >> 4)), idesc_o,
-                                       (uint32_t)(add || kk > 0));
+                    for (int kk = 0; kk < kTile / 8; ++kk)  // 16 keys: 8 columns of P, 16 rows of V; lo, then hi
+                        tc::mma_f16_ts(tO, tS + (uint32_t)((kk ^ (kTile / 16)) * 8),
+                                       vd + (uint64_t)(kk % (kTile / 16) * (2 * L::kGroup >> 4)), idesc_o, (uint32_t)(add || kk > 0));
                     tc::mma_commit(&empty[slot]);
                     tc::mma_commit(&odone[ob]);
                     if (++slot == kRing) slot = 0, ++fills;
@@ -420,16 +422,19 @@ __global__ void __launch_bounds__(kThreads, 1)
                         float2 sum[2];
 #pragma unroll
                         for (int ch = 0; ch < 2; ++ch) {
-                            uint32_t pk[16];
+                            uint32_t hi[16], low[16];
                             sum[ch] = f2(0.f, 0.f);
 #pragma unroll
                             for (int i = 0; i < 32; i += 2) {
-                                const float2 y = ffma2(f2(s[ch][i], s[ch][i + 1]), c22, base2);
-                                const uint32_t u = pack_bf16(ex2(y.x), ex2(y.y));
-                                pk[i / 2] = u;
-                                sum[ch] = fadd2(sum[ch], f2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u)));
+                                const float2 y = ffma2(f2(s[ch][i], s[ch][i + 1]), c22, base2), e = f2(ex2(y.x), ex2(y.y));
+                                const uint32_t u = pack_bf16(e.x, e.y);
+                                const float2 rest = ffma2(f2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u)), f2(-1.f, -1.f), e);
+                                hi[i / 2] = u;
+                                low[i / 2] = pack_bf16(rest.x, rest.y);
+                                sum[ch] = fadd2(sum[ch], e);
                             }
-                            tmem_st16(tS + (uint32_t)(half * 32 + ch * 16), pk);
+                            tmem_st16(tS + (uint32_t)(half * 32 + ch * 16), hi);
+                            tmem_st16(tS + (uint32_t)(kTile / 2 + half * 32 + ch * 16), low);
                         }
                         sum[0] = fadd2(sum[0], sum[1]);
                         l += sum[0].x + sum[0].y;
@@ -484,6 +489,22 @@ __global__ void __launch_bounds__(kThreads, 1)
                         } else if (row < rows) {
 #pragma unroll
                             for (int i = 0; i < 32; ++i) part[(ch * 32 + i) * kRows] = o[i];
+                        }
+                        if (row < rows && isnan(odd_mark(o))) {
+                            // a weight's second term may be zero or negative: a sum over values that are not
+                            // finite is taken from the values (read back: o stays in registers)
+#pragma unroll 1
+                            for (int d = ch * 32; d < ch * 32 + 32; ++d) {
+                                __nv_bfloat16 *y = reinterpret_cast<__nv_bfloat16 *>(dst) + d;
+                                if (isfinite(whole ? __bfloat162float(*y) : part[d * kRows])) continue;
+                                const float x = odd_values<__nv_bfloat16>(p, sh, w.seq, kvh, d, mask, (long long)w.tb * kTile,
+                                                                          (long long)w.te * kTile);
+                                if (x == 0.f) continue;
+                                if (whole)
+                                    store(y, x);
+                                else
+                                    part[d * kRows] = x;
+                            }
                         }
                         __syncwarp();  // tcgen05.ld is the whole warp's
                     }
