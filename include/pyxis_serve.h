@@ -50,8 +50,13 @@ typedef struct {
  *   LINEAR  those / factor                           (positions divided by factor)
  *   NTK     theta * factor^(rotary_dim / (rotary_dim - 2)) in theta's place
  *   YARN    plain / factor where the frequency turns less than beta_slow times over
- *           original_context positions, plain where it turns more than beta_fast times, a linear
- *           ramp over the index between them; *scale = 0.1 ln(factor) + 1
+ *           original_context positions, plain where it turns more than beta_fast times, a mixture
+ *           between them: with r = clamp((i - low) / (high - low), 0, 1),
+ *             freq[i] = plain (1 - r) + plain / factor r,
+ *             low = max(0, floor(at(beta_fast))), high = min(rotary_dim - 1, ceil(at(beta_slow))),
+ *             at(b) = rotary_dim ln(original_context / (2 pi b)) / (2 ln theta), the index of the
+ *             frequency that turns b times (which may lie past the last one)
+ *           (high <= low: plain up to low, plain / factor after it); *scale = 0.1 ln(factor) + 1
  * rotary_dim is even and positive, theta > 0, factor >= 1, and for YARN original_context > 0 and
  * beta_fast > beta_slow > 0 (others ignore those). */
 enum { PYXIS_ROPE_PLAIN = 0, PYXIS_ROPE_LINEAR = 1, PYXIS_ROPE_NTK = 2, PYXIS_ROPE_YARN = 3 };

@@ -123,7 +123,7 @@ int pyxis_rope_frequencies(int kind, double theta, int rotary_dim, double factor
             return rotary_dim * std::log(original_context / (beta * 6.283185307179586477)) / (2.0 * std::log(theta));
         };
         low = std::max(0.0, std::floor(index(beta_fast)));
-        high = std::max(low, std::min((double)(n - 1), std::ceil(index(beta_slow))));
+        high = std::max(low, std::min(rotary_dim - 1.0, std::ceil(index(beta_slow))));  // (past the last index, n - 1, too)
     }
     for (int i = 0; i < n; ++i) {
         const double f = std::pow(theta, -2.0 * i / rotary_dim);
