@@ -4,7 +4,10 @@
 // Every f32 operand is split into two fp16 terms after a scaling by a power of two (hi = fp16(x 2^e),
 // lo = fp16(x 2^e - hi), 22 significant bits of the values within 2^-12 of the largest of their group: a
 // query row, a tile of K, a tile of V; a key in a tile with drafts), and a product is taken as
-// lo.hi + hi.lo + hi.hi with f32 accumulation.  The tensor core's accumulation rounds toward zero, so
+// lo.hi + hi.lo + hi.hi with f32 accumulation.  Weights are taken in units of their row's largest in the
+// tile, which becomes 2^15: fp16 leaves 2^-40 of that, so that light keys keep their bits however heavy a
+// key of another tile is (in units of the running maximum the weights below 2^-25 of it would be lost:
+// 40000 of them behind a key 17 nats above, a part in 800 of the sum).  The tensor core's accumulation rounds toward zero, so
 // each chain is one tile's products, the small ones first, and the sum over tiles is taken in registers
 // with the tiles' scales.
 //
@@ -45,7 +48,7 @@ constexpr int kRegsLaunch = 128, kRegsFew = 88, kRegsSoft = 160;
 static_assert(2 * kRegsFew + 2 * kRegsSoft <= 4 * kRegsLaunch - 16, "register split");
 constexpr uint32_t kTmemCols = 512, kOCol = 2 * kTile, kQCol = kOCol + 2 * 128;  // S twice, O twice, Q hi and lo
 constexpr uint64_t kTimeoutNs = 2000000000ull;
-constexpr float kRaise = 11.0f;  // weights up to 2^11 stay in fp16's range
+constexpr float kTop = 15.0f;  // a tile's largest weight is 2^15, in fp16's range
 enum { kErrProd = 0x721, kErrMma = 0x722, kErrConv = 0x723, kErrSoft = 0x724, kErrDrain = 0x725, kErrAlign = 0x726 };
 
 template <int HD>
@@ -501,15 +504,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 const float c2row = fabsf(p.scale2) * qscale;
                 float m_run = -INFINITY, l = 0.f;
+                float unit = 0.f;  // the tile before's unit of weight, 2^(its maximum - kTop), in terms of 2^m_run
                 float acc[kOH];
 #pragma unroll
                 for (int i = 0; i < kOH; ++i) acc[i] = 0.f;
-                // (O + acc) of tile m into acc, then times alpha
+                // (O unit + acc) of tile m into acc, then times alpha
                 auto fold = [&](int m, float alpha) -> bool {
                     if (!wait(&odone[m & 1], m / 2)) return false;
                     if (active) {
                         tc::tc_fence_after();
-                        const float vs = scale[4 + (m & 3)];
+                        const float vs = scale[4 + (m & 3)] * unit;
 #pragma unroll
                         for (int ch = 0; ch < kOH / 32; ++ch) {
                             uint32_t o[32];
@@ -532,7 +536,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const uint32_t tS = tq + (uint32_t)(b * kTile);
                     const bool tail = k0 + kTile > sh.ctx;
                     ok = ok && wait(&sfull[b], n / 2);
-                    float alpha = 1.f;
+                    float alpha = 1.f, next_unit = 0.f;
                     if (active) {
                         float s[32];
                         float mt = -INFINITY, c2 = 0.f;
@@ -565,14 +569,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                         rd[half * kRows + row] = mt;
                         named_bar(1 + quad, 64);
                         mt = fmaxf(mt, rd[(1 - half) * kRows + row]);
-                        const bool raise = mt > m_run + kRaise || (m_run == -INFINITY && mt > m_run);
-                        if (raise) {
-                            alpha = ex2(m_run - mt);
-                            m_run = mt;
-                            l *= alpha;
-                        }
+                        const float m_new = fmaxf(m_run, mt);
+                        alpha = mt > m_run ? ex2(m_run - mt) : 1.f;
+                        next_unit = mt == -INFINITY ? 0.f : ex2(mt - m_new - kTop);
+                        m_run = m_new;
                         if (ok) {
-                            const float base = m_run == -INFINITY ? 0.f : m_run;
+                            const float base = mt == -INFINITY ? 0.f : mt - kTop;
                             uint32_t ph[16], pl[16];
                             float sum = 0.f;
 #pragma unroll
@@ -585,7 +587,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 ph[i] = *reinterpret_cast<const uint32_t *>(&h);
                                 pl[i] = *reinterpret_cast<const uint32_t *>(&q);
                             }
-                            l += sum;
+                            l = fmaf(sum, next_unit, l * alpha);
                             tmem_st16(tS + (uint32_t)(half * 16), ph);
                             tmem_st16(tS + (uint32_t)(kTile / 2 + half * 16), pl);
                             tc::tmem_wait_st();
@@ -596,6 +598,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (lane == 0) tc::mbar_arrive(&pfull[b]);
                     // the previous tile's P V, at the previous maximum, then this tile's rescale
                     if (j > 0) ok = ok && fold(n - 1, alpha);
+                    unit = next_unit;
                 }
                 ok = ok && fold(n - 1, 1.0f);
                 if (active) {  // the row sum of both halves

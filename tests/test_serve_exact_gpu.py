@@ -56,3 +56,37 @@ def test_bf16_weights_are_not_rounded_to_bf16(ctx, trees, hq, hkv, hd, page):
         tol = 2 * (e + n * U) * A * 1.05 + half_step(BF16) * want.abs() * 1.05 + 1e-30
         worst = max(worst, float(((out[rows, head] - want).abs() / tol).nan_to_num(nan=math.inf).max()))
     assert worst <= 1.0, worst
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("nodes", [2, 6, 24, 64])  # a form of the f32 kernels each
+@pytest.mark.parametrize("gap", [12.0, 17.25, 24.0])
+def test_many_light_keys_behind_a_heavy_one(dt, hd, nodes, gap):
+    """One key far above all others, whose weights (2^-17, 2^-24.9, 2^-34.6 of its own) are small, many and
+    alike: each of them has to keep its bits, as their sum is a part in 10^1 to 10^6 of the result."""
+    ctx = 40000
+    t = Tree(52, [ctx], [nodes], 2, 1, hd, dt)
+    pos = np.arange(ctx + nodes)
+    pages, slots = dev(t.table[0][pos // t.page].astype(np.int64)), dev(pos % t.page)
+    t.q.zero_()
+    t.q[..., 0] = 4.0
+    k, v = t.keys[0], t.vals[0].abs()
+    k[:, :, 0] = 0.0
+    k[0, :, 0] = 2 * gap  # exact in bf16; times q's 4 and the scale: the gap
+    v[0] = 2.0 ** -14    # so that the light keys' part is seen beside the heavy one's
+    t.k[pages, slots], t.v[pages, slots] = k.to(dt).cuda(), v.to(dt).cuda()
+    t.vals[0] = v
+    out = t.run(scale=0.125).double().cpu()
+    seen = np.concatenate([np.ones((nodes, ctx)), ((t.mask[:, None] >> np.arange(nodes, dtype=np.uint64)) & np.uint64(1)).astype(float)], 1)
+    w = torch.from_numpy(seen)
+    w[:, 1:] *= math.exp(-gap)
+    num, den = w @ t.vals[0][:, 0], w.sum(1, keepdim=True)
+    # The score is one product: q, its scale in log2 units and the product round, 4 u of 1.44 gap; exp2 2 u;
+    # two terms of a weight leave 2^-22 (f32 pages) or 2^-16 (bf16) of it; values of two terms 2^-22.  Sums
+    # run over at most 64 keys a tile, then over the ctx / 64 tiles (in halves of a row, of a tensor-core
+    # accumulation that cuts off: 2 u an addition), numerator and sum both.  All values are positive.
+    e = 4 * U * 1.45 * gap + 2 * U + (2.0 ** -21 if dt == F32 else 2.0 ** -16) + 2 * (2 * U * (64 + ctx / 64))
+    want = num / den
+    bad = (out - want[:, None]).abs() / want[:, None] / (e * 1.05 + half_step(dt) * 1.05)
+    assert bad.max() <= 1.0, bad.max()
