@@ -76,6 +76,25 @@ PYXIS_DEVINL float odd_mark(const float (&x)[N]) {
     return z[0] + z[1];
 }
 
+// q . k of the key at a position of an f32 cache (its head's address in page 0), in f32: for keys that
+// products in several terms cannot take.
+template <int HD>
+__device__ __noinline__ float key_score(const float *q, const char *head, const int32_t *pages, int num_pages, int page_size,
+                                        long long page_stride, long long slot_stride, long long pos) {
+    const long long i = pos / page_size;
+    const float *k = reinterpret_cast<const float *>(head + min(max(pages[i], 0), num_pages - 1) * page_stride +
+                                                     (pos - i * page_size) * slot_stride);
+    float x = 0.f;
+#pragma unroll 4
+    for (int d = 0; d < HD; ++d) x = fmaf(q[d], k[d], x);
+    return x;
+}
+template <int HD>
+PYXIS_DEVINL float key_score(const TreeParams &p, const float *q, int seq, int kvh, long long pos) {
+    return key_score<HD>(q, p.k + kvh * p.head_stride, p.block_table + seq * p.table_stride, p.num_pages, p.page_size,
+                         p.page_stride, p.slot_stride, pos);
+}
+
 // The tensor-core forms, bf16 and f32 pages of sizes that tile their blocks of keys: whether one takes
 // the call, its workspace, its launch.
 bool tree_attention_tc_supported(const pyxis_tree_attention_args &a, const pyxis_kv_pages &kv);

@@ -83,6 +83,16 @@ PYXIS_DEVINL void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
         : "memory");
 }
 
+// One column of this warp's 32 TMEM lanes (the store complete after tmem_wait_st).
+PYXIS_DEVINL float tmem_ld1(uint32_t taddr) {
+    uint32_t r;
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n tcgen05.wait::ld.sync.aligned;" : "=r"(r) : "r"(taddr) : "memory");
+    return __uint_as_float(r);
+}
+PYXIS_DEVINL void tmem_st1(uint32_t taddr, float x) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(taddr), "r"(__float_as_uint(x)) : "memory");
+}
+
 PYXIS_DEVINL uint32_t pack_bf16(float lo, float hi) {
     const __nv_bfloat162 x = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t *>(&x);

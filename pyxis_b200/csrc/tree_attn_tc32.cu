@@ -65,7 +65,8 @@ struct Smem {
     static constexpr uint32_t misc = bar + (kBars * 8 + 15) / 16 * 16;
     static constexpr uint32_t wmax = misc + 64;          // [2][kConvWarps] magnitudes
     static constexpr uint32_t scale = wmax + 64;         // [2][4]: 2^-e of K and of V of the latest tiles
-    static constexpr uint32_t aside = scale + 32;        // [4] a segment's drafts that are not in their tiles
+    static constexpr uint32_t kodd = scale + 32;         // [4] 1 + the latest tiles' numbers where their keys hold an infinity
+    static constexpr uint32_t aside = kodd + 16;         // [4] a segment's drafts that are not in their tiles
     static constexpr uint32_t vexp = aside + 32;         // [2][64] exponents of the values of a tile's drafts
     static constexpr uint32_t kexp = vexp + 2 * kTile;   // [4][64] 127 - e of a tile's keys, where each has its own
     static constexpr uint32_t red = kexp + 4 * kTile;    // [2][2 halves][128 rows]
@@ -122,6 +123,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // (the converters are at most two segments ahead of the softmax warps)
     unsigned long long *aside = reinterpret_cast<unsigned long long *>(smem + L::aside);
     uint8_t *kexp = smem + L::kexp;
+    volatile int *kodd = reinterpret_cast<volatile int *>(smem + L::kodd);
     volatile uint8_t *vexp = smem + L::vexp;
     long long &start_off = *reinterpret_cast<long long *>(smem + L::misc + 16);
     int &start_seq = *reinterpret_cast<int *>(smem + L::misc + 24);
@@ -155,6 +157,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc::mbar_init(&odone[b], 1);
         }
         *abort_flag = 0;
+        for (int i = 0; i < 4; ++i) kodd[i] = 0;
         tc::fence_mbar_init();
         tc::prefetch_tmap(&tm_k);
         tc::prefetch_tmap(&tm_v);
@@ -353,6 +356,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                             }
                             uint32_t m = __float_as_uint(mf);
                             if (m == 0x7F800000u) {  // an infinity, which sets no scale: the largest finite one
+                                if (!is_v) kodd[use[0] & 3] = use[0] + 1;
                                 m = 0;
                                 for (int i = cw; i < kSteps; i += kConvWarps) m = max(m, magnitude(src[i * 32]));
                             }
@@ -378,6 +382,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                             const float4 x = edge(i);
                             const int e = scale_exp(row_max(x));
                             put(i, x, attn_pow2(e));
+                            if (isinf(x.x) || isinf(x.y) || isinf(x.z) || isinf(x.w)) kodd[use[0] & 3] = use[0] + 1;
                             if (li == 0) kexp[(use[0] & 3) * kTile + i * kPer + sub] = (uint8_t)(127 - e);
                         }
                         used = 0;
@@ -544,6 +549,23 @@ __global__ void __launch_bounds__(kThreads, 1)
                             tc::tc_fence_after();
                             // log2 units: acc 2^-(eq + ek) scale log2 e (a masked score stays -inf with scale 0, too)
                             c2 = fmaxf(c2row * scale[n & 3], 1e-37f);
+                            if (kodd[n & 3] == n + 1) {
+                                // A key with an infinity has no second term and its products are NaN, which the
+                                // maximum passes over; where its score is -inf, its weight is zero.
+                                const int t = (r0 + row) / p.group;
+                                const float *q = reinterpret_cast<const float *>(
+                                    p.q + (sh.row0 + t) * p.q_row + (kvh * p.group + r0 + row - t * p.group) * p.q_head);
+#pragma unroll 1
+                                for (int i = half * 32; i < half * 32 + 32; ++i) {
+                                    float x = tmem_ld1(tS + (uint32_t)i);
+                                    if (row < rows && isnan(x) && k0 + i < sh.total &&
+                                        key_score<HD>(p, q, w.seq, kvh, k0 + i) * p.scale2 == -INFINITY)
+                                        x = -INFINITY;
+                                    __syncwarp();
+                                    tmem_st1(tS + (uint32_t)i, x);
+                                }
+                                tc::tmem_wait_st();
+                            }
                             tc::tmem_ld32(tS + (uint32_t)(half * 32), s);
                             if (tail) {
                                 const uint32_t *ke = reinterpret_cast<const uint32_t *>(kexp + (n & 3) * kTile + half * 32);
@@ -628,9 +650,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                     }
                     const long long at = ((long long)(c * 2 + (w.from_before ? 0 : 1)) * kRows + row);
+                    float *part = a.part_o + (at - row) * HD + (half * kOH) * kRows + row;  // column-major
+                    char *dst = p.out + (sh.row0 + t) * p.out_row + h * p.out_head + half * (kOH * 4);
                     if (whole) {
                         const float inv = l == 0.f ? 0.f : 1.f / l;
-                        char *dst = p.out + (sh.row0 + t) * p.out_row + h * p.out_head + half * (kOH * 4);
 #pragma unroll
                         for (int ch = 0; ch < kOH / 8; ++ch) {
                             uint32_t u[8];
@@ -639,13 +662,24 @@ __global__ void __launch_bounds__(kThreads, 1)
                             write_row<8, 4>(dst + ch * 32, u, a.vec_out);
                         }
                     } else {
-                        float *part = a.part_o + (at - row) * HD + (half * kOH) * kRows + row;  // column-major
 #pragma unroll
                         for (int i = 0; i < kOH; ++i) part[i * kRows] = acc[i];
                         if (half == 0) a.part_ml[at * 2] = m_run, a.part_ml[at * 2 + 1] = l;
                         if (half == 0 && !w.from_before && row == 0) {
                             const long long end = lo + count + (w.w.tiles - w.te) - 1;  // the unit's last tile
                             a.shared[c] = Shared{(int)(((end + 1) * g + total - 1) / total) - 1, sh.row0, kvh, r0, rows};
+                        }
+                    }
+                    if (isnan(odd_mark(acc))) {
+                        // an infinite value has no second term, and a weight's may be zero or negative: a sum over
+                        // values that are not finite is taken from the values (read back: acc stays in registers)
+#pragma unroll 1
+                        for (int i = 0; i < kOH; ++i) {
+                            float *y = whole ? reinterpret_cast<float *>(dst) + i : part + i * kRows;
+                            if (isfinite(*y)) continue;
+                            const float x = odd_values<float>(p, sh, w.seq, kvh, half * kOH + i, mask, (long long)w.tb * kTile,
+                                                              (long long)w.te * kTile);
+                            if (x != 0.f) *y = x;
                         }
                     }
                 }

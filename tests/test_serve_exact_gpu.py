@@ -90,3 +90,60 @@ def test_many_light_keys_behind_a_heavy_one(dt, hd, nodes, gap):
     want = num / den
     bad = (out - want[:, None]).abs() / want[:, None] / (e * 1.05 + half_step(dt) * 1.05)
     assert bad.max() <= 1.0, bad.max()
+
+
+# ------------------------------------------------------------------------------ infinities in the cache
+def place(t, pos):
+    return int(t.table[0, pos // t.page]), pos % t.page
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("nodes", [2, 24, 64])
+@pytest.mark.parametrize("ctx,at", [(300, 100), (300, 299), (40, 3), (2000, 1999)])  # in a tile of context alone, in the drafts' tile
+def test_a_key_with_an_infinity_reaches_rows_by_its_sign(dt, hd, nodes, ctx, at):
+    """Its score is -inf where q is negative there: weight 0, a row like any other; +inf elsewhere: NaN."""
+    t = Tree(53, [ctx, 70], [nodes, 3], 2, 1, hd, dt)
+    t.q = t.q.to(BF16).to(dt)  # queries of few bits, so that a second term of theirs is zero
+    pg, sl = place(t, at)
+    t.k[pg, sl, 0, 3] = math.inf
+    out = t.run(scale=1.0 / 16).cpu()
+    below = (t.q[:nodes, :, 3] < 0).cpu()
+    assert nodes == 2 or (below.any() and not below.all())
+    got = out[:nodes]
+    assert got[below].isfinite().all() and got[~below].isnan().all()
+    # the rows with a score of -inf: softmax over the other keys
+    q, keys, vals = t.q.double().cpu(), t.keys[0][:, 0], t.vals[0][:, 0]
+    bits = (t.mask[:nodes, None] >> np.arange(nodes, dtype=np.uint64)) & np.uint64(1)
+    seen = torch.from_numpy(np.concatenate([np.ones((nodes, ctx), bool), bits.astype(bool)], 1))
+    seen[:, at] = False
+    for h in range(2):
+        p = torch.softmax((q[:nodes, h] @ keys.T / 16).masked_fill(~seen, -math.inf), -1)
+        mag = (q[:nodes, h].abs() @ keys.abs().T).amax(-1, keepdim=True) / 16
+        e = 2 * (hd + 7) * U * mag + 4 * U + (2.0 ** -16 if dt == BF16 else 2.0 ** -21)
+        tol = 2 * (e + (ctx + nodes) * U) * (p @ vals.abs()) * 1.05 + half_step(dt) * (p @ vals).abs() * 1.05
+        rows = below[:, h]
+        assert ((got[rows, h].double() - p[rows] @ vals).abs() <= tol[rows]).all()
+    assert out[nodes:].isfinite().all()
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("nodes", [2, 24, 64])
+@pytest.mark.parametrize("ctx,at", [(300, 100), (300, 299), (40, 3), (1, 0), (7000, 6000)])
+def test_infinite_and_nan_values_stay_in_their_columns(dt, hd, nodes, ctx, at):
+    t, clean = (Tree(54, [ctx, 70], [nodes, 3], 2, 1, hd, dt) for _ in range(2))
+    pg, sl = place(t, at)
+    for x in (t, clean):  # the key of that place has most of the weight: its weight's second term may be zero
+        x.k[pg, sl, 0] = 0.3 * x.q[0, 0]
+    t.v[pg, sl, 0, 5], t.v[pg, sl, 0, 7], t.v[pg, sl, 0, hd - 1] = math.inf, -math.inf, math.nan
+    if ctx > 1:
+        pg2, sl2 = place(t, at - 1)  # both signs in one column
+        t.v[pg2, sl2, 0, 9], t.v[pg, sl, 0, 9] = math.inf, -math.inf
+    out, ref = t.run().cpu(), clean.run().cpu()
+    got = out[:nodes]
+    assert (got[..., 5] == math.inf).all() and (got[..., 7] == -math.inf).all() and got[..., hd - 1].isnan().all()
+    assert ctx == 1 or got[..., 9].isnan().all()
+    cols = [c for c in range(hd) if c not in (5, 7, 9, hd - 1)]
+    assert torch.equal(got[..., cols], ref[:nodes][..., cols])
+    assert torch.equal(out[nodes:], ref[nodes:])
