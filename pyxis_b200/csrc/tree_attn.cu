@@ -385,6 +385,15 @@ PYXIS_DEVINL void mma_tf32(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// q . k in f32, q as its two terms.
+template <int HD>
+__device__ __noinline__ float shared_score(const float *hi, const float *lo, const float *k) {
+    float x = 0.f;
+#pragma unroll 4
+    for (int d = 0; d < HD; ++d) x = fmaf(hi[d] + lo[d], k[d], x);
+    return x;
+}
+
 constexpr int kMmaKeys = 16;  // keys of a warp's block here: small buffers, so that more warps fit an SM
 
 template <typename T, int HD, int MT, int PER>
@@ -546,6 +555,29 @@ __global__ void __launch_bounds__(MmaCfg<T, HD, MT, PER>::kWarps * 32, PER) tree
                 for (int nt = 0; nt < kTiles; ++nt)
                     mma_tf32(s[mt][nt], h0[mt].z, h1[mt].z, h0[mt].w, h1[mt].w, kf[nt][2].hi, kf[nt][3].hi);
         }
+        if constexpr (kTwo) {
+            // A key with an infinity has no second term, and a query's may be zero: scores that are not finite
+            // are taken again in f32.
+            float z = 0.f;
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int nt = 0; nt < kTiles; ++nt)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) z = fmaf(s[mt][nt][k], 0.f, z);
+            if (__any_sync(0xffffffffu, isnan(z))) {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int nt = 0; nt < kTiles; ++nt)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (!isfinite(s[mt][nt][k])) {
+                                const float *q = sq + (mt * 16 + g + 8 * (k >> 1)) * C::kQPitch;
+                                s[mt][nt][k] = shared_score<HD>(q, q + RT * C::kQPitch, reinterpret_cast<const float *>(reinterpret_cast<const char *>(sk) + (nt * 8 + 2 * c + (k & 1)) * C::kPitch));
+                            }
+            }
+        }
         __syncwarp();
         if (b + kWarps < b1) load(p.k, sk, kbar, next_off);
         const bool tail = (b + 1) * kMmaKeys > sh.ctx;  // holds drafts or ends inside
@@ -702,7 +734,7 @@ __global__ void __launch_bounds__(MmaCfg<T, HD, MT, PER>::kWarps * 32, PER) tree
 
     // ---- join the warps: their outputs go where their K and V were
     __syncwarp();
-    float *so = reinterpret_cast<float *>(mine);
+    float *so = reinterpret_cast<float *>(mine), odd = 0.f;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -711,12 +743,29 @@ __global__ void __launch_bounds__(MmaCfg<T, HD, MT, PER>::kWarps * 32, PER) tree
 #pragma unroll
             for (int i = 0; i < HD / 8; ++i)
 #pragma unroll
-                for (int n = 0; n < 2; ++n) so[r * HD + 32 * (i >> 2) + 4 * (2 * c + n) + (i & 3)] = acc[mt][i][2 * h + n];
+                for (int n = 0; n < 2; ++n) {
+                    so[r * HD + 32 * (i >> 2) + 4 * (2 * c + n) + (i & 3)] = acc[mt][i][2 * h + n];
+                    odd = fmaf(acc[mt][i][2 * h + n], 0.f, odd);
+                }
             float l = l_run[mt][h];
             l += __shfl_xor_sync(0xffffffffu, l, 1);
             l += __shfl_xor_sync(0xffffffffu, l, 2);
             if (c == 0) sml[(warp * RT + r) * 2] = m_run[mt][h], sml[(warp * RT + r) * 2 + 1] = l;
         }
+    if (isnan(odd)) {
+        // A weight's second term may be zero, and an infinite value has none: a sum over values that are not
+        // finite is taken from the values of this warp's blocks (this lane's columns, read back: acc stays in
+        // registers).
+#pragma unroll 1
+        for (int n = 0; n < MT * 2 * HD / 4; ++n) {
+            const int r = n / (HD / 4) * 8 + g, i = n % (HD / 4), d = 32 * (i >> 3) + 4 * (2 * c + (i & 1)) + (i >> 1 & 3);
+            if (isfinite(so[r * HD + d])) continue;
+            float x = 0.f;
+            for (b = b0 + warp; b < b1; b += kWarps)
+                x += odd_values<T>(p, sh, seq, kvh, d, smask[r], b * kMmaKeys, (b + 1) * kMmaKeys);
+            if (x != 0.f) so[r * HD + d] = x;
+        }
+    }
     __syncthreads();
     join_warps<T, HD, RT, kWarps>(p, sh, smem, C::kWarpBytes, sml, rows, r0, kvh, split_i);
 }

@@ -99,7 +99,7 @@ def place(t, pos):
 
 @pytest.mark.parametrize("dt", [F32, BF16])
 @pytest.mark.parametrize("hd", [64, 128])
-@pytest.mark.parametrize("nodes", [2, 24, 64])
+@pytest.mark.parametrize("nodes", [2, 6, 24, 64])
 @pytest.mark.parametrize("ctx,at", [(300, 100), (300, 299), (40, 3), (2000, 1999)])  # in a tile of context alone, in the drafts' tile
 def test_a_key_with_an_infinity_reaches_rows_by_its_sign(dt, hd, nodes, ctx, at):
     """Its score is -inf where q is negative there: weight 0, a row like any other; +inf elsewhere: NaN."""
@@ -129,7 +129,7 @@ def test_a_key_with_an_infinity_reaches_rows_by_its_sign(dt, hd, nodes, ctx, at)
 
 @pytest.mark.parametrize("dt", [F32, BF16])
 @pytest.mark.parametrize("hd", [64, 128])
-@pytest.mark.parametrize("nodes", [2, 24, 64])
+@pytest.mark.parametrize("nodes", [2, 6, 24, 64])
 @pytest.mark.parametrize("ctx,at", [(300, 100), (300, 299), (40, 3), (1, 0), (7000, 6000)])
 def test_infinite_and_nan_values_stay_in_their_columns(dt, hd, nodes, ctx, at):
     t, clean = (Tree(54, [ctx, 70], [nodes, 3], 2, 1, hd, dt) for _ in range(2))
