@@ -368,6 +368,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     Shared &leader = *cluster.map_shared_rank(&s, 0);
     const size_t row = blockIdx.y;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    // first half of the barrier that tells every CTA of the cluster that the others have started (their
+    // shared memory may be written): waited on before the maxima are sent
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
 
     if (tid == 0) {
         s.temperature = a.temperature ? (double)a.temperature[row] : a.temperature_all;
@@ -437,6 +440,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     float *wtop = reinterpret_cast<float *>(s.scan);
     if (lane == 0) wtop[warp] = top;
     __syncthreads();
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     if (tid < (int)ranks) {
         float t = wtop[0];
         for (int w = 1; w < kWarps; ++w) t = fmaxf(t, wtop[w]);

@@ -147,3 +147,18 @@ def test_infinite_and_nan_values_stay_in_their_columns(dt, hd, nodes, ctx, at):
     cols = [c for c in range(hd) if c not in (5, 7, 9, hd - 1)]
     assert torch.equal(got[..., cols], ref[:nodes][..., cols])
     assert torch.equal(out[nodes:], ref[nodes:])
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("n", [4097, 4104, 8193, 8200])
+def test_short_segments_of_a_cluster(dt, n):
+    """Rows a little longer than one CTA's share: each CTA of a cluster has little to load before it writes its
+    maximum into the others' memory.  The largest logit lies in each CTA's segment once."""
+    m = 96
+    g = torch.Generator().manual_seed(n)
+    x = torch.randn(m, n, generator=g)
+    at = (torch.arange(m) * n) // m
+    x[torch.arange(m), at] = 30.0  # has all the weight that f32 shows
+    for _ in range(20):
+        idx, prob = px.sample_dev(x.to(dt).cuda(), torch.full((m,), 0.5, device="cuda"))
+        assert torch.equal(idx.cpu().long(), at) and (prob > 0.999).all()
