@@ -290,6 +290,7 @@ __global__ void __launch_bounds__(TreeCfg<T, HD, RT, PER>::kWarps * 32) tree_att
                     finite = finite && all_finite<T>(*x);
             }
             plain = __all_sync(0xffffffffu, finite);
+            tc::fence_proxy_async_smem();  // the buffer's next copy comes after these stores
             __syncwarp();
         }
         if (plain) {
@@ -652,6 +653,7 @@ __global__ void __launch_bounds__(MmaCfg<T, HD, MT, PER>::kWarps * 32, PER) tree
                 else
                     finite = finite && all_finite<T>(*x);
             }
+            tc::fence_proxy_async_smem();  // the buffer's next copy comes after these stores
             __syncwarp();
             unsigned odd = __ballot_sync(0xffffffffu, !finite);
             if (odd) {
@@ -684,6 +686,7 @@ __global__ void __launch_bounds__(MmaCfg<T, HD, MT, PER>::kWarps * 32, PER) tree
                 if (!finite)
                     for (int i = 0; i < HD; ++i)
                         if (!isfinite(to_f32(reinterpret_cast<const T *>(row)[i]))) store(reinterpret_cast<T *>(row) + i, 0.f);
+                tc::fence_proxy_async_smem();
                 __syncwarp();
             }
         }

@@ -246,6 +246,7 @@ PYXIS_DEVINL Range begin_walk(const TcParams &a, Walk<TILE> &w, long long *warp_
         if (mine > 0 && r.lo >= first && r.lo < first + mine) start_seq = s, start_off = r.lo - first;
         before += sum;
     }
+    tc::fence_proxy_async_smem();  // warp_sum may lie where a copy lands next
     __syncthreads();
     w.begin(p, start_seq, start_off, r.count);
     return r;
