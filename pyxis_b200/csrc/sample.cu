@@ -170,7 +170,7 @@ struct Row {
         return b >= last_bin || isinf(top) ? -INFINITY : top - (float)(b + 1) * (1.001f / bin_scale) - fabsf(top) * 1e-6f;
     }
     // exp((x - top) / temperature) 2^shift, rounded: 2^(shift - k / 256) from the table, times exp of
-    // the rest d ln 2 / 256, |d| <= 1/2, by its Taylor polynomial (cubic: off by 2^-47 of the weight)
+    // the rest d ln 2 / 256, |d| <= 1/2, by its Taylor polynomial (of degree four: off by 2^-54 of the weight)
     PYXIS_DEVINL u64 weight(float x) const {
         constexpr double c = 0.69314718055994530942 / kTable;
         constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: rounds to a whole number
@@ -178,7 +178,7 @@ struct Row {
         const double m = u + kRound;
         const int k = __double2loint(m);  // valid bins: u < 2^14
         const double d = (m - kRound) - u;
-        double e = fma(d, fma(d, fma(d, c * c * c / 6.0, c * c / 2.0), c), 1.0) * table[k & (kTable - 1)];
+        double e = fma(d, fma(d, fma(d, fma(d, c * c * c * c / 24.0, c * c * c / 6.0), c * c / 2.0), c), 1.0) * table[k & (kTable - 1)];
         e = __hiloint2double(__double2hiint(e) - ((k >> 8) << 20), __double2loint(e));  // 2^-(k / 256)
         // to a whole number in the low bits
         const u64 w = (u64)__double_as_longlong(e + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;

@@ -162,3 +162,23 @@ def test_short_segments_of_a_cluster(dt, n):
     for _ in range(20):
         idx, prob = px.sample_dev(x.to(dt).cuda(), torch.full((m,), 0.5, device="cuda"))
         assert torch.equal(idx.cpu().long(), at) and (prob > 0.999).all()
+
+
+# --------------------------------------------------------------------------------------- sampling
+def test_weights_next_to_min_p():
+    """min_p 1.6 steps of 2^-44 below a token's weight keeps the token.  The weight is exp() rounded to such a
+    step, half a step at most, and off by less than 0.05 of one before that (a few u of 64 bits, 2^-54.5 of
+    the polynomial); min_p rounds up to a step: below 1.1 steps of the two together."""
+    rng = np.random.default_rng(3)
+    x = -np.concatenate([(np.arange(1, 200) + f) * math.log(2) / 256 for f in (0.46, 0.49, 0.5, 0.51, 0.54)] + [rng.random(500) * 0.7])
+    x = x.astype(np.float32)
+    drop = []
+    for v in x:
+        w = math.exp(float(v))
+        idx, _ = px.sample_dev(torch.tensor([[0.0, float(v)]]).cuda(), torch.tensor([1 - 2.0 ** -24], device="cuda"),
+                               min_p=w - 1.6 * 2.0 ** -44)
+        drop.append(idx)
+        idx, _ = px.sample_dev(torch.tensor([[0.0, float(v)]]).cuda(), torch.tensor([1 - 2.0 ** -24], device="cuda"),
+                               min_p=w + 1.6 * 2.0 ** -44)
+        drop.append(1 - idx)
+    assert (torch.cat(drop) == 1).all()
