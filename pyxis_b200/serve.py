@@ -14,7 +14,9 @@
 Pages are two tensors of one shape and layout, ``[..., num_pages, page_size, n_kv_heads, head_dim]``
 with any strides whose last is 1, float32 or bfloat16; the page operators take a leading axis of
 layers.  Calls are asynchronous on ``stream`` (default: torch's current stream of the tensors'
-device) and raise PyxisError on bad arguments.
+device) and raise PyxisError on bad arguments.  Where a ``stream`` is given, it has to come after
+the work that makes the inputs, and outputs that the call makes itself belong to that stream: use
+them there, or elsewhere after waiting for it (and ``record_stream``).
 """
 from __future__ import annotations
 
@@ -66,6 +68,7 @@ class _Torch:
         self.f32, self.f64, self.i32, self.i64 = torch.float32, torch.float64, torch.int32, torch.int64
         self.masks = (torch.int64, torch.uint64)
         self.types = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16}
+        self.on_stream = torch.cuda.stream
         self.contexts: dict = {}
         raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
         self.raw_stream = raw or (lambda device: torch.cuda.current_stream(device).cuda_stream)
@@ -95,6 +98,14 @@ def _begin(t):
 def _stream(stream, device: int) -> int:
     # torch's default stream is 0, which the library reads as its own: name the legacy stream instead
     return (_torch.raw_stream(device) if stream is None else stream.cuda_stream) or CUDA_STREAM_LEGACY
+
+
+def _empty(like, shape, dtype, stream):
+    """An output of the call, from the memory of the stream that writes it."""
+    if stream is None:
+        return like.new_empty(shape, dtype=dtype)
+    with _torch.on_stream(stream):
+        return like.new_empty(shape, dtype=dtype)
 
 
 def _array(t, what: str, dtype, n: int, device: int) -> int:
@@ -165,7 +176,7 @@ def qk_norm_rope_dev(qkv, positions, inv_freq, n_q_heads: int, n_kv_heads: int, 
     if kv.n_kv_heads != n_kv_heads or kv.head_dim != head_dim or k_pages.dtype is not dtype:
         _fail("the cache's heads or type differ from qkv's")
     if q is None:
-        q = qkv.new_empty(n, n_q_heads, head_dim)
+        q = _empty(qkv, (n, n_q_heads, head_dim), dtype, stream)
         ld_q = n_q_heads * head_dim
     else:
         if q.shape != (n, n_q_heads, head_dim) or q.dtype is not dtype or q.get_device() != dev or q.stride(2) != 1 or (
@@ -202,7 +213,7 @@ def tree_attention_dev(q, k_pages, v_pages, block_table, context_len, q_start, t
         _fail("q must be [rows, n_q, head_dim] of the cache's type")
     rows, n_q, hd = shape
     if out is None:
-        out = q.new_empty(rows, n_q, hd)
+        out = _empty(q, (rows, n_q, hd), dtype, stream)
     elif out.shape != shape or out.dtype is not dtype or out.get_device() != dev or out.stride(2) != 1:
         _fail("out must have q's shape, type and device")
     o = out.stride()
@@ -245,7 +256,7 @@ def kv_compact_dev(k_pages, v_pages, block_table, context_len, accepted, new_len
     kv = _pages(k_pages, v_pages, dev, True)
     n_seq, width = _table(block_table, "block_table", dev)
     if new_len is None:
-        new_len = context_len.new_empty(n_seq)
+        new_len = _empty(context_len, (n_seq,), T.i32, stream)
     rc = T.compact(ctx, C.byref(kv), block_table.data_ptr(), block_table.stride(0), width,
                    _array(context_len, "context_len", T.i32, n_seq, dev), _array(accepted, "accepted", T.i64, n_seq, dev), n_seq,
                    _array(new_len, "new_len", T.i32, n_seq, dev), _stream(stream, dev))
@@ -275,9 +286,9 @@ def sample_dev(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
     params = _SampleParams(t, k, p, m, temperature if t is None else 1.0, top_k if k is None else 0, top_p if p is None else 1.0,
                            min_p if m is None else 0.0)
     if idx is None:
-        idx = logits.new_empty(M, dtype=T.i32)
+        idx = _empty(logits, (M,), T.i32, stream)
     if prob is None:
-        prob = logits.new_empty(M, dtype=T.f32)
+        prob = _empty(logits, (M,), T.f32, stream)
     rc = T.sample(ctx, logits.data_ptr(), kind, M, n, logits.stride(0), _array(uniforms, "uniforms", T.f32, M, dev), C.byref(params),
                   _array(idx, "idx", T.i32, M, dev), _array(prob, "prob", T.f32, M, dev), _stream(stream, dev))
     if rc:

@@ -182,3 +182,44 @@ def test_weights_next_to_min_p():
                                min_p=w + 1.6 * 2.0 ** -44)
         drop.append(1 - idx)
     assert (torch.cat(drop) == 1).all()
+
+
+# ----------------------------------------------------------------------------------------- streams
+def outputs_on(stream, call):
+    """The call's results, made on `stream` without an output of the caller's while the current stream still
+    reads memory that it has given back; those reads must see what was there."""
+    want = call(None)
+    sizes = [w.untyped_storage().nbytes() for w in want]
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    held = [torch.full((n,), 7, dtype=torch.uint8, device="cuda") for n in sizes for _ in range(2)]
+    copies = [torch.empty_like(h) for h in held]
+    torch.cuda.synchronize()
+    torch.cuda._sleep(200_000_000)  # about 0.1 s
+    for h, c in zip(held, copies):
+        c.copy_(h)
+    del held, h
+    got = call(stream)
+    stream.synchronize()
+    torch.cuda.synchronize()
+    for c in copies:
+        assert (c == 7).all()
+    for g, w in zip(got, want):
+        assert torch.equal(g, w)
+
+
+def test_outputs_for_another_stream_are_its_own():
+    s = torch.cuda.Stream()
+    t = Tree(60, [500, 90], [5, 3], 16, 2, 128, F32)
+    a = t.args()
+    outputs_on(s, lambda st: (px.tree_attention_dev(*a, max_tree=5, stream=st),))
+    x, u = torch.randn(300, 200, device="cuda"), torch.rand(300, device="cuda")
+    outputs_on(s, lambda st: px.sample_dev(x, u, stream=st))
+    g = torch.Generator().manual_seed(1)
+    qkv = torch.randn(9, 8 * 64, generator=g).cuda()
+    pages, vpages = (torch.zeros(2, 16, 2, 64, device="cuda") for _ in range(2))
+    slots = torch.arange(9, dtype=torch.int32, device="cuda")
+    outputs_on(s, lambda st: (px.qk_norm_rope_dev(qkv, None, None, 4, 2, 64, k_pages=pages, v_pages=vpages, slots=slots, stream=st),))
+    table = torch.zeros(300, 1, dtype=torch.int32, device="cuda")
+    ctx, acc = torch.arange(300, dtype=torch.int32, device="cuda") % 9, torch.zeros(300, dtype=torch.int64, device="cuda")
+    outputs_on(s, lambda st: (px.kv_compact_dev(pages[None], vpages[None], table, ctx, acc, stream=st),))
