@@ -333,12 +333,15 @@ class PagePool:
             self._uses[p] = 1
         return got
 
-    def _drop(self, pages) -> None:
-        if len(set(pages)) < len(pages):  # (all checks first: a refusal leaves the pool as it was)
+    def _check(self, pages) -> None:
+        if len(set(pages)) < len(pages):
             _fail("a page stands twice in a table")
         for p in pages:
             if not 0 <= p < self.num_pages or self._uses[p] <= 0:
                 _fail(f"page {p} is free already" if 0 <= p < self.num_pages else f"no page {p}")
+
+    def _drop(self, pages) -> None:
+        self._check(pages)  # (all checks first: a refusal leaves the pool as it was)
         for p in pages:
             self._uses[p] -= 1
             if self._uses[p] == 0:
@@ -364,6 +367,7 @@ class PagePool:
     def fork(self, table: list[int], tokens: int) -> tuple[list[int], list[int], list[int]]:
         if self._pages_for(tokens) > len(table):
             _fail(f"a fork at {tokens} tokens of a table of {len(table)} pages")
+        self._check(table)
         full = tokens // self.page_size
         new = self._take(self._pages_for(tokens) - full)
         for p in table[:full]:

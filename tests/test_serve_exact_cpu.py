@@ -39,3 +39,20 @@ def test_yarn_leaves_frequencies_that_turn_often_alone_at_the_slow_end():
     g, _ = px.rope_frequencies(128, 1e4, "yarn", factor=4.0, original_context=1e6)
     assert 1e6 * f[-1] / (2 * math.pi) > 18
     assert g[-1] > 0.8 * f[-1]
+
+
+def test_a_table_that_was_freed_is_not_forked():
+    pool = px.PagePool(8, 16)
+    t = pool.allocate(40)
+    stale, twice = list(t), [t[0], t[0], t[1]]
+    with pytest.raises(px.PyxisError):
+        pool.fork(twice, 40)
+    with pytest.raises(px.PyxisError):
+        pool.fork([0, 1, 99], 40)
+    pool.free(t)
+    assert pool.available == 8
+    with pytest.raises(px.PyxisError):
+        pool.fork(stale, 40)
+    assert pool.available == 8
+    a, b = pool.allocate(64), pool.allocate(64)
+    assert sorted(a + b) == list(range(8))  # no page is given out twice
