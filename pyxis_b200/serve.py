@@ -21,6 +21,7 @@ them there, or elsewhere after waiting for it (and ``record_stream``).
 from __future__ import annotations
 
 import ctypes as C
+from operator import index as _index
 
 import numpy as np
 
@@ -56,6 +57,13 @@ class _SampleParams(C.Structure):
 
 def _fail(msg: str):
     raise PyxisError(PYXIS_EINVAL, msg)
+
+
+def _int32(value, what: str) -> int:
+    value = _index(value)
+    if not -(1 << 31) <= value < 1 << 31:
+        _fail(f"{what} {value} is out of range")
+    return value
 
 
 class _Torch:
@@ -148,7 +156,7 @@ def rope_frequencies(rotary_dim: int, theta: float, kind: str = "plain", factor:
     (pyxis_rope_frequencies): kind "plain", "linear", "ntk" or "yarn"."""
     if kind not in ROPE_KINDS:
         _fail(f"unknown frequency scaling {kind!r}")
-    if rotary_dim <= 0:
+    if _int32(rotary_dim, "rotary_dim") <= 0:
         _fail(f"rotary_dim {rotary_dim} is not even and positive")
     freq = np.empty(rotary_dim // 2, np.float64)
     scale = C.c_double()
@@ -221,7 +229,8 @@ def tree_attention_dev(q, k_pages, v_pages, block_table, context_len, q_start, t
     a = _TreeArgs(q.data_ptr(), out.data_ptr(), s[0], s[1], o[0], o[1], rows, n_seq,
                   _array(q_start, "q_start", T.i32, n_seq + 1, dev), _array(context_len, "context_len", T.i32, n_seq, dev),
                   block_table.data_ptr(), None if tree_mask is None else _array(tree_mask, "tree_mask", T.i64, rows, dev),
-                  block_table.stride(0), width, n_q, max_tree, width * kv.page_size if max_context is None else max_context,
+                  block_table.stride(0), width, n_q, _int32(max_tree, "max_tree"),
+                  width * kv.page_size if max_context is None else max(-1, min(_index(max_context), (1 << 62))),
                   hd ** -0.5 if scale is None else scale)
     if workspace is None:
         rc = T.tree(ctx, C.byref(a), C.byref(kv), None, 0, _stream(stream, dev))
@@ -283,7 +292,8 @@ def sample_dev(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
 
     t, k, p, m = (per_row(temperature, "temperature", T.f32), per_row(top_k, "top_k", T.i32), per_row(top_p, "top_p", T.f32),
                   per_row(min_p, "min_p", T.f32))
-    params = _SampleParams(t, k, p, m, temperature if t is None else 1.0, top_k if k is None else 0, top_p if p is None else 1.0,
+    params = _SampleParams(t, k, p, m, temperature if t is None else 1.0,
+                           max(0, min(_index(top_k), n)) if k is None else 0, top_p if p is None else 1.0,
                            min_p if m is None else 0.0)
     if idx is None:
         idx = _empty(logits, (M,), T.i32, stream)

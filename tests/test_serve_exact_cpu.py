@@ -56,3 +56,10 @@ def test_a_table_that_was_freed_is_not_forked():
     assert pool.available == 8
     a, b = pool.allocate(64), pool.allocate(64)
     assert sorted(a + b) == list(range(8))  # no page is given out twice
+
+
+def test_sizes_past_32_bits_are_refused():
+    for rot in ((1 << 32) + 2, 1 << 31, -(1 << 40)):
+        with pytest.raises(px.PyxisError) as e:
+            px.rope_frequencies(rot, 1e4)
+        assert e.value.code == _native.PYXIS_EINVAL

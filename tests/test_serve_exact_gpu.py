@@ -223,3 +223,20 @@ def test_outputs_for_another_stream_are_its_own():
     table = torch.zeros(300, 1, dtype=torch.int32, device="cuda")
     ctx, acc = torch.arange(300, dtype=torch.int32, device="cuda") % 9, torch.zeros(300, dtype=torch.int64, device="cuda")
     outputs_on(s, lambda st: (px.kv_compact_dev(pages[None], vpages[None], table, ctx, acc, stream=st),))
+
+
+# --------------------------------------------------------------------------------------- arguments
+def test_numbers_past_32_bits_are_refused_or_mean_what_they_say():
+    x, u = torch.tensor([[0.0, 1.0, 2.0]]).cuda(), torch.tensor([0.99], device="cuda")
+    keep = px.sample_dev(x, u)[0].tolist()
+    assert keep == [0]
+    assert px.sample_dev(x, u, top_k=(1 << 32) + 1)[0].tolist() == keep  # more than the row: all of it
+    assert px.sample_dev(x, u, top_k=(1 << 31))[0].tolist() == keep
+    assert px.sample_dev(x, u, top_k=-(1 << 40) + 1)[0].tolist() == keep
+    t = Tree(61, [20], [3], 2, 1, 64, F32)
+    for bad in ((1 << 32) + 3, -(1 << 32) + 3):
+        with pytest.raises(px.PyxisError):
+            t.run(max_tree=bad)
+    assert torch.equal(t.run(max_context=1 << 80), t.run())  # a bound that bounds nothing
+    with pytest.raises(px.PyxisError):
+        t.run(max_context=-(1 << 64) + 5)
