@@ -305,9 +305,21 @@ def _stream_handle(stream, device) -> int:
     return h if h else CUDA_STREAM_LEGACY
 
 
+def _empty_on(stream, shape, dtype, device):
+    """An output of a call, from the memory of the stream that writes it (the current stream's may still be
+    in use by work that this stream does not wait for)."""
+    import torch
+
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
 def matmul_dev(X, weight: Weights, out_features: int, in_features: int, Y=None, stream=None, workspace=None):
     """Device-pointer form over torch CUDA tensors: X [M, in] f32 -> Y [M, out] f32, launched
-    asynchronously on ``stream`` (a torch.cuda.Stream; default: torch's current stream)."""
+    asynchronously on ``stream`` (a torch.cuda.Stream; default: torch's current stream), whose memory
+    a Y made by the call belongs to."""
     import torch
 
     if X.dim() == 1:
@@ -316,7 +328,7 @@ def matmul_dev(X, weight: Weights, out_features: int, in_features: int, Y=None, 
         raise PyxisError(_native.PYXIS_EINVAL, f"X/Y must be on cuda:{weight.ctx.device}, the weights' device")
     M = X.shape[0]
     if Y is None:
-        Y = torch.empty((M, out_features), dtype=torch.float32, device=X.device)
+        Y = _empty_on(stream, (M, out_features), torch.float32, X.device)
     st = _stream_handle(stream, X.device)
     ws_ptr, ws_bytes = (workspace.data_ptr(), workspace.numel() * workspace.element_size()) if workspace is not None else (None, 0)
     check(_native.lib().pyxis_cuda_matmul_dev(weight.ctx.handle, weight.handle, C.c_void_p(X.data_ptr()), M,
@@ -340,9 +352,9 @@ def argmax_dev(values, index_base: int = 0, idx=None, val=None, stream=None, dev
     M, n = values.shape
     ctx = _require_cuda(values.device.index or 0)
     if idx is None:
-        idx = torch.empty(M, dtype=torch.int32, device=values.device)
+        idx = _empty_on(stream, M, torch.int32, values.device)
     if val is None:
-        val = torch.empty(M, dtype=torch.float32, device=values.device)
+        val = _empty_on(stream, M, torch.float32, values.device)
     st = _stream_handle(stream, values.device)
     check(_native.lib().pyxis_cuda_argmax_dev(ctx.handle, C.c_void_p(values.data_ptr()), M, n, values.stride(0),
                                               index_base, C.c_void_p(idx.data_ptr()), C.c_void_p(val.data_ptr()),

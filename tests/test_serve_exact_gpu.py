@@ -240,3 +240,12 @@ def test_numbers_past_32_bits_are_refused_or_mean_what_they_say():
     assert torch.equal(t.run(max_context=1 << 80), t.run())  # a bound that bounds nothing
     with pytest.raises(px.PyxisError):
         t.run(max_context=-(1 << 64) + 5)
+
+
+def test_outputs_of_products_and_argmax_for_another_stream_are_its_own():
+    s = torch.cuda.Stream()
+    w = px.Weights.quantize_int8(px.synth_normal_bf16(3, 512 * 256, 0.02), 256)
+    x = torch.randn(5, 256, device="cuda")
+    outputs_on(s, lambda st: (px.matmul_dev(x, w, 512, 256, stream=st),))
+    v = torch.randn(300, 1000, device="cuda")
+    outputs_on(s, lambda st: px.argmax_dev(v, stream=st))
