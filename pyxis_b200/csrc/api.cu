@@ -139,22 +139,52 @@ constexpr size_t kWsTickets = 16384;  // 128-row tiles: matrices of up to 2M row
 
 int grow_workspace(pyxis_cuda_ctx *ctx, size_t want) {
     if (ctx->ws_cap >= want) return PYXIS_OK;
-    want = std::max(want, ctx->ws_cap + ctx->ws_cap / 2);  // few steps to any size
+    const size_t roomy = std::max(want, ctx->ws_cap + ctx->ws_cap / 2);  // few steps to any size, memory permitting
+    if (ctx->ws && ctx->ws_captured) {
+        try {  // (no exception leaves a C entry point)
+            ctx->ws_retired.reserve(ctx->ws_retired.size() + 1);
+        } catch (...) {
+            return fail(PYXIS_ENOMEM, "host allocation failed");
+        }
+    } else if (ctx->ws) {  // no graph names it: its memory counts for the next one
+        PYXIS_CUDA_TRY(cudaDeviceSynchronize(), "cudaDeviceSynchronize");
+        cudaFree(ctx->ws);
+        ctx->ws = nullptr;
+        ctx->ws_cap = 0;
+    }
     void *bigger = nullptr;
-    PYXIS_CUDA_TRY(cudaMalloc(&bigger, want), "cudaMalloc(workspace)");
-    // a captured graph may still name the smaller one: it lives as long as the context
+    size_t got = roomy;
+    cudaError_t e = cudaMalloc(&bigger, roomy);
+    if (e == cudaErrorMemoryAllocation && roomy > want) {
+        got = want;
+        e = cudaMalloc(&bigger, want);
+    }
+    if (e != cudaSuccess) {
+        cudaGetLastError();  // reported here, not by the caller's next launch
+        return cuda_fail(e, "cudaMalloc(workspace)");
+    }
     if (ctx->ws) ctx->ws_retired.push_back(ctx->ws);
     ctx->ws = bigger;
-    ctx->ws_cap = want;
+    ctx->ws_cap = got;
+    ctx->ws_captured = false;
     return PYXIS_OK;
 }
 
-// Grows the context workspace, refusing while `st` is being captured (an allocation there would
-// be an error, and a graph would keep the old pointer).
+// For work on `st` that uses the context workspace: grows it, refusing while `st` is being captured
+// (an allocation there would be an error), and notes whether a captured graph will name it.
 int ensure_ctx_workspace(pyxis_cuda_ctx *ctx, size_t want, cudaStream_t st) {
-    if (ctx->ws_cap >= want) return PYXIS_OK;
-    cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
-    if (cudaStreamIsCapturing(st, &cs) == cudaSuccess && cs != cudaStreamCaptureStatusNone)
+    bool capturing = false;
+    if (ctx->ws_cap < want || !ctx->ws_captured) {
+        cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+        const cudaError_t e = cudaStreamIsCapturing(st, &cs);
+        if (e != cudaSuccess) cudaGetLastError();  // (the legacy stream while another one is captured)
+        capturing = e == cudaSuccess && cs != cudaStreamCaptureStatusNone;
+    }
+    if (ctx->ws_cap >= want) {
+        ctx->ws_captured = ctx->ws_captured || capturing;
+        return PYXIS_OK;
+    }
+    if (capturing)
         return fail(PYXIS_EINVAL,
                     "the context workspace must grow to %zu bytes, which cannot happen during stream capture: "
                     "call pyxis_cuda_reserve_workspace first",

@@ -24,7 +24,8 @@ struct pyxis_cuda_ctx {
     // workspace kept for pyxis_cuda_matmul_dev calls that pass none
     void *ws = nullptr;
     size_t ws_cap = 0;
-    std::vector<void *> ws_retired;  // workspaces it outgrew, freed with the context
+    bool ws_captured = false;        // a captured call names it
+    std::vector<void *> ws_retired;  // those that it outgrew although captured calls name them: freed with the context
     // argmax scratch (allocated and zeroed at init)
     pyxis::ArgmaxScratch amax{};
     void *amax_mem = nullptr;

@@ -249,3 +249,61 @@ def test_outputs_of_products_and_argmax_for_another_stream_are_its_own():
     outputs_on(s, lambda st: (px.matmul_dev(x, w, 512, 256, stream=st),))
     v = torch.randn(300, 1000, device="cuda")
     outputs_on(s, lambda st: px.argmax_dev(v, stream=st))
+
+
+# --------------------------------------------------------------------------------- context workspace
+class Context:
+    def __enter__(self):
+        self.handle = C.c_void_p()
+        _native.check(_native.lib().pyxis_cuda_init(0, C.byref(self.handle)))
+        return self.handle
+
+    def __exit__(self, *_):
+        torch.cuda.synchronize()
+        _native.check(_native.lib().pyxis_cuda_destroy(self.handle))
+
+
+def leave_free(nbytes):
+    """Takes the GPU's memory but for about nbytes."""
+    torch.cuda.empty_cache()
+    return torch.empty(torch.cuda.mem_get_info()[0] - nbytes, dtype=torch.uint8, device="cuda")
+
+
+GB = 1 << 30
+
+
+def test_the_workspace_grows_into_what_memory_there_is():
+    L = _native.lib()
+    with Context() as ctx:
+        _native.check(L.pyxis_cuda_reserve_workspace(ctx, 2 * GB))
+        rest = leave_free(GB)
+        # 2.5 GB fit once the old 2 GB are given back, which no captured graph names; 1.5 times the old does not fit beside it
+        _native.check(L.pyxis_cuda_reserve_workspace(ctx, 5 * GB // 2))
+        free = torch.cuda.mem_get_info()[0]
+        assert free < GB
+        _native.check(L.pyxis_cuda_reserve_workspace(ctx, GB))  # has it
+        assert torch.cuda.mem_get_info()[0] == free
+        assert L.pyxis_cuda_reserve_workspace(ctx, 400 * GB) != 0  # an error, and no more than that
+        del rest
+        torch.cuda.empty_cache()
+        _native.check(L.pyxis_cuda_reserve_workspace(ctx, 3 * GB))
+
+
+def test_a_captured_call_keeps_its_workspace_when_the_context_grows():
+    t = Tree(62, [9000], [3], 2, 1, 64, F32)
+    want = t.run()
+    out = torch.empty_like(want)
+    a = t.args()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        px.tree_attention_dev(*a, max_tree=3, out=out)
+    L, ctx = _native.lib(), px.get_cuda(0).handle
+    _native.check(L.pyxis_cuda_reserve_workspace(ctx, 256 << 20))
+    junk = torch.full((64 << 20,), 255, dtype=torch.uint8, device="cuda")  # where a freed workspace might have been
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    assert (junk == 255).all()
