@@ -350,34 +350,38 @@ __global__ void __launch_bounds__(kThreads, 1)
             rd[half * kBQ + row] = mt;
             named_bar(1 + quad, 64);  // both halves of these 32 rows
             mt = fmaxf(mt, rd[(1 - half) * kBQ + row]);
-            if (!ok) continue;
             const bool raise = mt > m_run + kRaise;
             const float alpha = raise ? exp2f(m_run - mt) : 1.0f;  // 0 on the first tile
-            if (raise) {
-                l *= alpha;
-                m_run = mt;
-            }
             uint32_t ph[32], pl[32];
-            float sum = 0.f;
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                uint32_t r[32];
-                float s[32];
-                tc::tmem_ld32_async(tS + half * 64 + c * 32, r);
-                tc::tmem_wait_ld();
-                score32(r, c2, diag, half * 64 + c * 32, row, s);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float p0 = exp2f(s[2 * i] - m_run), p1 = exp2f(s[2 * i + 1] - m_run);
-                    sum += p0 + p1;
-                    const __half2 h = __floats2half2_rn(p0, p1);
-                    const float2 hf = __half22float2(h);
-                    const __half2 lo = __floats2half2_rn(p0 - hf.x, p1 - hf.y);
-                    ph[c * 16 + i] = *reinterpret_cast<const uint32_t *>(&h);
-                    pl[c * 16 + i] = *reinterpret_cast<const uint32_t *>(&lo);
+            if (ok) {
+                if (raise) {
+                    l *= alpha;
+                    m_run = mt;
                 }
+                float sum = 0.f;
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t r[32];
+                    float s[32];
+                    tc::tmem_ld32_async(tS + half * 64 + c * 32, r);
+                    tc::tmem_wait_ld();
+                    score32(r, c2, diag, half * 64 + c * 32, row, s);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float p0 = exp2f(s[2 * i] - m_run), p1 = exp2f(s[2 * i + 1] - m_run);
+                        sum += p0 + p1;
+                        const __half2 h = __floats2half2_rn(p0, p1);
+                        const float2 hf = __half22float2(h);
+                        const __half2 lo = __floats2half2_rn(p0 - hf.x, p1 - hf.y);
+                        ph[c * 16 + i] = *reinterpret_cast<const uint32_t *>(&h);
+                        pl[c * 16 + i] = *reinterpret_cast<const uint32_t *>(&lo);
+                    }
+                }
+                l += sum;
             }
-            l += sum;
+            // each half's terms lie over scores of both: written once both have read theirs a second time
+            named_bar(1 + quad, 64);
+            if (!ok) continue;
             // keys 2i, 2i+1 of this half -> column half * 32 + i (hi) and 64 + half * 32 + i (lo)
             tc::tmem_st32(tS + half * 32, ph);
             tc::tmem_st32(tS + 64 + half * 32, pl);
