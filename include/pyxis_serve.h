@@ -19,6 +19,8 @@
  * PYXIS_DTYPE_F32 or PYXIS_DTYPE_BF16; sums, maxima and norms are f32 or wider for both.  Indexes
  * read from device memory (pages, slots, lengths) are bounds-checked by the kernels: a page or slot
  * outside the cache is never read or written, and what a sequence naming one gets is unspecified.
+ * Kernels that wait for copies or tensor-core products give up after a limit, with their outputs partly
+ * unwritten: pyxis_cuda_check_device_error reports it.
  */
 #ifndef PYXIS_SERVE_H
 #define PYXIS_SERVE_H

@@ -51,6 +51,11 @@ class CudaMatmul:
     def synchronize(self) -> None:
         check(self._lib.pyxis_cuda_synchronize(self.handle))
 
+    def check_device_error(self) -> None:
+        """Waits for the device and raises PyxisError (PYXIS_ETIMEOUT) if a kernel's bounded wait ran out since
+        the last check; the outputs of that launch are invalid (pyxis_cuda_check_device_error)."""
+        check(self._lib.pyxis_cuda_check_device_error(self.handle))
+
     def close(self) -> None:
         if self.handle:
             self._lib.pyxis_cuda_destroy(self.handle)

@@ -17,6 +17,10 @@ layers.  Calls are asynchronous on ``stream`` (default: torch's current stream o
 device) and raise PyxisError on bad arguments.  Where a ``stream`` is given, it has to come after
 the work that makes the inputs, and outputs that the call makes itself belong to that stream: use
 them there, or elsewhere after waiting for it (and ``record_stream``).
+
+The attention's kernels never wait without a limit: where a wait runs out, the launch ends with its
+outputs partly unwritten and sets the context's error flag, which ``get_cuda(device).check_device_error()``
+reads (it waits for the device: once per some steps, not per call).
 """
 from __future__ import annotations
 
