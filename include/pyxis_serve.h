@@ -102,7 +102,14 @@ int pyxis_cuda_qk_norm_rope_dev(pyxis_cuda_ctx *ctx, const pyxis_qk_norm_rope_ar
  *   max_context  a bound of context_len that only plans the split of the keys over the GPU
  * out = softmax(scale * q . k) v; a row that attends to nothing is zero, rows outside
  * [q_start[0], q_start[n_seq]) are left as they are.  Non-finite keys or values at positions that
- * a row does not attend to do not reach it.  kv is one layer's pages, dtype that of q and out.
+ * a row does not attend to do not reach it; an infinite value that it attends to is infinite in its
+ * column of the output, a key whose score is -inf has no weight.
+ * Scores, weights and sums are f32.  bf16 pages: products are exact, weights enter P V in f32 or as two
+ * bf16 terms (off by 2^-16 at most), and the output is rounded to bf16 once.  f32 pages: up to 8 rows
+ * (nodes x query heads of a kv head) products are f32, above that two terms per operand leave 2^-21 of a
+ * product, and from 17 rows on an element below 2^-12 of the largest of its group (a query row, a kv
+ * head's 64 context positions) keeps 2^-34 of that largest instead.  How work is split, and with it the
+ * last bits, depends on the batch; the same call gives the same bits.  kv is one layer's pages, dtype that of q and out.
  * The split's partial sums need `workspace` of pyxis_cuda_tree_attention_workspace_size() bytes,
  * 256-byte aligned; NULL uses the context's, under the rules of pyxis_cuda_matmul_dev's. */
 typedef struct {

@@ -25,7 +25,7 @@
 //
 // Latency bounds it: a row is read once (0.6 MB: 0.1 us of the memory's time), but maximum, histogram,
 // gather and narrowing follow one another, with a cluster barrier between.  Measured, 151936 tokens: one
-// f32 row with top-p 23 us, 64 bf16 rows with top-k, top-p and min-p 16.4 us, with top-p alone 77 us
+// f32 row with top-p 23 us, 64 bf16 rows with top-k, top-p and min-p 16.4 us, with top-p alone 78 us
 // (the weights' exponentials and the histograms' shared-memory atomics).
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>

@@ -873,17 +873,17 @@ TreePlan plan_tree_attention(const pyxis_tree_attention_args &a, const pyxis_kv_
     const long long keys = std::max<long long>(1, std::min<long long>(std::min<long long>(a.max_context, 1ll << 40) + a.max_tree,
                                                                      (long long)a.table_width * kv.page_size));
     // bf16: few rows over few keys are done on the CUDA cores before the tensor-core kernel has started
-    // its pipeline.  Measured (16 query heads, 8 kv heads of 128): 2 rows, one sequence of 152 positions 8 us
-    // against 15, 16 of 600 16 against 24, of 2303 41 against 40, 64 of 600 45 against 49, of 1200 73 against
-    // 67; 4 rows, 16 of 600 19 against 25, of 1200 32 against 29; 8 rows, 4 of 600 21 against 18, 16 of 600 30
-    // against 23, of 300 18 against 21.
+    // its pipeline.  Measured (16 query heads, 8 kv heads of 128): 2 rows, one sequence of 152 positions 7 us
+    // against 14, 16 of 600 12 against 21, of 2303 40 against 38, 64 of 600 43 against 49, of 1200 72 against
+    // 67; 4 rows, 16 of 600 15 against 22, of 1200 30 against 28; 8 rows, 4 of 600 18 against 17, 16 of 600 26
+    // against 21, of 300 17 against 19.
     // f32: the tcgen05 kernel pays the same for 1 row as for 128 (three products of 128 rows and the
     // conversion of every key), the mma.sync kernel for each tile of 16.  16 sequences of 2303 positions:
-    // 16 rows 89 us against the tcgen05 kernel's 103, 32 rows 160 against 103, 64 rows 310 against 107;
-    // one sequence of 152: 16 rows 18 against 24, 128 rows 31 against 28.  Trees over next to no context are
-    // done before its pipeline has started: 4 sequences of 86 keys and 48 rows 23 against 25, 16 of 17 keys
-    // and 128 rows of one kv head 21 against 35; 4 of 224 keys 29 against 27, and 512 CTAs' worth, 16 of 65
-    // keys and 128 rows, 55 against 36.
+    // 16 rows 88 us against the tcgen05 kernel's 104, 32 rows 160 against 103, 64 rows 270 against 105;
+    // one sequence of 152: 16 rows 15 against 23, 128 rows 29 against 27.  Trees over next to no context are
+    // done before its pipeline has started: 4 sequences of 86 keys and 48 rows 21 against 23, 16 of 17 keys
+    // and 128 rows of one kv head 20 against 33; 4 of 224 keys 28 against 25, and 512 CTAs' worth, 16 of 65
+    // keys and 128 rows, 58 against 36.
     const bool f32 = kv.dtype == PYXIS_DTYPE_F32;
     const bool brief = keys <= 128 && (long long)a.n_seq * kv.n_kv_heads * ((rows + 31) / 32) <= num_sms;
     t.tensor = f32 ? tree_attention_tc32_supported(a, kv) && rows > 16 && !brief

@@ -26,12 +26,17 @@
 // P is two bf16 terms, hi = bf16(p) and lo = bf16(p - hi), which leaves 2^-16 of each weight at most: O is
 // f32 until its one rounding, as in the forms on the CUDA cores.  The tensor cores have the time for the
 // second product (1600 of the 2800 cycles that a tile takes to arrive), and TMEM the room: both terms lie
-// over the scores.
+// over the scores.  The softmax warps pay for it: with one term, off by 2^-9 of a weight, the two cases below
+// took 103 and 38 us where they take 110 and 39 (2.3e-3 from 64 bits in place of 1.7e-3, relative l2).  O
+// adds up in TMEM, where sums are cut off: 3e-4 of the sum over 64000 positions of one CTA, an eighth of
+// the output's rounding.
 //
-// Measured (16 query and 8 kv heads of 128): one sequence of 131000 positions and 64 nodes 107 us, 5.0 TB/s
-// (a floor of 83 us), 16 sequences of 2303 positions and 16 nodes 40 us (20): the tiles pass at HBM's rate;
-// the rest is the dealing and the first tiles' latency (about 4 us), the last tile's (3 us) and the join
-// of the shared units (2 to 7 us).
+// Measured (16 query and 8 kv heads of 128): one sequence of 131000 positions and 64 nodes 107 to 124 us, 4.3
+// to 5.0 TB/s (a floor of 83 us), 16 sequences of 2303 positions 39 to 45 us with 16 nodes and 38 to 41 with
+// one (20 and 21), 64 of them with one node 103 to 121 (84): the tiles pass at HBM's rate; the rest is the
+// dealing and the first tiles' latency (about 4 us), the last tile's (3 us) and the join of the shared units
+// (2 to 7 us).  The softmax warps have all 168 registers that a thread can have: for heads of 128 they spill
+// 64 bytes.
 #include <algorithm>
 #include <atomic>
 

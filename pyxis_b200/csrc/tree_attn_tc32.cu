@@ -20,7 +20,12 @@
 // instruction cache's sake, 106 -> 100: a floor of 41 us at the memory's rate.  Tiles with drafts, which
 // some rows see and others do not, must not let one draft cost another one bits: a scale for each of
 // their keys, and values out of the scale's range added in f32 (100 -> 103 us).  58 sequences of 1731
-// positions and 64 nodes 298 us (121).
+// positions and 64 nodes 301 us (121).  The softmax warps keep a row's scores and its half of O in 160 registers:
+// for heads of 128 they spill 256 bytes.
+//
+// Infinities: an infinite element has no second term (x - hi is NaN).  The converters mark a tile whose keys hold
+// one, and its scores that come out NaN are taken again in f32; a column of O that is not finite is summed again
+// from the values themselves.
 //
 // One CTA per SM takes an equal share of all units' tiles (tree_attn_tc.cuh).  Warps:
 //   0       producer: a tile's pages by TMA (one box per page) into a ring of f32 tiles, in the order
