@@ -755,18 +755,25 @@ __global__ void __launch_bounds__(MmaCfg<T, HD, MT, PER>::kWarps * 32, PER) tree
             l += __shfl_xor_sync(0xffffffffu, l, 2);
             if (c == 0) sml[(warp * RT + r) * 2] = m_run[mt][h], sml[(warp * RT + r) * 2 + 1] = l;
         }
-    if (isnan(odd)) {
+    if (__any_sync(0xffffffffu, isnan(odd))) {
         // A weight's second term may be zero, and an infinite value has none: a sum over values that are not
-        // finite is taken from the values of this warp's blocks (this lane's columns, read back: acc stays in
-        // registers).
+        // finite is taken from the values of this warp's blocks, a row per lane (one whose weights are NaN is NaN).
+        __syncwarp();
+        constexpr int kC = HD / 32;  // columns per lane
+        float4 bad = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (b = b0 + warp; b < b1; b += kWarps) {
+            const float4 x = odd_columns<T, kC>(p, sh, seq, kvh, 0, b * kMmaKeys, (b + 1) * kMmaKeys);
+            bad.x += x.x, bad.y += x.y, bad.z += x.z, bad.w += x.w;
+        }
+        const bool mine = lane < min(rows, RT) && isfinite(sml[(warp * RT + lane) * 2 + 1]);
 #pragma unroll 1
-        for (int n = 0; n < MT * 2 * HD / 4; ++n) {
-            const int r = n / (HD / 4) * 8 + g, i = n % (HD / 4), d = 32 * (i >> 3) + 4 * (2 * c + (i & 1)) + (i >> 1 & 3);
-            if (isfinite(so[r * HD + d])) continue;
-            float x = 0.f;
+        for (int d = 0; d < HD; ++d) {
+            const int e = d % kC;
+            float x = __shfl_sync(0xffffffffu, e == 0 ? bad.x : e == 1 ? bad.y : e == 2 ? bad.z : bad.w, d / kC);
+            if (!mine || isfinite(so[lane * HD + d])) continue;
             for (b = b0 + warp; b < b1; b += kWarps)
-                x += odd_values<T>(p, sh, seq, kvh, d, smask[r], b * kMmaKeys, (b + 1) * kMmaKeys);
-            if (x != 0.f) so[r * HD + d] = x;
+                x += odd_drafts<T>(p, sh, seq, kvh, d, smask[lane], b * kMmaKeys, (b + 1) * kMmaKeys);
+            if (x != 0.f) so[lane * HD + d] = x;
         }
     }
     __syncthreads();

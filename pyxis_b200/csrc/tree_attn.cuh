@@ -43,17 +43,44 @@ PYXIS_DEVINL SeqShape seq_shape(const TreeParams &p, int seq) {
 PYXIS_DEVINL void store(float *p, float x) { *p = x; }
 PYXIS_DEVINL void store(__nv_bfloat16 *p, float x) { *p = __float2bfloat16_rn(x); }
 
-// The sum of the values that are not finite in one column of a kv head (its address in page 0), over those of
-// the positions a .. b - 1 of a sequence with these pages that a row with this mask sees: infinite or NaN, or 0
-// if there are none.  Products in several terms need it (a weight's second term may be zero or negative, and an
-// infinite value has none); nothing else calls it, so it stays out of the kernels' registers.
+// Sums of values that are not finite (infinite or NaN; 0 if there are none).  Products in several terms need them
+// for the columns of their outputs that are not finite: a weight's second term may be zero or negative, and an
+// infinite value has none.  Nothing else calls them, so they stay out of the kernels' registers.
+//
+// In C columns per lane of a kv head (the first one's address in page 0), over the positions a .. b - 1 of a
+// sequence with these pages: one pass of the whole warp for all of its columns, as the others wait meanwhile.
+template <typename T, int C>
+__device__ __noinline__ float4 odd_columns(const char *columns, const int32_t *pages, int num_pages, int page_size,
+                                           long long page_stride, long long slot_stride, long long a, long long b) {
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    const T *mine = reinterpret_cast<const T *>(columns) + (threadIdx.x & 31) * C;
+#pragma unroll 4
+    for (; a < b; ++a) {
+        const long long i = a / page_size;
+        const int page = min(max(__ldg(pages + i), 0), num_pages - 1);
+        const T *v = reinterpret_cast<const T *>(reinterpret_cast<const char *>(mine) + page * page_stride +
+                                                 (a - i * page_size) * slot_stride);
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const float x = (float)v[c];
+            if (!isfinite(x)) sum[c] += x;
+        }
+    }
+    return make_float4(sum[0], sum[1], sum[2], sum[3]);
+}
+template <typename T, int C>
+PYXIS_DEVINL float4 odd_columns(const TreeParams &p, const SeqShape &sh, int seq, int kvh, int d, long long a, long long b) {
+    return odd_columns<T, C>(p.v + kvh * p.head_stride + d * (int)sizeof(T), p.block_table + seq * p.table_stride, p.num_pages,
+                             p.page_size, p.page_stride, p.slot_stride, a, min(b, sh.ctx));
+}
+// In one column, over those of the drafts at positions a .. b - 1 that a row with this mask sees.
 template <typename T>
-__device__ __noinline__ float odd_values(const char *column, const int32_t *pages, int num_pages, int page_size,
+__device__ __noinline__ float odd_drafts(const char *column, const int32_t *pages, int num_pages, int page_size,
                                          long long page_stride, long long slot_stride, long long ctx, unsigned long long mask,
                                          long long a, long long b) {
     float sum = 0.f;
     for (; a < b; ++a) {
-        if (a >= ctx && !((mask >> (a - ctx)) & 1)) continue;
+        if (!((mask >> (a - ctx)) & 1)) continue;
         const long long i = a / page_size;
         const int page = min(max(pages[i], 0), num_pages - 1);
         const float x = (float)*reinterpret_cast<const T *>(column + page * page_stride + (a - i * page_size) * slot_stride);
@@ -62,10 +89,10 @@ __device__ __noinline__ float odd_values(const char *column, const int32_t *page
     return sum;
 }
 template <typename T>
-PYXIS_DEVINL float odd_values(const TreeParams &p, const SeqShape &sh, int seq, int kvh, int d, unsigned long long mask, long long a,
+PYXIS_DEVINL float odd_drafts(const TreeParams &p, const SeqShape &sh, int seq, int kvh, int d, unsigned long long mask, long long a,
                               long long b) {
-    return odd_values<T>(p.v + kvh * p.head_stride + d * (int)sizeof(T), p.block_table + seq * p.table_stride, p.num_pages,
-                         p.page_size, p.page_stride, p.slot_stride, sh.ctx, mask, a, min(b, sh.total));
+    return odd_drafts<T>(p.v + kvh * p.head_stride + d * (int)sizeof(T), p.block_table + seq * p.table_stride, p.num_pages,
+                         p.page_size, p.page_stride, p.slot_stride, sh.ctx, mask, max(a, sh.ctx), min(b, sh.total));
 }
 // 0, or NaN if one of the values is not finite.
 template <int N>

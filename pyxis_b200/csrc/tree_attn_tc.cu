@@ -495,15 +495,20 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                             for (int i = 0; i < 32; ++i) part[(ch * 32 + i) * kRows] = o[i];
                         }
-                        if (row < rows && isnan(odd_mark(o))) {
-                            // a weight's second term may be zero or negative: a sum over values that are not
-                            // finite is taken from the values (read back: o stays in registers)
+                        // A weight's second term may be zero or negative: a sum over values that are not finite
+                        // is taken from the values (a row whose weights are NaN is NaN).
+                        const bool odd = row < rows && isfinite(l) && isnan(odd_mark(o));
+                        if (__any_sync(0xffffffffu, odd)) {
+                            const long long k0 = (long long)w.tb * kTile, k1 = (long long)w.te * kTile;
+                            const float bad_ctx = odd_columns<__nv_bfloat16, 1>(p, sh, w.seq, kvh, ch * 32, k0, k1).x;
 #pragma unroll 1
-                            for (int d = ch * 32; d < ch * 32 + 32; ++d) {
+                            for (int i = 0; i < 32; ++i) {
+                                const int d = ch * 32 + i;
+                                float x = __shfl_sync(0xffffffffu, bad_ctx, i);
                                 __nv_bfloat16 *y = reinterpret_cast<__nv_bfloat16 *>(dst) + d;
-                                if (isfinite(whole ? __bfloat162float(*y) : part[d * kRows])) continue;
-                                const float x = odd_values<__nv_bfloat16>(p, sh, w.seq, kvh, d, mask, (long long)w.tb * kTile,
-                                                                          (long long)w.te * kTile);
+                                // (read back: o stays in registers)
+                                if (!odd || isfinite(whole ? __bfloat162float(*y) : part[d * kRows])) continue;
+                                x += odd_drafts<__nv_bfloat16>(p, sh, w.seq, kvh, d, mask, k0, k1);
                                 if (x == 0.f) continue;
                                 if (whole)
                                     store(y, x);

@@ -21,7 +21,7 @@
 // some rows see and others do not, must not let one draft cost another one bits: a scale for each of
 // their keys, and values out of the scale's range added in f32 (100 -> 103 us).  58 sequences of 1731
 // positions and 64 nodes 301 us (121).  The softmax warps keep a row's scores and its half of O in 160 registers:
-// for heads of 128 they spill 256 bytes.
+// for heads of 128 they spill 264 bytes.
 //
 // Infinities: an infinite element has no second term (x - hi is NaN).  The converters mark a tile whose keys hold
 // one, and its scores that come out NaN are taken again in f32; a column of O that is not finite is summed again
@@ -634,6 +634,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                     named_bar(1 + quad, 64);
                     l += rd[(1 - half) * kRows + row];
                 }
+                bool odd = false;  // some of the row's sums are not finite; where they have been written
+                char *first = nullptr;
+                int step = 0;
                 if (active && ok && row < rows) {
                     const bool whole = w.whole();
                     const int t = (r0 + row) / p.group, h = kvh * p.group + (r0 + row) % p.group;
@@ -675,17 +678,23 @@ __global__ void __launch_bounds__(kThreads, 1)
                             a.shared[c] = Shared{(int)(((end + 1) * g + total - 1) / total) - 1, sh.row0, kvh, r0, rows};
                         }
                     }
-                    if (isnan(odd_mark(acc))) {
-                        // an infinite value has no second term, and a weight's may be zero or negative: a sum over
-                        // values that are not finite is taken from the values (read back: acc stays in registers)
+                    odd = isfinite(l) && isnan(odd_mark(acc));
+                    first = whole ? dst : reinterpret_cast<char *>(part);
+                    step = whole ? 4 : kRows * 4;
+                }
+                if (__any_sync(0xffffffffu, odd)) {
+                    // An infinite value has no second term, and a weight's may be zero or negative: a sum over values
+                    // that are not finite is taken from the values (a row whose weights are NaN is NaN).
+                    constexpr int kC = kOH / 32;  // columns per lane
+                    const long long c0 = (long long)w.tb * kTile, c1 = (long long)w.te * kTile;
+                    const float4 bad = odd_columns<float, kC>(p, sh, w.seq, kvh, half * kOH, c0, c1);
 #pragma unroll 1
-                        for (int i = 0; i < kOH; ++i) {
-                            float *y = whole ? reinterpret_cast<float *>(dst) + i : part + i * kRows;
-                            if (isfinite(*y)) continue;
-                            const float x = odd_values<float>(p, sh, w.seq, kvh, half * kOH + i, mask, (long long)w.tb * kTile,
-                                                              (long long)w.te * kTile);
-                            if (x != 0.f) *y = x;
-                        }
+                    for (int i = 0; i < kOH; ++i) {
+                        float x = __shfl_sync(0xffffffffu, i % kC ? bad.y : bad.x, i / kC);
+                        float *y = reinterpret_cast<float *>(first + i * step);  // (read back: acc stays in registers)
+                        if (!odd || isfinite(*y)) continue;
+                        x += odd_drafts<float>(p, sh, w.seq, kvh, half * kOH + i, mask, c0, c1);
+                        if (x != 0.f) *y = x;
                     }
                 }
                 __syncwarp();

@@ -307,3 +307,33 @@ def test_a_captured_call_keeps_its_workspace_when_the_context_grows():
         torch.cuda.synchronize()
         assert torch.equal(out, want)
     assert (junk == 255).all()
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("nodes", [6, 24])
+def test_pages_without_a_finite_number_in_long_contexts(dt, nodes):
+    """Sequences that fill a CTA each, whose last context page holds nothing finite: no wait runs out while the
+    columns are taken from the values."""
+    n_seq, ctx, hd, page = 150, 50000, 128, 64
+    per = -(-(ctx + nodes) // page)
+    k = torch.randn(n_seq * per, page, 1, hd, device="cuda", dtype=dt)
+    v = torch.randn(n_seq * per, page, 1, hd, device="cuda", dtype=dt)
+    table = torch.arange(n_seq * per, dtype=torch.int32, device="cuda").view(n_seq, per)
+    last = table[:, (ctx - 1) // page].long()
+    fill = v[last].clone()
+    q = torch.randn(n_seq * nodes, 2, hd, device="cuda", dtype=dt)
+    start = torch.arange(n_seq + 1, dtype=torch.int32, device="cuda") * nodes
+    lens = torch.full((n_seq,), ctx, dtype=torch.int32, device="cuda")
+
+    def run():
+        return px.tree_attention_dev(q, k, v, table, lens, start, max_tree=nodes, max_context=ctx)
+
+    v[last] = math.inf
+    assert (run() == math.inf).all()
+    v[last] = math.nan
+    assert run().isnan().all()
+    v[last] = fill
+    k[last] = math.nan
+    assert run().isnan().all()
+    k[last] = math.inf  # inf times both signs of q
+    assert run().isnan().all()
